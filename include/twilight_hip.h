@@ -70,6 +70,8 @@ enum twl_status {
 };
 
 enum twl_dtype { TWL_F16 = 0, TWL_BF16 = 1, TWL_F32 = 2 };
+/* formats of 8-bit K / V pages, beside the element types of twl_dtype */
+enum twl_kv_format { TWL_I8 = 3, TWL_E4M3 = 4 };
 
 /* how the top-p bisection initialises its upper bound */
 enum twl_top_p_high {
@@ -87,7 +89,7 @@ enum twl_top_p_high {
 const char* twl_strerror(int status);
 /* ABI version of this header; bumps when a signature changes. twl_abi_version() returns the
  * version the library was built with: a caller compares the two before anything else. */
-#define TWL_ABI_VERSION 10
+#define TWL_ABI_VERSION 11
 int twl_abi_version(void);
 /* Number of HIP devices visible, or a negative twl_status. */
 int twl_device_count(void);
@@ -518,6 +520,104 @@ int twl_qk_int8_lse(const int8_t* q, const int8_t* k, const float* q_scale, cons
                     uint32_t qo_len, uint32_t kv_len, uint32_t head_dim, int64_t sq_b,
                     int64_t sq_h, int64_t sq_n, int64_t sk_b, int64_t sk_h, int64_t sk_n,
                     void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * K / V held in 8 bits. No counterpart in the reference (its INT4 K, twilight/pyimpl/quantize.py:
+ * 4-13, stands beside a 16-bit cache and serves the estimator; here the cache itself is 8-bit).
+ * Pages k_cache / v_cache hold codes of one byte, addressed with element strides (page, token, kv
+ * head; channels contiguous); k_scale / v_scale hold one fp32 scale per (page, token, kv head) with
+ * strides of their own. format = TWL_I8 (T = 127) or TWL_E4M3 (T = 448, no infinities). For the 128
+ * channels x of a token and kv head
+ *   scale = max(max|x| / T, 2^-126)   code = round_to_nearest_even(x / scale)   value = code * scale
+ * in fp32 with IEEE division. A row with an infinity or a NaN gets scale NaN and codes 0.
+ * token_indptr int32 [batch + 1]: rows token_indptr[b] .. token_indptr[b + 1] of the dense tensors are
+ * the LAST tokens of request b as the page table counts them (the table already includes tokens
+ * that are being appended, so a call may be repeated). Rows of the dense tensors that no request
+ * names (from token_indptr[batch] on) are neither read into the cache nor written. A row whose
+ * request holds fewer tokens than token_indptr gives it, or whose page id is not below num_pages,
+ * is skipped by the append and read as zeros. Appending: a page that is written must belong to one
+ * request only.
+ *   twl_kv_quant_append  k_new / v_new [tokens, kv heads, 128] in dtype (TWL_F16 / TWL_BF16), element
+ *                        strides (token, head) that are multiples of 8
+ *   twl_kv_quant_read    k_out / v_out [tokens, kv heads, 128] contiguous, TWL_F16 / TWL_BF16 / TWL_F32
+ * ------------------------------------------------------------------------------------------- */
+int twl_kv_quant_append(const void* k_new, const void* v_new, int dtype, uint64_t new_token_stride,
+                        uint64_t new_head_stride, const int32_t* token_indptr, uint32_t tokens,
+                        void* k_cache, void* v_cache, int format, uint64_t page_stride,
+                        uint64_t token_stride, uint64_t head_stride, float* k_scale,
+                        float* v_scale, uint64_t scale_page_stride, uint64_t scale_token_stride,
+                        uint64_t scale_head_stride, uint32_t num_pages,
+                        const int32_t* kv_page_indices, const int32_t* kv_page_indptr,
+                        const int32_t* kv_last_page_len, uint32_t batch, uint32_t num_kv_heads,
+                        void* stream);
+int twl_kv_quant_read(void* k_out, void* v_out, int dtype, const int32_t* token_indptr,
+                      uint32_t tokens, const void* k_cache, const void* v_cache, int format,
+                      uint64_t page_stride, uint64_t token_stride, uint64_t head_stride,
+                      const float* k_scale, const float* v_scale, uint64_t scale_page_stride,
+                      uint64_t scale_token_stride, uint64_t scale_head_stride, uint32_t num_pages,
+                      const int32_t* kv_page_indices, const int32_t* kv_page_indptr,
+                      const int32_t* kv_last_page_len, uint32_t batch, uint32_t num_kv_heads,
+                      void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Dense paged decode attention over 16-bit or 8-bit pages, for requests that may share a prefix.
+ * Replaces: the dense decode of twilight/pyimpl/attention.py:199-201 (the reference repeats K / V per
+ * q head, attention.py:124-126, and has neither shared prefixes nor an 8-bit cache).
+ * Groups (groups > 0): requests group_indptr[g] .. group_indptr[g + 1] (int32 [groups + 1], ascending)
+ * see the tokens of prefix list g, a page list of the same cache given by prefix_page_indices /
+ * prefix_page_indptr / prefix_last_page_len, and then their own pages kv_page_*; a request outside
+ * every group sees its own pages only. groups == 0: no prefix, the prefix arguments are ignored.
+ *   out[b, h] = softmax(sm_scale * q[b, h] . K) V in dtype;  lse_out (nullable) float [batch, q heads]
+ * A request that sees no token gives a zero row and lse -inf.
+ * format: dtype itself for 16-bit pages, or TWL_I8 / TWL_E4M3 with k_scale / v_scale (see
+ * twl_kv_quant_append). Any number of q heads per kv head. max_prefix_tokens, max_group_size and
+ * max_tokens size the launch: prefix tokens beyond the first are not attended to, members of a group
+ * beyond the second do not see the prefix, own tokens beyond the third are not attended to
+ * (each <= 2^24, groups <= batch, max_group_size <= batch, batch * q heads <= 65535). A page id
+ * that is not below num_pages is read as page num_pages - 1.
+ * Strides in elements, multiples of 8 (16-bit pages) or 16 (8-bit); token stride <= 2^24.
+ * The softmax weights are rounded to the 16-bit type of the V product (dtype, or fp16 over 8-bit
+ * pages); their sum is not. workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means that the
+ * call needs none), 16-byte aligned, no initial contents required;
+ * calls that share it must not overlap in time.
+ * ------------------------------------------------------------------------------------------- */
+uint64_t twl_prefix_attn_workspace_bytes(uint32_t batch, uint32_t num_q_heads,
+                                         uint32_t num_kv_heads, uint32_t groups,
+                                         uint32_t max_prefix_tokens, uint32_t max_group_size,
+                                         uint32_t max_tokens);
+int twl_prefix_attn(const void* q, void* out, int dtype, const void* k_cache, const void* v_cache,
+                    int format, uint64_t page_stride, uint64_t token_stride, uint64_t head_stride,
+                    const float* k_scale, const float* v_scale, uint64_t scale_page_stride,
+                    uint64_t scale_token_stride, uint64_t scale_head_stride, uint32_t num_pages,
+                    const int32_t* prefix_page_indices, const int32_t* prefix_page_indptr,
+                    const int32_t* prefix_last_page_len, const int32_t* group_indptr,
+                    uint32_t groups, uint32_t max_prefix_tokens, uint32_t max_group_size,
+                    const int32_t* kv_page_indices, const int32_t* kv_page_indptr,
+                    const int32_t* kv_last_page_len, uint32_t max_tokens, uint32_t batch,
+                    uint32_t num_q_heads, uint32_t num_kv_heads, float sm_scale, float* lse_out,
+                    void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The next token of every row of logits, drawn with one given uniform number per row. The
+ * reference leaves sampling to its callers; its top-p kernel (csrc/include/sampling.cuh:119-231)
+ * prunes attention weights.
+ * logits [rows, vocab] in dtype (TWL_F16 / TWL_BF16 / TWL_F32), row_stride elements from row to row;
+ * vocab <= 2^18. u float [rows] in [0, 1). Every filter is a scalar, or an array [rows] (nullable)
+ * that overrides it. With x* the largest logit of the row and w = exp((x - x*) / temperature),
+ * tokens ranked by logit (the larger first, equal ones by index):
+ *   top_k > 0: ranks below top_k stay;  top_p < 1: of those, a rank stays if the w of the ranks
+ *   before it sum to less than top_p times the sum of all;  min_p > 0: w >= min_p stays.
+ *   The best rank always stays. tokens[r] int64 = the first token in vocabulary order whose running sum of
+ *   kept w exceeds u times the sum of all kept w.
+ * temperature <= 0 (or NaN in an array): the best token. -inf and NaN logits are never drawn; a row
+ * with nothing else gives -1. w is computed in 64 bits and held as a multiple of 2^-45; sums are
+ * exact, so the answer does not depend on their order.
+ * ------------------------------------------------------------------------------------------- */
+int twl_sample_tokens(const void* logits, int dtype, uint64_t row_stride, uint32_t rows,
+                      uint32_t vocab, const float* u, const float* temperature_arr,
+                      float temperature, const int32_t* top_k_arr, int32_t top_k,
+                      const float* top_p_arr, float top_p, const float* min_p_arr, float min_p,
+                      int64_t* tokens, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * The whole decode layer on one stream: quest select -> INT4 GEMV -> softmax + top-p -> sparse

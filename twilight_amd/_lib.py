@@ -14,7 +14,8 @@ from .build import LIB_PATH
 
 TWL_OK = 0
 TWL_F16, TWL_BF16, TWL_F32 = 0, 1, 2
-ABI_VERSION = 10  # TWL_ABI_VERSION of include/twilight_hip.h, checked when the library is loaded
+TWL_I8, TWL_E4M3 = 3, 4   # formats of 8-bit K / V pages
+ABI_VERSION = 11  # TWL_ABI_VERSION of include/twilight_hip.h, checked when the library is loaded
 TWL_HIGH_FIRST, TWL_HIGH_MAX = 0, 1
 PAGE = 16
 HEAD_DIM = 128
@@ -33,6 +34,8 @@ EXPORTS = (
     "twl_group_attn_workspace_bytes",
     "twl_group_union", "twl_rope_qk", "twl_quest_select",
     "twl_quest_page_scores", "twl_quest_topk_pages", "twl_kv_shadow_build", "twl_kv_append", "twl_meta_planes_build", "twl_quest_page_scores_planes", "twl_dequant_int4",
+    "twl_kv_quant_append", "twl_kv_quant_read", "twl_prefix_attn_workspace_bytes", "twl_prefix_attn",
+    "twl_sample_tokens",
     "twl_decode_layer", "twl_get_label_tensor", "twl_bgemv_int8", "twl_qk_int8_lse",
 )
 
@@ -125,6 +128,16 @@ def lib() -> ctypes.CDLL:
     L.twl_quest_topk_pages.argtypes = [vp, u32, vp, u32, u32, u32, u32, vp, u32, vp, vp]
     L.twl_kv_shadow_build.argtypes = [vp, i32, u64, u64, u64, vp, vp, u32, u32, vp, vp, vp]
     L.twl_dequant_int4.argtypes = [vp, u32, vp, vp]
+    L.twl_kv_quant_append.argtypes = [vp, vp, i32, u64, u64, vp, u32, vp, vp, i32, u64, u64, u64, vp, vp,
+                                      u64, u64, u64, u32, vp, vp, vp, u32, u32, vp]
+    L.twl_kv_quant_read.argtypes = [vp, vp, i32, vp, u32, vp, vp, i32, u64, u64, u64, vp, vp, u64, u64,
+                                    u64, u32, vp, vp, vp, u32, u32, vp]
+    L.twl_prefix_attn_workspace_bytes.argtypes = [u32] * 7
+    L.twl_prefix_attn.argtypes = [vp, vp, i32, vp, vp, i32, u64, u64, u64, vp, vp, u64, u64, u64, u32, vp,
+                                  vp, vp, vp, u32, u32, u32, vp, vp, vp, u32, u32, u32, u32, f32, vp, vp,
+                                  u64, vp]
+    L.twl_sample_tokens.argtypes = [vp, i32, u64, u32, u32, vp, vp, f32, vp, c_int32, vp, f32, vp, f32, vp,
+                                    vp]
     L.twl_decode_layer.argtypes = [POINTER(LayerArgs), vp]
     L.twl_get_label_tensor.argtypes = [vp, vp, vp, u32, u32, u32, u32] + [c_int64] * 8 + [vp]
     L.twl_bgemv_int8.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32] + [c_int64] * 11 + [vp]
@@ -138,10 +151,11 @@ def lib() -> ctypes.CDLL:
                                   i64, i64, i64, vp]
     for name in EXPORTS:
         if name not in ("twl_strerror", "twl_sparse_attn_workspace_bytes",
-                        "twl_group_attn_workspace_bytes"):
+                        "twl_group_attn_workspace_bytes", "twl_prefix_attn_workspace_bytes"):
             getattr(L, name).restype = c_int
     L.twl_sparse_attn_workspace_bytes.restype = c_uint64
     L.twl_group_attn_workspace_bytes.restype = c_uint64
+    L.twl_prefix_attn_workspace_bytes.restype = c_uint64
     _lib = L
     return L
 

@@ -1,0 +1,722 @@
+// Paged decode attention over 16-bit or 8-bit pages, for requests in groups that share a prefix.
+//
+// Request b of group g sees the tokens of the group's prefix pages and then its own:
+//     out[b, h] = softmax(sm_scale * q[b, h] . K) V        lse[b, h] = log sum exp(logit)
+// A softmax over a set of tokens is the merge of softmaxes over its parts: every part leaves
+// (m, l, acc) = (running maximum, sum of exp2(s - m), sum of exp2(s - m) V) of its tokens, and parts
+// are joined by rescaling to the common maximum. So the prefix is read once per group and kv head,
+// with the queries of all its requests as the columns of one matrix product, and the requests' own
+// tokens are ordinary parts beside it.
+//
+// One wavefront works on tiles of 32 tokens (two pages) and NQ sets of 16 query rows, without LDS
+// and without moving anything between lanes. With n = lane % 16, kb = lane / 16:
+//   S^T = K Q^T   A operand: token n of a page, 8 channels per lane; B operand: query n. A lane of
+//                 the result holds query n's logits of tokens 4 kb + i of either page.
+//   O^T += V^T P^T   The order of the 32 tokens inside the product is free, so k-slot (kb, i) is
+//                 given to exactly the eight tokens whose weights the lane already has: the weights
+//                 are the B operand as they stand. The A operand wants the same eight tokens of
+//                 one channel: a lane loads 8 channels 8 n .. 8 n + 7 of its eight tokens (a row of
+//                 16 lanes covers a token's 128 channels) and transposes 8 x 8 in registers; product
+//                 j takes channel 8 n + j of every lane.
+// A lane of O^T then holds 32 consecutive channels of ONE query, so maxima, sums and rescaling are
+// per-lane scalars. The maximum is only raised (and the accumulators rescaled) when a logit exceeds
+// it by more than 8 in base 2: weights stay below 2^8, exact in what fp32 and the 16-bit operands
+// can hold, and most tiles need no reduction across lanes at all.
+//
+// 8-bit pages run on fp16 products (codes are exact in fp16). The scale of K multiplies the logit.
+// The scale of V joins the weight, relative to a running power of two that bounds the V scales seen
+// (weight * scale * 2^-e < 2^9 fits fp16 whatever the scales are); a bf16 query is first brought
+// into fp16's range by a power of two of its own.
+//
+// The weights are rounded to the product's 16-bit type (half a step, relative to each weight); the
+// sum l takes them before that rounding, in fp32.
+#include "twl_common.h"
+
+namespace twl {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kPaThreads = 256;
+constexpr int kPaWaves = kPaThreads / kWave;
+constexpr int kPaTile = 32;                 // tokens of one step of a wavefront
+constexpr float kPaNoMax = -3.0e38f;        // running maximum before the first token
+constexpr float kPaSlack = 8.0f;            // how far a logit may exceed it, in base 2
+constexpr float kLn2 = 0.693147180559945309f;
+
+struct PrefixAttnArgs {
+  const uint16_t* q;                        // [batch, num_q_heads, 128]
+  void* out;
+  float* lse;
+  const uint8_t* k;
+  const uint8_t* v;
+  uint64_t page_bytes, head_bytes;
+  uint32_t token_bytes;
+  const float* ks;                          // 8-bit pages: one scale per (page, token, kv head)
+  const float* vs;
+  uint64_t scale_page, scale_head;
+  uint32_t scale_token;
+  uint32_t num_pages;
+  const int32_t *p_ids, *p_ptr, *p_last, *g_ptr;   // prefix tables, members of every group
+  const int32_t *ids, *ptr, *last;                 // the requests' own pages
+  uint32_t batch, num_q_heads, num_kv_heads, G, groups;
+  uint32_t max_prefix, max_group, max_tokens;
+  uint32_t p_chunk, p_chunks, p_tiles;      // prefix: tokens per part, parts, row tiles per group
+  uint32_t chunk, chunks, tiles;            // own tokens: the same
+  uint32_t p_blocks;                        // workgroups of the prefix parts, first in the grid
+  float scale_log2;
+  float* acc;                               // [rows, parts, 128]
+  f32x2* ml;                                // [rows, parts]
+};
+
+__device__ __forceinline__ float max_over_kb(float x) {
+  const uint32_t u = as_u32(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t y = as_u32(fmaxf(as_f32(a[0]), as_f32(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(as_f32(b[0]), as_f32(b[1]));
+}
+__device__ __forceinline__ float sum_over_kb(float x) {
+  const uint32_t u = as_u32(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t y = as_u32(as_f32(a[0]) + as_f32(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return as_f32(b[0]) + as_f32(b[1]);
+}
+
+template <int MT>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if (MT == TWL_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a),
+                                                  __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+template <int MT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  return f32_to_bits16<MT>(x) | (f32_to_bits16<MT>(y) << 16);
+}
+
+// four 8-bit codes -> four fp16 values
+template <int KV>
+__device__ __forceinline__ u32x2 widen4(uint32_t w) {
+  if (KV == TWL_E4M3) {
+    const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false);
+    const half2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true);
+    return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+  }
+  // 0x6400 | u is the fp16 number 1024 + u; u = code + 128
+  const uint32_t u = w ^ 0x80808080u;
+  const half2_t bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+  const half2_t a = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+  const half2_t b = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+  return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+
+template <bool NT, class T>
+__device__ __forceinline__ T load_kv(const uint8_t* p) {
+  return NT ? __builtin_nontemporal_load((const T*)p) : *(const T*)p;
+}
+
+// Tokens of a page list, bounded by what the caller sized the launch for.
+__device__ __forceinline__ int list_len(const int32_t* ptr, const int32_t* last, uint32_t i, uint32_t bound) {
+  const int64_t np = (int64_t)ptr[i + 1] - ptr[i];
+  if (np <= 0) return 0;
+  return (int)min((np - 1) * TWL_PAGE + min(max(last[i], 0), TWL_PAGE), (int64_t)bound);
+}
+
+// Group of request b: the g with g_ptr[g] <= b < g_ptr[g + 1], or -1. By a whole wavefront.
+__device__ __forceinline__ int group_of(const PrefixAttnArgs& a, uint32_t b) {
+  int g = -1;
+  for (uint32_t g0 = 0; g0 < a.groups; g0 += kWave) {
+    const uint32_t i = g0 + lane_id();
+    const bool in = i < a.groups && a.g_ptr[i] <= (int)b && (int)b < a.g_ptr[i + 1];
+    const uint64_t hit = __ballot(in);
+    if (hit) g = (int)g0 + __builtin_ctzll(hit);
+  }
+  return g;
+}
+
+// Four channels of a row's part: into the workspace, or, where a row has one part, the answer.
+template <int QT>
+__device__ __forceinline__ void put_row(const PrefixAttnArgs& a, int row, uint32_t part, uint32_t parts, int c,
+                                        f32x4 x, float m, float l) {
+  if (parts > 1) {
+    const size_t at = (size_t)row * parts + part;
+    *(f32x4*)(a.acc + at * TWL_HEAD_DIM + c) = x;
+    if (c == 0) a.ml[at] = f32x2{m, l};
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *(u32x2*)((uint16_t*)a.out + (size_t)row * TWL_HEAD_DIM + c) =
+      u32x2{pack2<QT>(x[0] * inv, x[1] * inv), pack2<QT>(x[2] * inv, x[3] * inv)};
+  if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : m * kLn2 + logf(l);
+}
+
+// One workgroup's part: tokens [begin, end) of a page list (first id at `ids`, `num_ids` of them)
+// for kv head kvh, and 16 * NQ * WR query rows. The four wavefronts are WR sets of rows times
+// 4 / WR interleaved sets of token tiles. row_of(local row) -> row of q / out, or -1.
+template <int QT, int KV, int NQ, int WR, class RowOf>
+__device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32_t* ids, int num_ids,
+                                            int begin, int end, uint32_t kvh, RowOf row_of,
+                                            uint32_t part, uint32_t parts) {
+  constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
+  constexpr int MT = k8 ? TWL_F16 : QT;
+  constexpr int WT = kPaWaves / WR;
+  constexpr int ROWS = 16 * NQ;
+  constexpr bool NT = WR == 1;              // several sets of rows read the pages again
+  constexpr int NKL = k8 ? 2 : 4;           // 16-byte loads of K per lane and page
+  const int lane = lane_id(), n = lane & 15, kb = lane >> 4;
+  const int wave = threadIdx.x / kWave, wr = wave / WT, wt = wave % WT;
+
+  // ---- queries: B operand of S^T, with the channel order of the K loads ------------------------
+  u32x4 qf[NQ][4];
+  float row_scale[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int row = row_of((wr * NQ + x) * 16 + n);
+    const uint16_t* src = a.q + (size_t)max(row, 0) * TWL_HEAD_DIM;
+    row_scale[x] = a.scale_log2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = k8 ? 64 * (j >> 1) + 16 * kb + 8 * (j & 1) : 32 * j + 8 * kb;
+      qf[x][j] = *(const u32x4*)(src + d);
+      if (row < 0) qf[x][j] = u32x4{0, 0, 0, 0};
+    }
+    if (k8 && QT == TWL_BF16) {
+      float f[4][8];
+      int top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unpack8<QT>(qf[x][j], f[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, as_i32(f[j][i]) & 0x7FFFFFFF);
+      }
+      top = as_i32(max_over_kb(as_f32(top)));
+      const int e = min(max((top >> 23) - 127, -126), 126);   // |q| < 2^(e + 1); NaN stays NaN
+      const float down = as_f32((127 - e) << 23);
+      row_scale[x] *= as_f32((127 + e) << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          qf[x][j][i] = pack2<TWL_F16>(f[j][2 * i] * down, f[j][2 * i + 1] * down);
+    }
+  }
+
+  f32x4 o[NQ][8];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = kPaNoMax;
+    l[x] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[x][j] = f32x4{0, 0, 0, 0};
+  }
+  int vexp = -126;                          // V scales so far are below 2^(vexp + 1)
+
+  const uint8_t* const kbase = a.k + kvh * a.head_bytes;
+  const uint8_t* const vbase = a.v + kvh * a.head_bytes;
+  const uint32_t koff = n * a.token_bytes + 16 * kb;
+  const uint32_t voff = 4 * kb * a.token_bytes + (k8 ? 8 : 16) * n;
+  const int tiles = (end - begin + kPaTile - 1) / kPaTile;
+  int window = -1, held = 0;
+  for (int t = wt; t < tiles; t += WT) {
+    const int tok0 = begin + t * kPaTile;
+    // page ids come 64 at a time, one per lane (32 tiles)
+    if ((t >> 5) != window) {
+      window = t >> 5;
+      const int at = min(begin / TWL_PAGE + window * kWave + lane, num_ids - 1);
+      held = (int)min((uint32_t)ids[at], a.num_pages - 1);
+    }
+    const uint32_t id0 = (uint32_t)__builtin_amdgcn_readlane(held, 2 * (t & 31));
+    const uint32_t id1 = (uint32_t)__builtin_amdgcn_readlane(held, 2 * (t & 31) + 1);
+    const uint8_t* kp[2] = {kbase + id0 * a.page_bytes, kbase + id1 * a.page_bytes};
+    const uint8_t* vp[2] = {vbase + id0 * a.page_bytes, vbase + id1 * a.page_bytes};
+
+    u32x4 kr[2][NKL];
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int j = 0; j < NKL; ++j) kr[p][j] = load_kv<NT, u32x4>(kp[p] + koff + 64 * j);
+    float ks[2][4], vs[2][4];
+    if (k8) {
+      const float* sk = a.ks + kvh * a.scale_head;
+      const float* sv = a.vs + kvh * a.scale_head;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const size_t so = (size_t)(p ? id1 : id0) * a.scale_page + 4 * kb * a.scale_token;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ks[p][i] = sk[so + i * a.scale_token];
+          vs[p][i] = sv[so + i * a.scale_token];
+        }
+      }
+    }
+    u32x4 vr[8];                            // eight tokens, 16 bytes (16-bit) or 8 (8-bit) each
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint8_t* p = vp[i >> 2] + voff + (i & 3) * a.token_bytes;
+      if (k8) {
+        const u32x2 w = load_kv<NT, u32x2>(p);
+        vr[i].x = w.x;
+        vr[i].y = w.y;
+      } else {
+        vr[i] = load_kv<NT, u32x4>(p);
+      }
+    }
+
+    // ---- logits --------------------------------------------------------------------------------
+    f32x4 s[NQ][2];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) s[x][p] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4 kf;
+        if (k8) {
+          const u32x2 lo = widen4<KV>(kr[p][j >> 1][2 * (j & 1)]);
+          const u32x2 hi = widen4<KV>(kr[p][j >> 1][2 * (j & 1) + 1]);
+          kf = u32x4{lo.x, lo.y, hi.x, hi.y};
+        } else {
+          kf = kr[p][j];
+        }
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) s[x][p] = mfma16<MT>(kf, qf[x][j], s[x][p]);
+      }
+
+    const bool cut = tok0 + kPaTile > end;
+    if (cut) {
+      // slots behind the last token hold whatever was there: their scales and V must not reach a
+      // product, not even times zero
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = tok0 + 16 * (i >> 2) + 4 * kb + (i & 3) < end;
+        if (k8) {
+          ks[i >> 2][i & 3] = in ? ks[i >> 2][i & 3] : 0.0f;
+          vs[i >> 2][i & 3] = in ? vs[i >> 2][i & 3] : 0.0f;
+        }
+        vr[i] = in ? vr[i] : u32x4{0, 0, 0, 0};
+      }
+    }
+    int rise = 0;                           // how far the V exponent has to go up
+    if (k8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(vs[i >> 2][i & 3]));
+      const int e = min((as_i32(top) >> 23) - 127, 126);
+      if (__any(e > vexp)) {
+        const int up = min((as_i32(max_over_kb(top)) >> 23) - 127, 126);
+        const int e1 = __builtin_amdgcn_readfirstlane(max(up, vexp));
+        rise = e1 - vexp;
+        vexp = e1;
+      }
+      const float down = as_f32((127 - vexp) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vs[i >> 2][i & 3] *= down;
+    }
+
+    u32x4 pf[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      float top = kPaNoMax;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float z = s[x][i >> 2][i & 3] * (k8 ? row_scale[x] * ks[i >> 2][i & 3] : row_scale[x]);
+        if (cut) z = tok0 + 16 * (i >> 2) + 4 * kb + (i & 3) < end ? z : -__builtin_inff();
+        s[x][i >> 2][i & 3] = z;
+        top = fmaxf(top, z);
+      }
+      if (__any(top > m[x] + kPaSlack)) {
+        const float up = fmaxf(m[x], max_over_kb(top));
+        const float alpha = __builtin_amdgcn_exp2f(m[x] - up);
+        m[x] = up;
+        l[x] *= alpha;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[x][j] *= alpha;
+      }
+      if (k8 && rise > 0) {
+        const float alpha = rise > 126 ? 0.0f : as_f32((127 - rise) << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[x][j] *= alpha;
+      }
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(s[x][i >> 2][i & 3] - m[x]);
+        l[x] += w[i];
+        if (k8) w[i] *= vs[i >> 2][i & 3];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[x][i] = pack2<MT>(w[2 * i], w[2 * i + 1]);
+    }
+
+    // ---- O^T += V^T P^T ------------------------------------------------------------------------
+    if (k8) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {         // channels 4 c .. 4 c + 3
+        uint32_t by_ch[2][4];               // [tokens 0-3 / 4-7][channel], one byte per token
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t r0 = vr[4 * h][c], r1 = vr[4 * h + 1][c], r2 = vr[4 * h + 2][c], r3 = vr[4 * h + 3][c];
+          const uint32_t a01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);   // r0.0 r1.0 r0.1 r1.1
+          const uint32_t b01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+          const uint32_t a23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
+          const uint32_t b23 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+          by_ch[h][0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+          by_ch[h][1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+          by_ch[h][2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+          by_ch[h][3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x2 lo = widen4<KV>(by_ch[0][j]), hi = widen4<KV>(by_ch[1][j]);
+          const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+          for (int x = 0; x < NQ; ++x) o[x][4 * c + j] = mfma16<MT>(vf, pf[x], o[x][4 * c + j]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {         // channels 2 c, 2 c + 1
+        u32x4 lo, hi;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c], vr[2 * i][c], 0x05040100u);
+          hi[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c], vr[2 * i][c], 0x07060302u);
+        }
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          o[x][2 * c] = mfma16<MT>(lo, pf[x], o[x][2 * c]);
+          o[x][2 * c + 1] = mfma16<MT>(hi, pf[x], o[x][2 * c + 1]);
+        }
+      }
+    }
+  }
+
+  // ---- join the wavefronts that share rows, and leave the part --------------------------------
+  const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
+  __shared__ float lds_m[kPaWaves][ROWS], lds_l[kPaWaves][ROWS];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    l[x] = sum_over_kb(l[x]);
+    if (kb == 0) {
+      lds_m[wave][16 * x + n] = m[x];
+      lds_l[wave][16 * x + n] = l[x];
+    }
+  }
+  __syncthreads();
+  float top[NQ], total[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    top[x] = kPaNoMax;
+#pragma unroll
+    for (int w = 0; w < WT; ++w) top[x] = fmaxf(top[x], lds_m[wr * WT + w][16 * x + n]);
+    total[x] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WT; ++w)
+      total[x] += lds_l[wr * WT + w][16 * x + n] * __builtin_amdgcn_exp2f(lds_m[wr * WT + w][16 * x + n] - top[x]);
+    const float f = __builtin_amdgcn_exp2f(m[x] - top[x]) * vfac;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[x][j] *= f;
+  }
+  if (WT == 1) {
+    // a lane holds 32 consecutive channels of its query's row
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      const int row = row_of((wr * NQ + x) * 16 + n);
+      if (row >= 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; j += 4)
+            put_row<QT>(a, row, part, parts, 32 * kb + 8 * i + j,
+                        f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]}, top[x], total[x]);
+      }
+    }
+    return;
+  }
+  __shared__ float lds_o[WT > 1 ? WR : 1][WT > 1 ? ROWS : 1][TWL_HEAD_DIM + 4];
+  for (int w = 0; w < WT; ++w) {
+    if (wt == w) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* p = &lds_o[wr][16 * x + n][32 * kb + 8 * i];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = w == 0 ? o[x][j][i] : p[j] + o[x][j][i];
+        }
+    }
+    __syncthreads();
+  }
+  // the maxima and sums of the joined rows
+  if (wt == 0 && kb == 0) {
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      lds_m[wr][16 * x + n] = top[x];
+      lds_l[wr][16 * x + n] = total[x];
+    }
+  }
+  __syncthreads();
+  // 32 threads write a row
+  for (int r = threadIdx.x >> 5; r < ROWS * WR; r += kPaThreads / 32) {
+    const int row = row_of(r);
+    if (row < 0) continue;
+    const int c = 4 * (threadIdx.x & 31);
+    put_row<QT>(a, row, part, parts, c, *(const f32x4*)&lds_o[r / ROWS][r % ROWS][c], lds_m[r / ROWS][r % ROWS],
+                lds_l[r / ROWS][r % ROWS]);
+  }
+}
+
+// Grid: the prefix parts (kv head, part, group, row tile), then the own parts (kv head, part,
+// request, row tile).
+template <int QT, int KV, int NQ, int WR>
+__global__ __launch_bounds__(kPaThreads) void prefix_attn_kernel(PrefixAttnArgs a) {
+  const uint32_t parts = a.p_chunks + a.chunks;
+  uint32_t id = blockIdx.x;
+  if (id < a.p_blocks) {
+    const uint32_t kvh = id % a.num_kv_heads;
+    id /= a.num_kv_heads;
+    const uint32_t c = id % a.p_chunks;
+    id /= a.p_chunks;
+    const uint32_t g = id % a.groups, tile = id / a.groups;
+    const int first = max(a.g_ptr[g], 0);
+    const int members = min(min((int)a.batch, a.g_ptr[g + 1]) - first, (int)a.max_group);
+    const int rows = members * (int)a.G, row0 = (int)(tile * 16 * NQ * WR);
+    const int len = list_len(a.p_ptr, a.p_last, g, a.max_prefix);
+    const int begin = (int)(c * a.p_chunk), end = min(len, begin + (int)a.p_chunk);
+    if (begin >= end || row0 >= rows) return;
+    auto row_of = [&](int r) {
+      const int lr = row0 + r;
+      if (lr >= rows) return -1;
+      const int b = lr / (int)a.G;
+      return (int)((first + b) * a.num_q_heads + kvh * a.G) + lr - b * (int)a.G;
+    };
+    attend_part<QT, KV, NQ, WR>(a, a.p_ids + a.p_ptr[g], a.p_ptr[g + 1] - a.p_ptr[g], begin, end,
+                                kvh, row_of, c, parts);
+  } else {
+    id -= a.p_blocks;
+    const uint32_t kvh = id % a.num_kv_heads;
+    id /= a.num_kv_heads;
+    const uint32_t c = id % a.chunks;
+    id /= a.chunks;
+    const uint32_t b = id % a.batch, tile = id / a.batch;
+    const int row0 = (int)(tile * 16);
+    const int len = list_len(a.ptr, a.last, b, a.max_tokens);
+    const int begin = (int)(c * a.chunk), end = min(len, begin + (int)a.chunk);
+    auto row_of = [&](int r) {
+      return row0 + r < (int)a.G ? (int)(b * a.num_q_heads + kvh * a.G) + row0 + r : -1;
+    };
+    if (begin >= end) {
+      // a row of one part has nobody else to say that it sees no token
+      if (parts == 1)
+        for (int r = threadIdx.x >> 5; r < 16; r += kPaThreads / 32)
+          if (row_of(r) >= 0)
+            put_row<QT>(a, row_of(r), 0, 1, 4 * (threadIdx.x & 31), f32x4{0, 0, 0, 0}, 0.0f, 0.0f);
+      return;
+    }
+    attend_part<QT, KV, 1, 1>(a, a.ids + a.ptr[b], a.ptr[b + 1] - a.ptr[b], begin, end, kvh, row_of,
+                              a.p_chunks + c, parts);
+  }
+}
+
+// Joins the parts of a row: one wavefront per row, two channels per lane. Which parts exist follows
+// from the lengths alone, so the workspace needs no initial contents. Where a row has at most one part
+// (a prefix of one part and no own tokens, or neither) it only writes the rows that see no token.
+template <int QT>
+__global__ __launch_bounds__(kPaThreads) void prefix_attn_merge_kernel(PrefixAttnArgs a) {
+  const uint32_t row = blockIdx.x * kPaWaves + threadIdx.x / kWave;
+  if (row >= a.batch * a.num_q_heads) return;
+  const uint32_t b = row / a.num_q_heads, parts = a.p_chunks + a.chunks;
+  const int lane = lane_id();
+  int np = 0;
+  if (a.p_chunks) {
+    const int g = group_of(a, b);
+    if (g >= 0 && (int)b - max(a.g_ptr[g], 0) < (int)a.max_group)
+      np = (list_len(a.p_ptr, a.p_last, g, a.max_prefix) + (int)a.p_chunk - 1) / (int)a.p_chunk;
+  }
+  const int no = a.chunks ? (list_len(a.ptr, a.last, b, a.max_tokens) + (int)a.chunk - 1) / (int)a.chunk : 0;
+  const int count = np + no;
+  if (parts <= 1 && count > 0) return;      // the part has written the row
+  const size_t at = (size_t)row * parts;
+  auto slot = [&](int i) { return i < np ? i : (int)a.p_chunks + i - np; };
+  float top = kPaNoMax;
+  for (int i = lane; i < count; i += kWave) top = fmaxf(top, a.ml[at + slot(i)].x);
+  top = wave_allreduce<OpMax>(top);
+  float l = 0.0f;
+  f32x2 acc = {0.0f, 0.0f};
+  for (int i0 = 0; i0 < count; i0 += kWave) {
+    float w = 0.0f;
+    if (i0 + lane < count) {
+      const f32x2 ml = a.ml[at + slot(i0 + lane)];
+      w = __builtin_amdgcn_exp2f(ml.x - top);
+      l += w * ml.y;
+    }
+    const int here = min(count - i0, kWave);
+#pragma unroll 4
+    for (int i = 0; i < here; ++i) {
+      const float wi = as_f32(__builtin_amdgcn_readlane(as_i32(w), i));
+      const f32x2 x = *(const f32x2*)(a.acc + (at + slot(i0 + i)) * TWL_HEAD_DIM + 2 * lane);
+      acc.x = fmaf(wi, x.x, acc.x);
+      acc.y = fmaf(wi, x.y, acc.y);
+    }
+  }
+  l = wave_allreduce<OpSum>(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *(uint32_t*)((uint16_t*)a.out + (size_t)row * TWL_HEAD_DIM + 2 * lane) = pack2<QT>(acc.x * inv, acc.y * inv);
+  if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : top * kLn2 + logf(l);
+}
+
+// How a call is cut into workgroups: from the sizes alone, the same for the workspace and the launch.
+struct PrefixPlan {
+  uint32_t nq, wr;                          // sets of 16 rows per wavefront, wavefronts across rows
+  uint32_t p_chunk, p_chunks, p_tiles, chunk, chunks, tiles;
+};
+
+constexpr uint32_t kPaMaxParts = 256;       // of one kind, per row
+
+static void cut_tokens(uint32_t tokens, uint64_t others, uint32_t target, uint32_t least, uint32_t* chunk,
+                       uint32_t* chunks) {
+  *chunk = 0;
+  *chunks = 0;
+  if (tokens == 0 || others == 0) return;
+  uint64_t want = (target + others - 1) / others;
+  if (want > kPaMaxParts) want = kPaMaxParts;
+  if (want < 1) want = 1;
+  uint64_t c = (tokens + want - 1) / want;
+  c = (c + least - 1) / least * least;
+  *chunk = (uint32_t)c;
+  *chunks = (uint32_t)((tokens + c - 1) / c);
+}
+
+static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num_kv_heads,
+                              uint32_t groups, uint32_t max_prefix, uint32_t max_group,
+                              uint32_t max_tokens) {
+  PrefixPlan p{};
+  const uint32_t G = num_q_heads / num_kv_heads;
+  const uint64_t rows = (uint64_t)max_group * G;
+  p.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.wr = rows <= 64 ? 1 : rows <= 128 ? 2 : 4;
+  const uint32_t per = 16 * p.nq * p.wr;
+  p.p_tiles = (uint32_t)((rows + per - 1) / per);
+  p.tiles = (G + 15) / 16;
+  cut_tokens(groups ? max_prefix : 0, (uint64_t)num_kv_heads * groups * p.p_tiles, 512, 128, &p.p_chunk,
+             &p.p_chunks);
+  cut_tokens(max_tokens, (uint64_t)num_kv_heads * batch * p.tiles, 1024, 128, &p.chunk, &p.chunks);
+  return p;
+}
+
+template <int QT, int KV>
+static void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& p, uint32_t blocks, hipStream_t st) {
+#define TWL_PA(NQ, WR) \
+  hipLaunchKernelGGL((prefix_attn_kernel<QT, KV, NQ, WR>), dim3(blocks), dim3(kPaThreads), 0, st, a)
+  if (a.p_chunks == 0 || p.nq == 1) TWL_PA(1, 1);
+  else if (p.nq == 2) TWL_PA(2, 1);
+  else if (p.wr == 1) TWL_PA(4, 1);
+  else if (p.wr == 2) TWL_PA(4, 2);
+  else TWL_PA(4, 4);
+#undef TWL_PA
+}
+
+}  // namespace twl
+
+extern "C" uint64_t twl_prefix_attn_workspace_bytes(uint32_t batch, uint32_t num_q_heads,
+                                                    uint32_t num_kv_heads, uint32_t groups,
+                                                    uint32_t max_prefix_tokens,
+                                                    uint32_t max_group_size, uint32_t max_tokens) {
+  if (batch == 0 || num_kv_heads == 0 || num_q_heads == 0 || num_q_heads % num_kv_heads != 0) return 0;
+  const twl::PrefixPlan p = twl::prefix_plan(batch, num_q_heads, num_kv_heads, groups,
+                                             max_prefix_tokens, max_group_size, max_tokens);
+  const uint64_t parts = (uint64_t)p.p_chunks + p.chunks;
+  if (parts <= 1) return 0;
+  return (uint64_t)batch * num_q_heads * parts * (TWL_HEAD_DIM + 2) * sizeof(float);
+}
+
+extern "C" int twl_prefix_attn(
+    const void* q, void* out, int dtype, const void* k_cache, const void* v_cache, int format,
+    uint64_t page_stride, uint64_t token_stride, uint64_t head_stride, const float* k_scale,
+    const float* v_scale, uint64_t scale_page_stride, uint64_t scale_token_stride,
+    uint64_t scale_head_stride, uint32_t num_pages, const int32_t* prefix_page_indices,
+    const int32_t* prefix_page_indptr, const int32_t* prefix_last_page_len,
+    const int32_t* group_indptr, uint32_t groups, uint32_t max_prefix_tokens,
+    uint32_t max_group_size, const int32_t* kv_page_indices, const int32_t* kv_page_indptr,
+    const int32_t* kv_last_page_len, uint32_t max_tokens, uint32_t batch, uint32_t num_q_heads,
+    uint32_t num_kv_heads, float sm_scale, float* lse_out, void* workspace,
+    uint64_t workspace_bytes, void* stream) {
+  const bool k8 = format == TWL_I8 || format == TWL_E4M3;
+  if (!q || !out || !k_cache || !v_cache || !kv_page_indices || !kv_page_indptr || !kv_last_page_len)
+    return TWL_ENULL;
+  if (groups && (!prefix_page_indices || !prefix_page_indptr || !prefix_last_page_len || !group_indptr))
+    return TWL_ENULL;
+  if (k8 && (!k_scale || !v_scale)) return TWL_ENULL;
+  if (dtype != TWL_F16 && dtype != TWL_BF16) return TWL_EDTYPE;
+  if (!k8 && format != dtype) return TWL_EDTYPE;
+  if (batch == 0 || num_q_heads == 0 || num_kv_heads == 0 || num_q_heads % num_kv_heads != 0 ||
+      num_pages == 0 || num_pages > 0x7FFFFFFFu)
+    return TWL_EINVAL;
+  if ((uint64_t)batch * num_q_heads > 65535u || groups > batch) return TWL_EINVAL;
+  if (groups && (max_group_size == 0 || max_group_size > batch)) return TWL_EINVAL;
+  if (max_tokens > (1u << 24) || max_prefix_tokens > (1u << 24)) return TWL_EINVAL;
+  if (token_stride > (1u << 24) || scale_token_stride > (1u << 24)) return TWL_EINVAL;
+  if (!(sm_scale == sm_scale)) return TWL_EINVAL;
+  const uint64_t align = k8 ? 15u : 7u;     // 16-byte loads of a token's channels
+  if ((page_stride | token_stride | head_stride) & align) return TWL_EALIGN;
+  if ((((uintptr_t)q) | ((uintptr_t)k_cache) | ((uintptr_t)v_cache) | ((uintptr_t)workspace)) & 15u)
+    return TWL_EALIGN;
+  if ((((uintptr_t)out) & 7u) || ((((uintptr_t)k_scale) | ((uintptr_t)v_scale) | ((uintptr_t)lse_out)) & 3u))
+    return TWL_EALIGN;
+  if (!groups) { max_prefix_tokens = 0; max_group_size = 0; }
+  const twl::PrefixPlan p = twl::prefix_plan(batch, num_q_heads, num_kv_heads, groups,
+                                             max_prefix_tokens, max_group_size, max_tokens);
+  const uint64_t need = twl_prefix_attn_workspace_bytes(batch, num_q_heads, num_kv_heads, groups,
+                                                        max_prefix_tokens, max_group_size, max_tokens);
+  if (need && !workspace) return TWL_ENULL;
+  if (workspace_bytes < need) return TWL_EINVAL;
+  const uint64_t p_blocks = (uint64_t)num_kv_heads * p.p_chunks * groups * p.p_tiles;
+  const uint64_t blocks = p_blocks + (uint64_t)num_kv_heads * p.chunks * batch * p.tiles;
+  if (blocks > 0x7FFFFFFFull) return TWL_EINVAL;
+  const uint64_t parts = (uint64_t)p.p_chunks + p.chunks, rows = (uint64_t)batch * num_q_heads;
+  twl::PrefixAttnArgs a{};
+  const uint64_t eb = k8 ? 1 : 2;
+  a.q = (const uint16_t*)q; a.out = out; a.lse = lse_out; a.k = (const uint8_t*)k_cache;
+  a.v = (const uint8_t*)v_cache; a.page_bytes = page_stride * eb; a.head_bytes = head_stride * eb;
+  a.token_bytes = (uint32_t)(token_stride * eb); a.ks = k_scale; a.vs = v_scale;
+  a.scale_page = scale_page_stride; a.scale_head = scale_head_stride;
+  a.scale_token = (uint32_t)scale_token_stride; a.num_pages = num_pages;
+  a.p_ids = prefix_page_indices; a.p_ptr = prefix_page_indptr; a.p_last = prefix_last_page_len;
+  a.g_ptr = group_indptr; a.ids = kv_page_indices; a.ptr = kv_page_indptr; a.last = kv_last_page_len;
+  a.batch = batch; a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads;
+  a.G = num_q_heads / num_kv_heads; a.groups = groups; a.max_prefix = max_prefix_tokens;
+  a.max_group = max_group_size; a.max_tokens = max_tokens; a.p_chunk = p.p_chunk;
+  a.p_chunks = p.p_chunks; a.p_tiles = p.p_tiles; a.chunk = p.chunk; a.chunks = p.chunks;
+  a.tiles = p.tiles; a.p_blocks = (uint32_t)p_blocks;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.acc = (float*)workspace;
+  a.ml = (twl::f32x2*)((float*)workspace + rows * parts * TWL_HEAD_DIM);
+  hipStream_t st = (hipStream_t)stream;
+  if (blocks) {
+    if (dtype == TWL_F16) {
+      if (format == TWL_I8) twl::launch_prefix<TWL_F16, TWL_I8>(a, p, (uint32_t)blocks, st);
+      else if (format == TWL_E4M3) twl::launch_prefix<TWL_F16, TWL_E4M3>(a, p, (uint32_t)blocks, st);
+      else twl::launch_prefix<TWL_F16, TWL_F16>(a, p, (uint32_t)blocks, st);
+    } else {
+      if (format == TWL_I8) twl::launch_prefix<TWL_BF16, TWL_I8>(a, p, (uint32_t)blocks, st);
+      else if (format == TWL_E4M3) twl::launch_prefix<TWL_BF16, TWL_E4M3>(a, p, (uint32_t)blocks, st);
+      else twl::launch_prefix<TWL_BF16, TWL_BF16>(a, p, (uint32_t)blocks, st);
+    }
+    if (hipGetLastError() != hipSuccess) return TWL_ELAUNCH;
+  }
+  if (p.p_chunks == 0 && p.chunks == 1) return TWL_OK;   // every row is written by its one part
+  const dim3 mgrid((uint32_t)((rows + twl::kPaWaves - 1) / twl::kPaWaves));
+  if (dtype == TWL_F16)
+    hipLaunchKernelGGL((twl::prefix_attn_merge_kernel<TWL_F16>), mgrid, dim3(twl::kPaThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((twl::prefix_attn_merge_kernel<TWL_BF16>), mgrid, dim3(twl::kPaThreads), 0, st, a);
+  return hipGetLastError() == hipSuccess ? TWL_OK : TWL_ELAUNCH;
+}

@@ -1,0 +1,133 @@
+"""K / V pages held in 8 bits: written from dense rows, and read back."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _lib
+from ._check import (check_cuda, check_dim, check_dtype, check_input, check_same_device, dtype_code, ptr,
+                     stream_of)
+from .attention import _cache_strides
+
+_FORMATS = {torch.int8: _lib.TWL_I8, torch.float8_e4m3fn: _lib.TWL_E4M3}
+
+
+def kv_format_code(dt: torch.dtype, name: str) -> int:
+    """Library code of an 8-bit page format."""
+    if dt not in _FORMATS:
+        raise RuntimeError(f"{name}: 8-bit pages are int8 or float8_e4m3fn, got {dt}")
+    return _FORMATS[dt]
+
+
+def check_quant_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                      v_scale: torch.Tensor):
+    """Checks of the four tensors of an 8-bit cache: ``(format, cache strides, scale strides)``."""
+    ks = _cache_strides(k_cache, "k_cache")
+    if _cache_strides(v_cache, "v_cache") != ks or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise RuntimeError("k_cache and v_cache must share shape, dtype and strides")
+    fmt = kv_format_code(k_cache.dtype, "k_cache")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        check_cuda(t, name); check_dtype(t, torch.float32, name)
+        if tuple(t.shape) != tuple(k_cache.shape[:3]):
+            raise RuntimeError(f"{name} must be [pages, 16, kv_heads] like the cache")
+    if k_scale.stride() != v_scale.stride():
+        raise RuntimeError("k_scale and v_scale must share strides")
+    check_same_device(k_cache, ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale))
+    return fmt, ks, k_scale.stride()
+
+
+def check_page_table(ref: torch.Tensor, batch: int, indices: torch.Tensor, indptr: torch.Tensor,
+                     last: torch.Tensor, prefix: str = "kv") -> None:
+    """Checks of a CSR page table of ``batch`` lists."""
+    names = (f"{prefix}_page_indices", f"{prefix}_page_indptr", f"{prefix}_last_page_len")
+    for name, t in zip(names, (indices, indptr, last)):
+        check_input(t, name); check_dtype(t, torch.int32, name)
+    if indptr.numel() != batch + 1 or last.numel() != batch:
+        raise RuntimeError(f"{names[1]} must have {batch + 1} and {names[2]} {batch} elements")
+    check_same_device(ref, *zip(names, (indices, indptr, last)))
+
+
+def _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len) -> int:
+    check_input(token_indptr, "token_indptr"); check_dtype(token_indptr, torch.int32, "token_indptr")
+    batch = token_indptr.numel() - 1
+    if batch < 1:
+        raise RuntimeError("token_indptr must have batch + 1 elements")
+    check_same_device(k_cache, ("token_indptr", token_indptr))
+    check_page_table(k_cache, batch, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    return batch
+
+
+def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torch.Tensor,
+                    k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, kv_page_indices: torch.Tensor,
+                    kv_page_indptr: torch.Tensor, kv_last_page_len: torch.Tensor) -> None:
+    """Quantise the rows of ``k_new`` / ``v_new`` [T,Hkv,128] (fp16 / bf16, head_dim contiguous) into
+    8-bit pages in one launch.
+
+    ``k_cache`` / ``v_cache`` [pages,16,Hkv,128] int8 or float8_e4m3fn (any page / token / head
+    strides), ``k_scale`` / ``v_scale`` fp32 [pages,16,Hkv]. Every (token, kv head) row is scaled by its
+    own largest magnitude: ``scale = max(max|x| / T, 2**-126)`` with T = 127 or 448, code = x / scale
+    rounded to nearest even. Rows ``token_indptr[b]`` to ``token_indptr[b + 1]`` (int32 [B+1]) are the
+    last tokens of request b: the page table counts them already. Rows from ``token_indptr[B]`` on are
+    ignored; rows that have no place in the table are skipped. A page that is written must belong
+    to one request only. A row with a non-finite element reads back as NaN."""
+    fmt, cs, ss = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
+    Hkv = k_cache.size(2)
+    for name, t in (("k_new", k_new), ("v_new", v_new)):
+        check_cuda(t, name); check_dim(3, t, name)
+        if t.size(1) != Hkv or t.size(2) != _lib.HEAD_DIM or t.stride(2) != 1:
+            raise RuntimeError(f"{name} must be [T, {Hkv}, {_lib.HEAD_DIM}] with contiguous head_dim")
+        if t.dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError(f"{name} must be float16 or bfloat16")
+    if v_new.shape != k_new.shape or v_new.stride() != k_new.stride() or v_new.dtype != k_new.dtype:
+        raise RuntimeError("k_new and v_new must share shape, dtype and strides")
+    batch = _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    check_same_device(k_cache, ("k_new", k_new), ("v_new", v_new))
+    if k_new.size(0) == 0:
+        return
+    with torch.cuda.device(k_cache.device):
+        rc = _lib.lib().twl_kv_quant_append(
+            ptr(k_new), ptr(v_new), dtype_code(k_new.dtype, "k_new"), k_new.stride(0), k_new.stride(1),
+            ptr(token_indptr), k_new.size(0), ptr(k_cache), ptr(v_cache), fmt, *cs, ptr(k_scale),
+            ptr(v_scale), *ss, k_cache.size(0), ptr(kv_page_indices), ptr(kv_page_indptr),
+            ptr(kv_last_page_len), batch, Hkv, stream_of(k_cache))
+    _lib.check(rc, "KvQuantAppend")
+
+
+def kv_quant_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, kv_page_indices: torch.Tensor, kv_page_indptr: torch.Tensor,
+                  kv_last_page_len: torch.Tensor, token_indptr: torch.Tensor, tokens: int,
+                  dtype: torch.dtype = torch.bfloat16, k_out: Optional[torch.Tensor] = None,
+                  v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values 8-bit pages hold, as dense rows ``(k, v)`` [tokens,Hkv,128] in ``dtype`` (fp16, bf16
+    or fp32): rows ``token_indptr[b]`` to ``token_indptr[b + 1]`` are the last tokens of request b (all
+    of them when ``token_indptr`` adds up the requests' lengths). Arguments as in
+    :func:`kv_quant_append`. Rows from ``token_indptr[B]`` on are left as they were (undefined in
+    outputs this call allocates); rows that have no place in the table are zeros."""
+    fmt, cs, ss = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
+    Hkv = k_cache.size(2)
+    batch = _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    tokens = int(tokens)
+    if tokens < 0:
+        raise RuntimeError("tokens must not be negative")
+    code, dev = dtype_code(dtype, "dtype"), k_cache.device
+    outs = []
+    with torch.cuda.device(dev):
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is None:
+                t = torch.empty((tokens, Hkv, _lib.HEAD_DIM), dtype=dtype, device=dev)
+            else:
+                check_input(t, name)
+                if tuple(t.shape) != (tokens, Hkv, _lib.HEAD_DIM) or t.dtype != dtype:
+                    raise RuntimeError(f"{name} must be [{tokens}, {Hkv}, {_lib.HEAD_DIM}] of {dtype}")
+                check_same_device(k_cache, (name, t))
+            outs.append(t)
+        if tokens == 0:
+            return outs[0], outs[1]
+        rc = _lib.lib().twl_kv_quant_read(
+            ptr(outs[0]), ptr(outs[1]), code, ptr(token_indptr), tokens, ptr(k_cache), ptr(v_cache), fmt,
+            *cs, ptr(k_scale), ptr(v_scale), *ss, k_cache.size(0), ptr(kv_page_indices),
+            ptr(kv_page_indptr), ptr(kv_last_page_len), batch, Hkv, stream_of(k_cache))
+    _lib.check(rc, "KvQuantRead")
+    return outs[0], outs[1]

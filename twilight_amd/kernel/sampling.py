@@ -188,3 +188,64 @@ def softmax_top_p(scores: torch.Tensor, top_p: Union[torch.Tensor, float],
     if return_low:
         out.append(low)
     return tuple(out)
+
+
+def _row_filter(value, name: str, rows: int, ref: torch.Tensor, dtype: torch.dtype, lo: float, hi: float):
+    """A filter of :func:`sample_tokens`: one number for every row, or a tensor with one per row."""
+    if isinstance(value, torch.Tensor):
+        check_input(value, name); check_dtype(value, dtype, name)
+        check_same_device(ref, (name, value))
+        if value.numel() != rows:
+            raise RuntimeError(f"{name} tensor must have one element per row ({rows})")
+        return value, 0
+    value = int(value) if dtype == torch.int32 else float(value)
+    if not lo <= value <= hi:
+        raise RuntimeError(f"{name} must be in [{lo}, {hi}], got {value}")
+    return None, value
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Draw the next token of every row of ``logits`` [B,V] (fp16, bf16 or fp32; V <= 262144, contiguous
+    along V) with the given uniform numbers ``u`` fp32 [B] in [0, 1). Returns int64 [B].
+
+    ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are numbers, or tensors with one value per row
+    (fp32; ``top_k`` int32). With w = exp((x - max) / temperature) and tokens ranked by logit, the
+    larger first and equal ones by index: ``top_k`` > 0 keeps the ranks below it; ``top_p`` < 1 keeps, of
+    those, the ranks before which less than ``top_p`` of their mass lies; ``min_p`` keeps w >= ``min_p``;
+    the best token is always kept. The answer is the first token, in vocabulary order, whose running
+    sum of kept w exceeds ``u`` times the sum of all kept w: sums are exact in fixed point, so equal
+    inputs give equal tokens. ``temperature`` 0 takes the best token. Logits of -inf or NaN are never
+    drawn; a row that has nothing else gives -1. In tensors, ``temperature`` <= 0 or NaN takes the best
+    token; ``top_k`` <= 0, ``top_p`` >= 1 or NaN and ``min_p`` <= 0 or NaN are off; ``top_p`` <= 0 keeps the
+    best token only and ``min_p`` >= 1 those whose logit equals the best."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise RuntimeError("logits must be a CUDA tensor")
+    check_dim(2, logits, "logits")
+    rows, vocab = logits.shape
+    if rows == 0 or vocab == 0 or vocab > 1 << 18:
+        raise RuntimeError("logits must have at least one row and 1 to 262144 columns")
+    if vocab > 1 and logits.stride(1) != 1:
+        raise RuntimeError("logits must be contiguous along the vocabulary")
+    code = dtype_code(logits.dtype, "logits")
+    check_input(u, "u"); check_dtype(u, torch.float32, "u"); check_same_device(logits, ("u", u))
+    if u.numel() != rows:
+        raise RuntimeError(f"u must have one element per row ({rows})")
+    f32 = torch.float32
+    t_arr, t_val = _row_filter(temperature, "temperature", rows, logits, f32, 0.0, 3e38)
+    k_arr, k_val = _row_filter(top_k, "top_k", rows, logits, torch.int32, 0, 2 ** 31 - 1)
+    p_arr, p_val = _row_filter(top_p, "top_p", rows, logits, f32, 0.0, 1.0)
+    m_arr, m_val = _row_filter(min_p, "min_p", rows, logits, f32, 0.0, 1.0)
+    with torch.cuda.device(logits.device):
+        if out is None:
+            out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+        else:
+            check_input(out, "out"); check_dtype(out, torch.int64, "out")
+            check_same_device(logits, ("out", out))
+            if out.numel() != rows:
+                raise RuntimeError(f"out must have one element per row ({rows})")
+        rc = _lib.lib().twl_sample_tokens(
+            ptr(logits), code, logits.stride(0), rows, vocab, ptr(u), ptr(t_arr), t_val, ptr(k_arr), k_val,
+            ptr(p_arr), p_val, ptr(m_arr), m_val, ptr(out), stream_of(logits))
+    _lib.check(rc, "SampleTokens")
+    return out
