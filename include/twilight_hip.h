@@ -610,14 +610,17 @@ int twl_prefix_attn(const void* q, void* out, int dtype, const void* k_cache, co
  *   The best rank always stays. tokens[r] int64 = the first token in vocabulary order whose running sum of
  *   kept w exceeds u times the sum of all kept w.
  * temperature <= 0 (or NaN in an array): the best token. -inf and NaN logits are never drawn; a row
- * with nothing else gives -1. w is computed in 64 bits and held as a multiple of 2^-45; sums are
- * exact, so the answer does not depend on their order.
+ * with nothing else gives -1. w is computed in 64 bits and held as a multiple of 2^-45 in integers;
+ * equal inputs give equal tokens. workspace: at least twl_sample_tokens_workspace_bytes(rows, vocab)
+ * bytes, 8-byte aligned, no initial contents required; calls that share it must not overlap in
+ * time. rows <= 65535.
  * ------------------------------------------------------------------------------------------- */
+uint64_t twl_sample_tokens_workspace_bytes(uint32_t rows, uint32_t vocab);
 int twl_sample_tokens(const void* logits, int dtype, uint64_t row_stride, uint32_t rows,
                       uint32_t vocab, const float* u, const float* temperature_arr,
                       float temperature, const int32_t* top_k_arr, int32_t top_k,
                       const float* top_p_arr, float top_p, const float* min_p_arr, float min_p,
-                      int64_t* tokens, void* stream);
+                      int64_t* tokens, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * The whole decode layer on one stream: quest select -> INT4 GEMV -> softmax + top-p -> sparse

@@ -35,7 +35,7 @@ EXPORTS = (
     "twl_group_union", "twl_rope_qk", "twl_quest_select",
     "twl_quest_page_scores", "twl_quest_topk_pages", "twl_kv_shadow_build", "twl_kv_append", "twl_meta_planes_build", "twl_quest_page_scores_planes", "twl_dequant_int4",
     "twl_kv_quant_append", "twl_kv_quant_read", "twl_prefix_attn_workspace_bytes", "twl_prefix_attn",
-    "twl_sample_tokens",
+    "twl_sample_tokens", "twl_sample_tokens_workspace_bytes",
     "twl_decode_layer", "twl_get_label_tensor", "twl_bgemv_int8", "twl_qk_int8_lse",
 )
 
@@ -137,7 +137,8 @@ def lib() -> ctypes.CDLL:
                                   vp, vp, vp, u32, u32, u32, vp, vp, vp, u32, u32, u32, u32, f32, vp, vp,
                                   u64, vp]
     L.twl_sample_tokens.argtypes = [vp, i32, u64, u32, u32, vp, vp, f32, vp, c_int32, vp, f32, vp, f32, vp,
-                                    vp]
+                                    vp, u64, vp]
+    L.twl_sample_tokens_workspace_bytes.argtypes = [u32, u32]
     L.twl_decode_layer.argtypes = [POINTER(LayerArgs), vp]
     L.twl_get_label_tensor.argtypes = [vp, vp, vp, u32, u32, u32, u32] + [c_int64] * 8 + [vp]
     L.twl_bgemv_int8.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32] + [c_int64] * 11 + [vp]
@@ -151,11 +152,13 @@ def lib() -> ctypes.CDLL:
                                   i64, i64, i64, vp]
     for name in EXPORTS:
         if name not in ("twl_strerror", "twl_sparse_attn_workspace_bytes",
-                        "twl_group_attn_workspace_bytes", "twl_prefix_attn_workspace_bytes"):
+                        "twl_group_attn_workspace_bytes", "twl_prefix_attn_workspace_bytes",
+                        "twl_sample_tokens_workspace_bytes"):
             getattr(L, name).restype = c_int
     L.twl_sparse_attn_workspace_bytes.restype = c_uint64
     L.twl_group_attn_workspace_bytes.restype = c_uint64
     L.twl_prefix_attn_workspace_bytes.restype = c_uint64
+    L.twl_sample_tokens_workspace_bytes.restype = c_uint64
     _lib = L
     return L
 

@@ -10,14 +10,36 @@
 //
 // Sums decide, so they must not depend on their order: w is computed in 64 bits and held as a
 // multiple of 2^-45 in 64-bit integers, whose sums are exact (2^18 tokens of weight 1 fill 63
-// bits). What is lost is below 2^-46 of the best token's weight, per token.
+// bits). What is lost is below 2^-46 of the best token's weight, per token: a token more than 32 T
+// below the best weighs nothing.
 //
-// One workgroup per row. The cuts by rank are found digit by digit of the logit's ordered bit
-// pattern (count or mass per digit in LDS); the tokens that share the last kept value are kept in
-// index order.
+// No row is sorted. Three launches, the first two with several workgroups (slices) per row so that a
+// small batch fills the chip (w costs about twenty 64-bit operations per token, which a single
+// compute unit would be at for most of the time):
+//   hist  Every slice finds its largest logit and, relative to that, adds up w (top-p) or counts tokens
+//         (top-k) in 512 bins of width T / 16. A bin is floor(16 x / T), so bins of different slices
+//         are the same intervals and the slices' sums join after one rescaling each.
+//   keep  Every slice joins its row's bins and finds the one that holds the cut. With top-p, tokens
+//         above it are kept: their w goes into sums over 512 consecutive tokens, and the tokens of the
+//         cut bin become candidates. With top-k, all tokens down to the cut bin are candidates.
+//   pick  One workgroup per row finds the exact cut among the candidates, digit by digit of the logit's
+//         ordered bit pattern (then of the index, where equal logits are cut), adds the kept ones to
+//         the sums and draws.
+// A row whose candidates do not fit (more than kSmpMaxCand tokens within T / 16 of the cut) is done by
+// pick alone, digit by digit over the whole row.
 #include "twl_common.h"
 
 namespace twl {
+
+constexpr int kSmpThreads = 512;
+constexpr int kSmpWaves = kSmpThreads / kWave;
+constexpr uint32_t kSmpMaxVocab = 1u << 18;
+constexpr double kSmpOne = 35184372088832.0;   // 2^45: the weight 1
+constexpr int kSmpBins = 512;
+constexpr int kSmpSeg = 512;                   // tokens of one running sum: a wavefront, 8 a lane
+constexpr int kSmpStep = kSmpThreads * 8;      // tokens of one pass of a workgroup
+constexpr int kSmpPerThread = 16;
+constexpr uint32_t kSmpMaxCand = kSmpThreads * kSmpPerThread;
 
 struct SampleArgs {
   const void* logits;
@@ -31,50 +53,313 @@ struct SampleArgs {
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
   int64_t* tokens;
+  // workspace
+  uint32_t slices, iters;     // slices of iters * kSmpStep tokens
+  uint64_t* best;             // [rows, slices]  key, then the lowest index
+  uint64_t* hist;             // [rows, slices, kSmpBins]
+  uint64_t* seg;              // [rows, segments]
+  uint64_t* cand;             // [rows, cand_stride]  key, then the complement of the index
+  uint32_t cand_stride;       // min(kSmpMaxCand, vocab)
+  struct SampleCut* cut;      // [rows]
+  uint32_t* cand_count;       // [rows]
 };
 
-constexpr int kSmpThreads = 1024;
-constexpr int kSmpWaves = kSmpThreads / kWave;
-constexpr uint32_t kSmpMaxVocab = 1u << 18;
-constexpr double kSmpOne = 35184372088832.0;   // 2^45: the weight 1
+// What keep leaves for pick: the bin of the cut (bins run down from the best token's, 0), and for
+// top-p the mass above it and the mass to reach.
+struct SampleCut {
+  double before, goal;
+  int32_t bin, pad;
+};
 
+template <int DT>
+__device__ __forceinline__ float masked_logit(float x) {
+  return x != x ? -__builtin_inff() : x + 0.0f;   // NaN counts as masked; -0 ranks as +0
+}
 template <int DT>
 __device__ __forceinline__ float logit_at(const SampleArgs& a, uint32_t row, uint32_t i) {
   float x;
   if (DT == TWL_F32) x = ((const float*)a.logits)[row * a.row_stride + i];
   else x = bits16_to_f32<DT>(((const uint16_t*)a.logits)[row * a.row_stride + i]);
-  return x != x ? -__builtin_inff() : x + 0.0f;   // NaN counts as masked; -0 ranks as +0
+  return masked_logit<DT>(x);
 }
-// order-preserving bit pattern
+// Eight consecutive logits from i on; -inf behind the vocabulary.
+template <int DT>
+__device__ __forceinline__ void logits8(const SampleArgs& a, uint32_t row, uint32_t i, float* x) {
+  constexpr int kBytes = DT == TWL_F32 ? 4 : 2;
+  const uint8_t* p = (const uint8_t*)a.logits + (row * a.row_stride + i) * kBytes;
+  if (i + 8 <= a.vocab && (((uintptr_t)p) & 15u) == 0) {
+    if (DT == TWL_F32) {
+      const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
+    } else {
+      unpack8<DT>(*(const u32x4*)p, x);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = masked_logit<DT>(x[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = i + j < a.vocab ? logit_at<DT>(a, row, i + j) : -__builtin_inff();
+  }
+}
+// order-preserving bit pattern, and back
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = as_u32(x);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return as_f32(key ^ (~(uint32_t)((int32_t)key >> 31) | 0x80000000u));
+}
+constexpr uint32_t kKeyNone = 0x007FFFFFu;     // key_of(-inf)
 
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
   return v;
 }
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {   // inclusive, in lane order
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) v = max(v, (uint64_t)__shfl_xor(v, d));
+  return v;
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {   // inclusive, in lane order
   const int lane = lane_id();
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
-    const uint64_t x = __shfl_up(v, d);
+    const T x = __shfl_up(v, d);
     if (lane >= d) v += x;
   }
   return v;
 }
 
+// How a row is filtered.
+struct RowFilter {
+  double T, p, min_p;
+  int32_t k;
+  bool greedy, by_rank, by_mass;   // the best token only; top-k cuts; top-p cuts (and no top-k)
+};
+__device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, uint32_t row) {
+  RowFilter f;
+  const float T = a.temperature ? a.temperature[row] : a.temperature_all;
+  f.T = fmin((double)T, 1e300);                 // finite: a masked logit has weight 0 at every T
+  f.p = a.top_p ? a.top_p[row] : a.top_p_all;
+  f.min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+  f.k = a.top_k ? a.top_k[row] : a.top_k_all;
+  f.greedy = !(T > 0.0f) || f.k == 1;
+  f.by_rank = f.k > 0 && (uint32_t)f.k < a.vocab;
+  f.by_mass = !f.by_rank && f.p < 1.0;
+  return f;
+}
+
+// w and its fixed-point form, for logits relative to `top`.
+//   2^z = 2^(n >> 6) * 2^((n & 63) / 64) * 2^f,   n = rint(64 z),  |f| <= 1/128
+// with the middle factor from a table and the last from its series to the fifth power
+// (next term (ln 2 / 128)^6 / 720 < 4e-17).
+struct Weigher {
+  const double* table;        // LDS, 2^(i / 64)
+  double top, per;            // per = log2(e) / T
+  __device__ __forceinline__ double z_of(float x) const { return x == top ? 0.0 : ((double)x - top) * per; }
+  __device__ __forceinline__ double exp2_of(double z) const {
+    z = fmax(z, -1000.0);
+    const double n = rint(z * 64.0);
+    const double f = fma(n, -1.0 / 64, z) * 0.693147180559945309417;
+    const int i = (int)n;
+    double y = fma(f, 1.0 / 120, 1.0 / 24);
+    y = fma(f, y, 1.0 / 6);
+    y = fma(f, y, 0.5);
+    y = fma(f, y, 1.0);
+    y = fma(f, y, 1.0);
+    return __builtin_amdgcn_ldexp(y * table[i & 63], i >> 6);
+  }
+  __device__ __forceinline__ double weight(float x) const { return exp2_of(z_of(x)); }
+  static __device__ __forceinline__ uint64_t fixed(double w) {
+    // adding 2^52 leaves the integer nearest w 2^45 in the low bits
+    return __builtin_bit_cast(uint64_t, fma(w, kSmpOne, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+  }
+  __device__ __forceinline__ uint64_t mass(float x) const { return fixed(weight(x)); }
+};
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+}
+
+// Bins of width T / 16 from the best token's down: monotone in x, the same intervals for every slice.
+struct Binner {
+  float per;
+  __device__ __forceinline__ int bin(float x) const {
+    return (int)fminf(fmaxf(floorf(x * per), -1073741824.0f), 1073741824.0f);
+  }
+};
+__device__ __forceinline__ Binner binner(const RowFilter& f) {
+  // bounded away from 0 and infinity, either of which could make a NaN of a logit
+  return Binner{fminf(fmaxf((float)(16.0 / f.T), 1e-37f), 1e30f)};
+}
+
+// ---- first launch ------------------------------------------------------------------------------
+template <int DT, int ITERS>
+__global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) {
+  __shared__ uint64_t hist[kSmpBins];
+  __shared__ uint64_t wbest[kSmpWaves];
+  __shared__ double table[64];
+  const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
+  const uint32_t first = slice * (ITERS * kSmpStep) + threadIdx.x * 8;
+  float x[ITERS][8];
+#pragma unroll
+  for (int t = 0; t < ITERS; ++t) logits8<DT>(a, row, first + t * kSmpStep, x[t]);
+  const RowFilter f = row_filter(a, row);
+  for (int i = threadIdx.x; i < kSmpBins; i += kSmpThreads) hist[i] = 0;
+  fill_table(table);
+  // a thread's tokens ascend, so the first of equal ones is found by a strict comparison
+  float m = -__builtin_inff();
+  uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+  for (int t = 0; t < ITERS; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (x[t][j] > m) { m = x[t][j]; at = first + t * kSmpStep + j; }
+  uint64_t best = wave_max(((uint64_t)key_of(m) << 32) | (0xFFFFFFFFu - at));
+  if (lane_id() == 0) wbest[threadIdx.x / kWave] = best;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSmpWaves; ++w) best = max(best, wbest[w]);
+  const size_t out = (size_t)row * a.slices + slice;
+  if (threadIdx.x == 0) {
+    a.best[out] = best;
+    if (slice == 0) a.cand_count[row] = 0;
+  }
+  if (f.greedy || !(f.by_rank || f.by_mass) || (uint32_t)(best >> 32) <= kKeyNone) return;
+  const float top = key_value((uint32_t)(best >> 32));
+  const Weigher wt{table, top, 1.4426950408889634074 / f.T};
+  const Binner bn = binner(f);
+  const int top_bin = bn.bin(top);
+#pragma unroll
+  for (int t = 0; t < ITERS; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t rel = (uint32_t)(top_bin - bn.bin(x[t][j]));
+      if (rel < kSmpBins) {
+        const uint64_t v = f.by_rank ? (x[t][j] > -__builtin_inff() ? 1ull : 0ull) : wt.mass(x[t][j]);
+        atomicAdd((unsigned long long*)&hist[rel], (unsigned long long)v);
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kSmpBins; i += kSmpThreads) a.hist[out * kSmpBins + i] = hist[i];
+}
+
+// best token of a row from its slices, by every thread
+__device__ __forceinline__ uint64_t row_best(const SampleArgs& a, uint32_t row) {
+  uint64_t b = 0;
+  for (uint32_t s = lane_id(); s < a.slices; s += kWave) b = max(b, a.best[(size_t)row * a.slices + s]);
+  return wave_max(b);
+}
+
+// ---- second launch -----------------------------------------------------------------------------
+template <int DT, int ITERS>
+__global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) {
+  static_assert(kSmpBins == kSmpThreads, "one bin per thread");
+  __shared__ uint64_t list[kSmpMaxCand];
+  __shared__ double wsum[kSmpWaves], table[64];
+  __shared__ double cut_before;
+  __shared__ int cut_bin;
+  __shared__ uint32_t list_n, list_at;
+  const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
+  const uint32_t first = slice * (ITERS * kSmpStep) + threadIdx.x * 8;
+  float x[ITERS][8];
+#pragma unroll
+  for (int t = 0; t < ITERS; ++t) logits8<DT>(a, row, first + t * kSmpStep, x[t]);
+  const RowFilter f = row_filter(a, row);
+  const uint64_t best = row_best(a, row);
+  const uint32_t top_key = (uint32_t)(best >> 32);
+  if (f.greedy || top_key <= kKeyNone) return;
+  const float top = key_value(top_key);
+  const Binner bn = binner(f);
+  const int top_bin = bn.bin(top);
+  fill_table(table);
+  if (threadIdx.x == 0) {
+    list_n = 0;
+    cut_bin = f.by_rank ? kSmpBins - 1 : kSmpBins;
+    cut_before = 0.0;
+  }
+  __syncthreads();
+  const Weigher wt{table, top, 1.4426950408889634074 / f.T};
+  double goal = (double)f.k;
+  if (f.by_rank || f.by_mass) {
+    // this thread's bin of the row, from the slices in order
+    double v = 0.0;
+    for (uint32_t s = 0; s < a.slices; ++s) {
+      const size_t at = (size_t)row * a.slices + s;
+      const uint32_t key = (uint32_t)(a.best[at] >> 32);
+      if (key <= kKeyNone) continue;
+      const float stop = key_value(key);
+      const int64_t mine = (int64_t)threadIdx.x - ((int64_t)top_bin - bn.bin(stop));
+      if (mine < 0) continue;
+      const double h = (double)a.hist[at * kSmpBins + mine];
+      v += f.by_rank ? h : h * wt.weight(stop);
+    }
+    const int wave = threadIdx.x / kWave;
+    const double incl = wave_scan(v);
+    if (lane_id() == kWave - 1) wsum[wave] = incl;
+    __syncthreads();
+    double off = 0.0, total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmpWaves; ++w) {
+      if (w < wave) off += wsum[w];
+      total += wsum[w];
+    }
+    if (f.by_mass) goal = f.p * total;
+    const double after = off + incl, before = after - v;
+    // the first bin whose running sum reaches the goal. before may be off by a rounding from the
+    // previous bin's after, so the choice is made once, by the lowest bin that reaches it
+    const uint64_t hit = __ballot(after >= goal && v > 0.0);
+    if (hit && lane_id() == __builtin_ctzll(hit)) atomicMin(&cut_bin, (int)threadIdx.x);
+    __syncthreads();
+    if ((int)threadIdx.x == cut_bin) cut_before = before;
+    __syncthreads();
+  }
+  const int cut = cut_bin;
+  if (slice == 0 && threadIdx.x == 0) a.cut[row] = SampleCut{cut_before, goal, cut, 0};
+  const uint32_t segs = (a.vocab + kSmpSeg - 1) / kSmpSeg;
+#pragma unroll
+  for (int t = 0; t < ITERS; ++t) {
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = x[t][j];
+      const int rel = top_bin - bn.bin(y);
+      if ((uint32_t)rel >= kSmpBins || !(y > -__builtin_inff())) continue;
+      if (rel == cut || (f.by_rank && rel < cut)) {
+        const uint32_t at = atomicAdd(&list_n, 1u);
+        if (at < kSmpMaxCand)
+          list[at] = ((uint64_t)key_of(y) << 32) | (0xFFFFFFFFu - (first + t * kSmpStep + j));
+      } else if (!f.by_rank && rel < cut) {
+        const double w = wt.weight(y);
+        if (y == top || !(w < f.min_p)) mine += Weigher::fixed(w);
+      }
+    }
+    if (!f.by_rank) {
+      const uint64_t s = wave_sum(mine);
+      const uint32_t g = (first + t * kSmpStep) / kSmpSeg;
+      if (lane_id() == 0 && g < segs) a.seg[(size_t)row * segs + g] = s;
+    }
+  }
+  __syncthreads();
+  const uint32_t n = list_n;
+  if (n == 0) return;
+  if (threadIdx.x == 0) list_at = atomicAdd(&a.cand_count[row], n);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < min(n, kSmpMaxCand); i += kSmpThreads)
+    if (list_at + i < a.cand_stride) a.cand[(size_t)row * a.cand_stride + list_at + i] = list[i];
+}
+
+// ---- third launch ------------------------------------------------------------------------------
 struct SampleShared {
-  uint64_t seg[kSmpMaxVocab / kWave];   // measure of every 64 tokens
-  uint64_t mass[256];
-  uint32_t count[256];
+  uint64_t seg[kSmpMaxVocab / kWave];   // generic: measure of every 64 tokens; else of every kSmpSeg
+  uint64_t hist[2048];
   uint64_t wsum[kSmpWaves];
+  double table[64];
   uint32_t word[8];
   uint64_t wide[4];
 };
-
 // Sum of measure(i) over the row, by 64 tokens in sh.seg.
 template <class F>
 __device__ __forceinline__ uint64_t measure_row(SampleShared& sh, uint32_t vocab, F measure) {
@@ -139,19 +424,19 @@ __device__ __forceinline__ uint32_t key_reaching(SampleShared& sh, uint32_t voca
   uint32_t prefix = 0;
   above = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (threadIdx.x < 256) sh.mass[threadIdx.x] = 0;
+    if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < vocab; i += kSmpThreads) {
       uint32_t key;
       const uint64_t m = measure(i, key);
       if (m && (shift == 24 || (key >> (shift + 8)) == prefix))
-        atomicAdd((unsigned long long*)&sh.mass[(key >> shift) & 255], (unsigned long long)m);
+        atomicAdd((unsigned long long*)&sh.hist[(key >> shift) & 255], (unsigned long long)m);
     }
     __syncthreads();
     if (threadIdx.x < kWave) {          // lane 0 holds the four largest digits
       const int lane = lane_id();
       uint64_t m[4], s = 0;
-      for (int j = 0; j < 4; ++j) s += m[j] = sh.mass[255 - (4 * lane + j)];
+      for (int j = 0; j < 4; ++j) s += m[j] = sh.hist[255 - (4 * lane + j)];
       uint64_t run = wave_scan(s) - s + above;
       for (int j = 0; j < 4; ++j) {
         if (run < target && run + m[j] >= target) {
@@ -169,64 +454,38 @@ __device__ __forceinline__ uint32_t key_reaching(SampleShared& sh, uint32_t voca
   return prefix;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kSmpThreads) void sample_kernel(SampleArgs a) {
-  __shared__ SampleShared sh;
-  const uint32_t row = blockIdx.x, V = a.vocab;
-  const int wave = threadIdx.x / kWave;
-  const float T0 = a.temperature ? a.temperature[row] : a.temperature_all;
-  const double T = fmin((double)T0, 1e300);   // finite: a masked logit has weight 0 at every T
-  const double p = a.top_p ? a.top_p[row] : a.top_p_all;
-  const double min_p = a.min_p ? a.min_p[row] : a.min_p_all;
-  const int32_t k = a.top_k ? a.top_k[row] : a.top_k_all;
-
-  // ---- the best token ---------------------------------------------------------------------------
-  uint64_t best = 0;                    // key, then the lowest index
-  for (uint32_t i = threadIdx.x; i < V; i += kSmpThreads)
-    best = max(best, ((uint64_t)key_of(logit_at<DT>(a, row, i)) << 32) | (0xFFFFFFFFu - i));
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) best = max(best, (uint64_t)__shfl_xor(best, d));
-  if (lane_id() == 0) sh.wsum[wave] = best;
-  __syncthreads();
-  for (int w = 0; w < kSmpWaves; ++w) best = max(best, sh.wsum[w]);
-  __syncthreads();
-  const uint32_t top_key = (uint32_t)(best >> 32), top_at = 0xFFFFFFFFu - (uint32_t)best;
-  if (top_key <= key_of(-__builtin_inff()) || !(T0 > 0.0f) || k == 1) {
-    if (threadIdx.x == 0) a.tokens[row] = top_key <= key_of(-__builtin_inff()) ? -1 : (int64_t)top_at;
-    return;
-  }
-  const double top = logit_at<DT>(a, row, top_at);
-  auto weight = [&](float x) { return (double)x == top ? 1.0 : exp(((double)x - top) / T); };
-  auto mass = [&](float x) { return (uint64_t)(weight(x) * kSmpOne + 0.5); };
-
+// The whole of a row by one workgroup, without candidates.
+template <int DT, class Aim>
+__device__ uint32_t pick_from_row(SampleShared& sh, const SampleArgs& a, uint32_t row, const RowFilter& f,
+                                  const Weigher& wt, uint32_t top_key, Aim aim) {
+  const uint32_t V = a.vocab;
   // ---- cuts by rank: keys above `cut` are kept, and of those equal to it the first `ties` --------
   uint32_t cut = 0, ties = V;
   uint64_t above = 0;
-  if (k > 0 && (uint32_t)k < V) {
-    cut = key_reaching(sh, V, (uint64_t)k, [&](uint32_t i, uint32_t& key) {
+  if (f.by_rank) {
+    cut = key_reaching(sh, V, (uint64_t)f.k, [&](uint32_t i, uint32_t& key) {
       key = key_of(logit_at<DT>(a, row, i));
       return 1ull;
     }, above);
-    ties = (uint32_t)((uint64_t)k - above);
+    ties = (uint32_t)((uint64_t)f.k - above);
   }
-  auto key_value = [](uint32_t key) { return as_f32(key ^ (~(uint32_t)((int32_t)key >> 31) | 0x80000000u)); };
-  if (p < 1.0) {
-    const uint64_t tie_mass = cut ? mass(key_value(cut)) : 0;
+  if (f.p < 1.0) {
+    const uint64_t tie_mass = cut ? wt.mass(key_value(cut)) : 0;
     uint64_t total = measure_row(sh, V, [&](uint32_t i) {
       const float x = logit_at<DT>(a, row, i);
-      return key_of(x) > cut ? mass(x) : 0ull;
+      return key_of(x) > cut ? wt.mass(x) : 0ull;
     });
     total += tie_mass * (cut ? ties : 0);
-    const double goal = p * (double)total;
+    const double goal = f.p * (double)total;
     const uint64_t target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
     // the last kept token is the one whose running mass reaches the target. Equal keys weigh the
     // same, so all tokens of the cut's key may count here: those beyond `ties` come after the goal
     const uint32_t pcut = key_reaching(sh, V, target, [&](uint32_t i, uint32_t& key) {
       const float x = logit_at<DT>(a, row, i);
       key = key_of(x);
-      return key >= cut ? mass(x) : 0ull;
+      return key >= cut ? wt.mass(x) : 0ull;
     }, above);
-    const uint64_t each = mass(key_value(pcut));
+    const uint64_t each = wt.mass(key_value(pcut));
     const uint64_t want = (target - above + each - 1) / each;
     if (pcut > cut) ties = (uint32_t)min(want, (uint64_t)V);
     else ties = (uint32_t)min(want, (uint64_t)ties);
@@ -245,43 +504,304 @@ __global__ __launch_bounds__(kSmpThreads) void sample_kernel(SampleArgs a) {
     const float x = logit_at<DT>(a, row, i);
     const uint32_t key = key_of(x);
     if (key < cut || (key == cut && i > last_tie)) return 0ull;
-    const double w = weight(x);
-    if (key != top_key && w < min_p) return 0ull;
-    return (unsigned long long)(w * kSmpOne + 0.5);
+    const double w = wt.weight(x);
+    if (key != top_key && w < f.min_p) return 0ull;
+    return (unsigned long long)Weigher::fixed(w);
   };
   const uint64_t total = measure_row(sh, V, kept);
+  return first_beyond(sh, V, aim(total), kept);
+}
+
+// Exclusive running sum of v over the threads, and the sum of all.
+__device__ __forceinline__ uint64_t block_scan(SampleShared& sh, uint64_t v, uint64_t& total) {
+  const int wave = threadIdx.x / kWave;
+  const uint64_t incl = wave_scan(v);
+  if (lane_id() == kWave - 1) sh.wsum[wave] = incl;
+  __syncthreads();
+  uint64_t off = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSmpWaves; ++w) {
+    if (w < wave) off += sh.wsum[w];
+    total += sh.wsum[w];
+  }
+  __syncthreads();
+  return off + incl - v;
+}
+
+// Among the threads' values (those with a measure), the value at which the running measure, from the
+// largest value down, first reaches `target` (>= 1, <= the total), and the measure above it.
+__device__ __forceinline__ uint32_t value_reaching(SampleShared& sh, const uint32_t* val, const uint64_t* meas,
+                                                   uint64_t target, uint64_t& above) {
+  uint32_t lo = 0, hi = 0xFFFFFFFFu;
+  above = 0;
+  for (;;) {
+    // the range that is in use: 16-bit logits and few candidates are through after a digit or two
+    uint32_t mn = 0xFFFFFFFFu, mx = 0;
+#pragma unroll
+    for (int j = 0; j < kSmpPerThread; ++j)
+      if (meas[j] && val[j] >= lo && val[j] <= hi) {
+        mn = min(mn, val[j]);
+        mx = max(mx, val[j]);
+      }
+    uint32_t nmn = 0xFFFFFFFFu - mn;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      mx = max(mx, (uint32_t)__shfl_xor(mx, d));
+      nmn = max(nmn, (uint32_t)__shfl_xor(nmn, d));
+    }
+    if (lane_id() == 0) sh.wsum[threadIdx.x / kWave] = ((uint64_t)mx << 32) | nmn;
+    for (int i = threadIdx.x; i < 2048; i += kSmpThreads) sh.hist[i] = 0;
+    __syncthreads();
+    uint32_t top = 0, low = 0;
+#pragma unroll
+    for (int w = 0; w < kSmpWaves; ++w) {
+      top = max(top, (uint32_t)(sh.wsum[w] >> 32));
+      low = max(low, (uint32_t)sh.wsum[w]);
+    }
+    hi = top;
+    lo = 0xFFFFFFFFu - low;
+    __syncthreads();
+    if (lo >= hi) return hi;
+    const int bits = 32 - __builtin_clz(hi - lo);
+    const int shift = max(0, bits - 11);
+#pragma unroll
+    for (int j = 0; j < kSmpPerThread; ++j)
+      if (meas[j] && val[j] >= lo && val[j] <= hi)
+        atomicAdd((unsigned long long*)&sh.hist[(hi - val[j]) >> shift], (unsigned long long)meas[j]);
+    __syncthreads();
+    uint64_t m[4], s = 0, total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += m[j] = sh.hist[4 * threadIdx.x + j];
+    uint64_t run = block_scan(sh, s, total) + above;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (run < target && run + m[j] >= target) {
+        sh.word[0] = 4 * threadIdx.x + j;
+        sh.wide[0] = run;
+      }
+      run += m[j];
+    }
+    __syncthreads();
+    const uint32_t digit = sh.word[0];
+    above = sh.wide[0];
+    __syncthreads();
+    hi -= digit << shift;
+    const uint32_t width = (1u << shift) - 1;
+    lo = max(lo, hi > width ? hi - width : 0u);
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) {
+  __shared__ SampleShared sh;
+  const uint32_t row = blockIdx.x, V = a.vocab;
+  const RowFilter f = row_filter(a, row);
+  const uint64_t best = row_best(a, row);
+  const uint32_t top_key = (uint32_t)(best >> 32);
+  if (f.greedy || top_key <= kKeyNone) {
+    if (threadIdx.x == 0) a.tokens[row] = top_key <= kKeyNone ? -1 : (int64_t)(0xFFFFFFFFu - (uint32_t)best);
+    return;
+  }
+  const float top = key_value(top_key);
+  const Weigher wt{sh.table, top, 1.4426950408889634074 / f.T};
+  fill_table(sh.table);
   const float u = a.u[row];
-  const double at = (u > 0.0f ? fmin((double)u, 1.0) : 0.0) * (double)total;
-  const uint64_t target = min((uint64_t)at, total - 1);
-  const uint32_t token = first_beyond(sh, V, target, kept);
-  if (threadIdx.x == 0) a.tokens[row] = token;
+  auto aim = [&](uint64_t total) {
+    const double at = (u > 0.0f ? fmin((double)u, 1.0) : 0.0) * (double)total;
+    return min((uint64_t)at, total - 1);
+  };
+  const uint32_t n = a.cand_count[row];
+  __syncthreads();
+  if (n > kSmpMaxCand) {
+    const uint32_t token = pick_from_row<DT>(sh, a, row, f, wt, top_key, aim);
+    if (threadIdx.x == 0) a.tokens[row] = token;
+    return;
+  }
+  const SampleCut c = a.cut[row];
+  uint32_t key[kSmpPerThread], inv[kSmpPerThread];      // complement of the index: larger is earlier
+  uint64_t mass[kSmpPerThread];
+#pragma unroll
+  for (int j = 0; j < kSmpPerThread; ++j) {
+    const uint32_t i = j * kSmpThreads + threadIdx.x;
+    key[j] = 0;
+    inv[j] = 0;
+    mass[j] = 0;
+    if (i < n) {
+      const uint64_t e = a.cand[(size_t)row * a.cand_stride + i];
+      key[j] = (uint32_t)(e >> 32);
+      inv[j] = (uint32_t)e;
+      mass[j] = wt.mass(key_value(key[j]));
+    }
+  }
+  // kept candidates: key above key_cut, or equal to it with a complement of at least inv_cut
+  uint32_t key_cut = 0, inv_cut = 0;
+  uint64_t one[kSmpPerThread], above;
+  if (f.by_rank && (uint32_t)f.k < n) {
+#pragma unroll
+    for (int j = 0; j < kSmpPerThread; ++j) one[j] = key[j] ? 1 : 0;
+    key_cut = value_reaching(sh, key, one, (uint64_t)f.k, above);
+    const uint64_t ties = (uint64_t)f.k - above;
+#pragma unroll
+    for (int j = 0; j < kSmpPerThread; ++j) one[j] = key[j] == key_cut && key[j] ? 1 : 0;
+    inv_cut = value_reaching(sh, inv, one, ties, above);
+#pragma unroll
+    for (int j = 0; j < kSmpPerThread; ++j)
+      if (key[j] < key_cut || (key[j] == key_cut && inv[j] < inv_cut)) key[j] = 0;
+  }
+  if (f.p < 1.0 && n > 0) {
+    uint64_t mine = 0, total;
+#pragma unroll
+    for (int j = 0; j < kSmpPerThread; ++j) {
+      if (!key[j]) mass[j] = 0;
+      mine += mass[j];
+    }
+    block_scan(sh, mine, total);
+    const double goal = f.by_rank ? f.p * (double)total : c.goal - c.before;
+    const uint64_t target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
+    if (target <= total) {
+      const uint32_t rank_cut = key_cut;
+      key_cut = value_reaching(sh, key, mass, target, above);
+      const uint64_t each = wt.mass(key_value(key_cut));
+      const uint64_t ties = (target - above + each - 1) / each;
+      uint64_t have = 0, all;
+#pragma unroll
+      for (int j = 0; j < kSmpPerThread; ++j) {
+        one[j] = key[j] == key_cut && key[j] ? 1 : 0;
+        have += one[j];
+      }
+      block_scan(sh, have, all);
+      if (ties < all) inv_cut = value_reaching(sh, inv, one, ties, above);
+      else if (key_cut != rank_cut) inv_cut = 0;        // else what top-k left of these
+#pragma unroll
+      for (int j = 0; j < kSmpPerThread; ++j)
+        if (key[j] < key_cut || (key[j] == key_cut && inv[j] < inv_cut)) key[j] = 0;
+    }
+  }
+  // ---- sums over kSmpSeg tokens, and the draw -------------------------------------------------
+  const uint32_t segs = (V + kSmpSeg - 1) / kSmpSeg;
+  if (threadIdx.x < segs) sh.seg[threadIdx.x] = f.by_rank ? 0 : a.seg[(size_t)row * segs + threadIdx.x];
+  __syncthreads();
+  auto passes = [&](uint32_t k, double w) { return k == top_key || !(w < f.min_p); };
+#pragma unroll
+  for (int j = 0; j < kSmpPerThread; ++j)
+    if (key[j]) {
+      const double w = wt.weight(key_value(key[j]));
+      if (passes(key[j], w))
+        atomicAdd((unsigned long long*)&sh.seg[(0xFFFFFFFFu - inv[j]) / kSmpSeg], (unsigned long long)Weigher::fixed(w));
+    }
+  __syncthreads();
+  const uint64_t mine = threadIdx.x < segs ? sh.seg[threadIdx.x] : 0;
+  uint64_t total;
+  const uint64_t off = block_scan(sh, mine, total);
+  const uint64_t target = aim(total);
+  if (off <= target && off + mine > target) {
+    sh.word[0] = threadIdx.x;
+    sh.wide[0] = off;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  const Binner bn = binner(f);
+  const int top_bin = bn.bin(top);
+  const uint32_t i0 = sh.word[0] * kSmpSeg + lane_id() * 8;
+  float x[8];
+  logits8<DT>(a, row, i0, x);
+  uint64_t m[8], sum = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int rel = top_bin - bn.bin(x[j]);
+    const uint32_t k = key_of(x[j]), comp = 0xFFFFFFFFu - (i0 + j);
+    bool in = k > kKeyNone && rel < kSmpBins;
+    // tokens of the candidates' bins are kept by the exact cut, those above by their bin
+    if (rel == c.bin || (f.by_rank && rel < c.bin)) in = in && (k > key_cut || (k == key_cut && comp >= inv_cut));
+    else in = in && rel < c.bin;
+    const double w = wt.weight(x[j]);
+    m[j] = in && passes(k, w) ? Weigher::fixed(w) : 0;
+    sum += m[j];
+  }
+  uint64_t run = sh.wide[0] + wave_scan(sum) - sum;
+  int found = -1;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (found < 0 && run + m[j] > target && run <= target) found = j;
+    run += m[j];
+  }
+  if (found >= 0) a.tokens[row] = i0 + found;
+}
+
+struct SamplePlan {
+  uint32_t slices, iters;
+  uint64_t best, hist, seg, cand, cut, count, bytes;   // offsets into the workspace
+};
+// Slices of 4096, 8192 or 16384 tokens: as large as leaves about two workgroups per compute unit.
+static SamplePlan sample_plan(uint32_t rows, uint32_t vocab) {
+  SamplePlan p{};
+  p.iters = 4;
+  while (p.iters > 1 && (uint64_t)rows * ((vocab + p.iters * kSmpStep - 1) / (p.iters * kSmpStep)) < 512) p.iters >>= 1;
+  p.slices = (vocab + p.iters * kSmpStep - 1) / (p.iters * kSmpStep);
+  const uint64_t r = rows, segs = (vocab + kSmpSeg - 1) / kSmpSeg;
+  p.best = 0;
+  p.hist = p.best + r * p.slices * 8;
+  p.seg = p.hist + r * p.slices * kSmpBins * 8;
+  p.cand = p.seg + r * segs * 8;
+  p.cut = p.cand + r * (vocab < kSmpMaxCand ? vocab : kSmpMaxCand) * 8;
+  p.count = p.cut + r * sizeof(SampleCut);
+  p.bytes = p.count + r * 4;
+  return p;
+}
+
+template <int DT>
+static void launch_sample(const SampleArgs& a, hipStream_t st) {
+  const dim3 grid(a.rows * a.slices), block(kSmpThreads);
+#define TWL_SMP(ITERS)                                                                  \
+  do {                                                                                  \
+    hipLaunchKernelGGL((sample_hist_kernel<DT, ITERS>), grid, block, 0, st, a);         \
+    hipLaunchKernelGGL((sample_keep_kernel<DT, ITERS>), grid, block, 0, st, a);         \
+  } while (0)
+  if (a.iters == 1) TWL_SMP(1);
+  else if (a.iters == 2) TWL_SMP(2);
+  else TWL_SMP(4);
+#undef TWL_SMP
+  hipLaunchKernelGGL((sample_pick_kernel<DT>), dim3(a.rows), block, 0, st, a);
 }
 
 }  // namespace twl
+
+extern "C" uint64_t twl_sample_tokens_workspace_bytes(uint32_t rows, uint32_t vocab) {
+  if (rows == 0 || vocab == 0 || vocab > twl::kSmpMaxVocab) return 0;
+  return twl::sample_plan(rows, vocab).bytes;
+}
 
 extern "C" int twl_sample_tokens(const void* logits, int dtype, uint64_t row_stride, uint32_t rows,
                                  uint32_t vocab, const float* u, const float* temperature_arr,
                                  float temperature, const int32_t* top_k_arr, int32_t top_k,
                                  const float* top_p_arr, float top_p, const float* min_p_arr,
-                                 float min_p, int64_t* tokens, void* stream) {
-  if (!logits || !u || !tokens) return TWL_ENULL;
+                                 float min_p, int64_t* tokens, void* workspace,
+                                 uint64_t workspace_bytes, void* stream) {
+  if (!logits || !u || !tokens || !workspace) return TWL_ENULL;
   if (dtype != TWL_F16 && dtype != TWL_BF16 && dtype != TWL_F32) return TWL_EDTYPE;
-  if (rows == 0 || vocab == 0 || vocab > twl::kSmpMaxVocab || rows > 0x7FFFFFFFu) return TWL_EINVAL;
+  if (rows == 0 || vocab == 0 || vocab > twl::kSmpMaxVocab || rows > 65535u) return TWL_EINVAL;
   if (temperature != temperature || top_p != top_p || min_p != min_p) return TWL_EINVAL;
   if (((uintptr_t)logits) & (dtype == TWL_F32 ? 3u : 1u)) return TWL_EALIGN;
   if ((((uintptr_t)u) | ((uintptr_t)temperature_arr) | ((uintptr_t)top_k_arr) | ((uintptr_t)top_p_arr) |
        ((uintptr_t)min_p_arr)) & 3u)
     return TWL_EALIGN;
-  if (((uintptr_t)tokens) & 7u) return TWL_EALIGN;
+  if ((((uintptr_t)tokens) | ((uintptr_t)workspace)) & 7u) return TWL_EALIGN;
+  const twl::SamplePlan p = twl::sample_plan(rows, vocab);
+  if (workspace_bytes < p.bytes) return TWL_EINVAL;
   twl::SampleArgs a{};
   a.logits = logits; a.row_stride = row_stride; a.rows = rows; a.vocab = vocab; a.u = u;
   a.temperature = temperature_arr; a.top_k = top_k_arr; a.top_p = top_p_arr; a.min_p = min_p_arr;
   a.temperature_all = temperature; a.top_k_all = top_k; a.top_p_all = top_p; a.min_p_all = min_p;
   a.tokens = tokens;
-  const dim3 grid(rows), block(twl::kSmpThreads);
+  uint8_t* const ws = (uint8_t*)workspace;
+  a.slices = p.slices; a.iters = p.iters; a.best = (uint64_t*)(ws + p.best); a.hist = (uint64_t*)(ws + p.hist);
+  a.seg = (uint64_t*)(ws + p.seg); a.cand = (uint64_t*)(ws + p.cand); a.cut = (twl::SampleCut*)(ws + p.cut);
+  a.cand_count = (uint32_t*)(ws + p.count);
+  a.cand_stride = vocab < twl::kSmpMaxCand ? vocab : twl::kSmpMaxCand;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == TWL_F16) hipLaunchKernelGGL((twl::sample_kernel<TWL_F16>), grid, block, 0, st, a);
-  else if (dtype == TWL_BF16) hipLaunchKernelGGL((twl::sample_kernel<TWL_BF16>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((twl::sample_kernel<TWL_F32>), grid, block, 0, st, a);
+  if (dtype == TWL_F16) twl::launch_sample<TWL_F16>(a, st);
+  else if (dtype == TWL_BF16) twl::launch_sample<TWL_BF16>(a, st);
+  else twl::launch_sample<TWL_F32>(a, st);
   return hipGetLastError() == hipSuccess ? TWL_OK : TWL_ELAUNCH;
 }

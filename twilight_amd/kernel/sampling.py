@@ -204,8 +204,14 @@ def _row_filter(value, name: str, rows: int, ref: torch.Tensor, dtype: torch.dty
     return None, value
 
 
+def sample_tokens_workspace_bytes(rows: int, vocab: int) -> int:
+    """Bytes of scratch :func:`sample_tokens` needs for ``rows`` rows of ``vocab`` logits."""
+    return int(_lib.lib().twl_sample_tokens_workspace_bytes(rows, vocab))
+
+
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
-                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Draw the next token of every row of ``logits`` [B,V] (fp16, bf16 or fp32; V <= 262144, contiguous
     along V) with the given uniform numbers ``u`` fp32 [B] in [0, 1). Returns int64 [B].
 
@@ -218,13 +224,15 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     inputs give equal tokens. ``temperature`` 0 takes the best token. Logits of -inf or NaN are never
     drawn; a row that has nothing else gives -1. In tensors, ``temperature`` <= 0 or NaN takes the best
     token; ``top_k`` <= 0, ``top_p`` >= 1 or NaN and ``min_p`` <= 0 or NaN are off; ``top_p`` <= 0 keeps the
-    best token only and ``min_p`` >= 1 those whose logit equals the best."""
+    best token only and ``min_p`` >= 1 those whose logit equals the best. ``workspace``: a uint8 tensor of
+    :func:`sample_tokens_workspace_bytes` bytes that calls on one stream may share; by default a
+    fresh one is allocated."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise RuntimeError("logits must be a CUDA tensor")
     check_dim(2, logits, "logits")
     rows, vocab = logits.shape
-    if rows == 0 or vocab == 0 or vocab > 1 << 18:
-        raise RuntimeError("logits must have at least one row and 1 to 262144 columns")
+    if rows == 0 or vocab == 0 or vocab > 1 << 18 or rows > 65535:
+        raise RuntimeError("logits must have 1 to 65535 rows and 1 to 262144 columns")
     if vocab > 1 and logits.stride(1) != 1:
         raise RuntimeError("logits must be contiguous along the vocabulary")
     code = dtype_code(logits.dtype, "logits")
@@ -244,8 +252,15 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
             check_same_device(logits, ("out", out))
             if out.numel() != rows:
                 raise RuntimeError(f"out must have one element per row ({rows})")
+        need = sample_tokens_workspace_bytes(rows, vocab)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        else:
+            check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
+            if workspace.numel() < need or workspace.device != logits.device:
+                raise RuntimeError(f"workspace must hold {need} bytes on {logits.device}")
         rc = _lib.lib().twl_sample_tokens(
             ptr(logits), code, logits.stride(0), rows, vocab, ptr(u), ptr(t_arr), t_val, ptr(k_arr), k_val,
-            ptr(p_arr), p_val, ptr(m_arr), m_val, ptr(out), stream_of(logits))
+            ptr(p_arr), p_val, ptr(m_arr), m_val, ptr(out), ptr(workspace), workspace.numel(), stream_of(logits))
     _lib.check(rc, "SampleTokens")
     return out
