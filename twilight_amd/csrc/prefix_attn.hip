@@ -36,6 +36,7 @@ namespace twl {
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPaThreads = 256;
@@ -57,6 +58,7 @@ struct PrefixAttnArgs {
   const float* vs;
   uint64_t scale_page, scale_head;
   uint32_t scale_token;
+  bool scale_vec;                           // the scales of four tokens are one aligned 16-byte load
   uint32_t num_pages;
   const int32_t *p_ids, *p_ptr, *p_last, *g_ptr;   // prefix tables, members of every group
   const int32_t *ids, *ptr, *last;                 // the requests' own pages
@@ -69,6 +71,9 @@ struct PrefixAttnArgs {
   float* acc;                               // [rows, parts, 128]
   f32x2* ml;                                // [rows, parts]
 };
+
+struct Always { static constexpr bool value = true; };
+struct Never { static constexpr bool value = false; };
 
 __device__ __forceinline__ float max_over_kb(float x) {
   const uint32_t u = as_u32(x);
@@ -95,8 +100,10 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 template <int MT>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  return f32_to_bits16<MT>(x) | (f32_to_bits16<MT>(y) << 16);
+__device__ __forceinline__ uint32_t pack2(float x, float y) {   // one convert for both
+  const f32x2 v = {x, y};
+  if (MT == TWL_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2_t));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
 // four 8-bit codes -> four fp16 values
@@ -139,6 +146,39 @@ __device__ __forceinline__ int group_of(const PrefixAttnArgs& a, uint32_t b) {
   return g;
 }
 
+// The queries of a set of 16 rows as the B operand of S^T, and the factor that makes base-2 logits of
+// its products. PAIRED: channels in the order in which 16-byte loads of 8-bit K deliver them. TO_F16:
+// for products in fp16; a bf16 query goes there by way of a power of two.
+template <int QT, bool PAIRED, bool TO_F16>
+__device__ __forceinline__ void load_query(const PrefixAttnArgs& a, int row, int kb, u32x4* qf, float& scale) {
+  const uint16_t* src = a.q + (size_t)max(row, 0) * TWL_HEAD_DIM;
+  scale = a.scale_log2;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d = PAIRED ? 64 * (j >> 1) + 16 * kb + 8 * (j & 1) : 32 * j + 8 * kb;
+    qf[j] = *(const u32x4*)(src + d);
+    if (row < 0) qf[j] = u32x4{0, 0, 0, 0};
+  }
+  if (TO_F16 && QT == TWL_BF16) {
+    float f[4][8];
+    int top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unpack8<QT>(qf[j], f[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, as_i32(f[j][i]) & 0x7FFFFFFF);
+    }
+    top = as_i32(max_over_kb(as_f32(top)));
+    const int e = min(max((top >> 23) - 127, -126), 126);   // |q| < 2^(e + 1); NaN stays NaN
+    const float down = as_f32((127 - e) << 23);
+    scale *= as_f32((127 + e) << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[j][i] = pack2<TWL_F16>(f[j][2 * i] * down, f[j][2 * i + 1] * down);
+  }
+}
+
 // Four channels of a row's part: into the workspace, or, where a row has one part, the answer.
 template <int QT>
 __device__ __forceinline__ void put_row(const PrefixAttnArgs& a, int row, uint32_t part, uint32_t parts, int c,
@@ -171,40 +211,11 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   const int lane = lane_id(), n = lane & 15, kb = lane >> 4;
   const int wave = threadIdx.x / kWave, wr = wave / WT, wt = wave % WT;
 
-  // ---- queries: B operand of S^T, with the channel order of the K loads ------------------------
   u32x4 qf[NQ][4];
   float row_scale[NQ];
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    const int row = row_of((wr * NQ + x) * 16 + n);
-    const uint16_t* src = a.q + (size_t)max(row, 0) * TWL_HEAD_DIM;
-    row_scale[x] = a.scale_log2;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = k8 ? 64 * (j >> 1) + 16 * kb + 8 * (j & 1) : 32 * j + 8 * kb;
-      qf[x][j] = *(const u32x4*)(src + d);
-      if (row < 0) qf[x][j] = u32x4{0, 0, 0, 0};
-    }
-    if (k8 && QT == TWL_BF16) {
-      float f[4][8];
-      int top = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        unpack8<QT>(qf[x][j], f[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, as_i32(f[j][i]) & 0x7FFFFFFF);
-      }
-      top = as_i32(max_over_kb(as_f32(top)));
-      const int e = min(max((top >> 23) - 127, -126), 126);   // |q| < 2^(e + 1); NaN stays NaN
-      const float down = as_f32((127 - e) << 23);
-      row_scale[x] *= as_f32((127 + e) << 23);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          qf[x][j][i] = pack2<TWL_F16>(f[j][2 * i] * down, f[j][2 * i + 1] * down);
-    }
-  }
+  for (int x = 0; x < NQ; ++x)
+    load_query<QT, k8, k8>(a, row_of((wr * NQ + x) * 16 + n), kb, qf[x], row_scale[x]);
 
   f32x4 o[NQ][8];
   float m[NQ], l[NQ];
@@ -223,7 +234,9 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   const uint32_t voff = 4 * kb * a.token_bytes + (k8 ? 8 : 16) * n;
   const int tiles = (end - begin + kPaTile - 1) / kPaTile;
   int window = -1, held = 0;
-  for (int t = wt; t < tiles; t += WT) {
+  // one tile; only the last one of a part can be cut short by the end of the list
+  auto step = [&](int t, auto last) {
+    constexpr bool cut = decltype(last)::value;
     const int tok0 = begin + t * kPaTile;
     // page ids come 64 at a time, one per lane (32 tiles)
     if ((t >> 5) != window) {
@@ -248,10 +261,16 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const size_t so = (size_t)(p ? id1 : id0) * a.scale_page + 4 * kb * a.scale_token;
+        if (a.scale_vec) {
+          const f32x4 x = *(const f32x4*)(sk + so), y = *(const f32x4*)(sv + so);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ks[p][i] = sk[so + i * a.scale_token];
-          vs[p][i] = sv[so + i * a.scale_token];
+          for (int i = 0; i < 4; ++i) { ks[p][i] = x[i]; vs[p][i] = y[i]; }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ks[p][i] = sk[so + i * a.scale_token];
+            vs[p][i] = sv[so + i * a.scale_token];
+          }
         }
       }
     }
@@ -290,7 +309,6 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         for (int x = 0; x < NQ; ++x) s[x][p] = mfma16<MT>(kf, qf[x][j], s[x][p]);
       }
 
-    const bool cut = tok0 + kPaTile > end;
     if (cut) {
       // slots behind the last token hold whatever was there: their scales and V must not reach a
       // product, not even times zero
@@ -397,7 +415,10 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         }
       }
     }
-  }
+  };
+  const int whole = (end - begin) / kPaTile;
+  for (int t = wt; t < whole; t += WT) step(t, Never{});
+  if (whole < tiles && whole % WT == wt) step(whole, Always{});
 
   // ---- join the wavefronts that share rows, and leave the part --------------------------------
   const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
@@ -474,21 +495,246 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   }
 }
 
-// Grid: the prefix parts (kv head, part, group, row tile), then the own parts (kv head, part,
-// request, row tile).
-template <int QT, int KV, int NQ, int WR>
-__global__ __launch_bounds__(kPaThreads) void prefix_attn_kernel(PrefixAttnArgs a) {
+// The same part for many rows: 128 rows per workgroup (32 per wavefront), whose wavefronts take every
+// tile of K and V from LDS. Streaming from L2 into every wavefront's registers would need
+// 16 KB of L1 traffic per 32 tokens and 32 rows, twice what the products take.
+//
+// Tiles of 64 tokens, two buffers: while the products of one run, the next is on its way into registers;
+// it is written to the other buffer after them, one barrier per tile. 8-bit pages are widened to fp16
+// on that way, once per workgroup. A row of 256 bytes holds its 16 chunks of 16 bytes at place
+// c ^ (row % 16): the K operand's loads (16 rows, one chunk) and the V operand's (one row, 16 chunks)
+// both touch every bank once.
+constexpr int kStTile = 64, kStRows = 128;
+
+template <int QT, int KV, class RowOf>
+__device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int32_t* ids, int num_ids, int begin,
+                                              int end, uint32_t kvh, int rows_here, RowOf row_of, uint32_t part,
+                                              uint32_t parts) {
+  constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
+  constexpr int MT = k8 ? TWL_F16 : QT;
+  constexpr int NQ = 2;
+  constexpr int NL = k8 ? 2 : 4;            // 16-byte loads of K (and of V) per thread and tile
+  __shared__ u32x4 lds_k[2][kStTile * 16], lds_v[2][kStTile * 16];
+  __shared__ float lds_ks[2][k8 ? kStTile : 1], lds_vs[2][k8 ? kStTile : 1];
+  const int tx = threadIdx.x, lane = lane_id(), n = lane & 15, kb = lane >> 4, wave = tx / kWave;
+  const bool busy = wave * 16 * NQ < rows_here;   // a wavefront without rows only stages
+
+  u32x4 qf[NQ][4];
+  float row_scale[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x)
+    load_query<QT, false, k8>(a, row_of((wave * NQ + x) * 16 + n), kb, qf[x], row_scale[x]);
+
+  f32x4 o[NQ][8];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = kPaNoMax;
+    l[x] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[x][j] = f32x4{0, 0, 0, 0};
+  }
+  int vexp = -126;
+
+  const uint8_t* const kbase = a.k + kvh * a.head_bytes;
+  const uint8_t* const vbase = a.v + kvh * a.head_bytes;
+  const int tiles = (end - begin + kStTile - 1) / kStTile;
+  // a thread's place in a page: 16-bit, one page per load; 8-bit, two pages per load
+  const int tok = k8 ? (tx >> 3) & 15 : tx >> 4, chunk = k8 ? tx & 7 : tx & 15;
+  const uint32_t off = tok * a.token_bytes + 16 * chunk;
+  int window = -1, held = 0;
+  u32x4 raw[NL];
+  float sc = 0.0f;
+
+  // One of K and V of tile t, into registers; and from there into LDS.
+  auto fetch = [&](int t, bool is_v) {
+    if ((t >> 4) != window) {               // 64 page ids, 16 tiles
+      window = t >> 4;
+      const int at = min(begin / TWL_PAGE + window * kWave + lane, num_ids - 1);
+      held = (int)min((uint32_t)ids[at], a.num_pages - 1);
+    }
+    const uint8_t* const base = is_v ? vbase : kbase;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int pg = k8 ? 2 * i + __builtin_amdgcn_readfirstlane(tx >> 7) : i;
+      const uint64_t id = (uint32_t)__builtin_amdgcn_readlane(held, 4 * (t & 15) + pg);
+      raw[i] = *(const u32x4*)(base + id * a.page_bytes + off);
+    }
+    if (k8 && wave == 0) {                  // one scale per lane
+      const uint64_t id = (uint32_t)__shfl(held, 4 * (t & 15) + (lane >> 4));
+      sc = (is_v ? a.vs : a.ks)[id * a.scale_page + (lane & 15) * (size_t)a.scale_token + kvh * a.scale_head];
+    }
+  };
+  auto stage = [&](int t, bool is_v) {
+    const int left = end - begin - t * kStTile, buf = t & 1;
+    u32x4* const dst = (is_v ? lds_v : lds_k)[buf];
+    if (left < kStTile) {
+      // slots behind the last token hold whatever was there and must not reach a product
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (16 * (k8 ? 2 * i + (tx >> 7) : i) + tok >= left) raw[i] = u32x4{0, 0, 0, 0};
+      if (lane >= left) sc = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = 16 * (k8 ? 2 * i + (tx >> 7) : i) + tok;
+      if (k8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x2 lo = widen4<KV>(raw[i][2 * h]), hi = widen4<KV>(raw[i][2 * h + 1]);
+          dst[row * 16 + ((2 * chunk + h) ^ tok)] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+      } else {
+        dst[row * 16 + (chunk ^ tok)] = raw[i];
+      }
+    }
+    if (k8 && wave == 0) (is_v ? lds_vs : lds_ks)[buf][lane] = sc;
+  };
+
+  // the products of 32 tokens: pages 2 h and 2 h + 1 of tile t
+  auto products = [&](int t, int h, auto last) {
+    constexpr bool cut = decltype(last)::value;
+    const int left = end - begin - t * kStTile - 32 * h, buf = t & 1;
+    const u32x4* const kt = lds_k[buf] + 512 * h;
+    const u32x4* const vt = lds_v[buf] + 512 * h;
+    f32x4 s[NQ][2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) s[x][p] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x4 kf = kt[(16 * p + n) * 16 + ((4 * j + kb) ^ n)];
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) s[x][p] = mfma16<MT>(kf, qf[x][j], s[x][p]);
+      }
+    }
+    f32x4 ks[2], vs[2];
+    int rise = 0;
+    if (k8) {
+      const float top = wave_allreduce<OpMax>(fabsf(lds_vs[buf][32 * h + (lane & 31)]));
+      const int e = max(min((as_i32(top) >> 23) - 127, 126), vexp);
+      rise = e - vexp;
+      vexp = e;
+      const float down = as_f32((127 - vexp) << 23);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        ks[p] = *(const f32x4*)&lds_ks[buf][32 * h + 16 * p + 4 * kb];
+        vs[p] = *(const f32x4*)&lds_vs[buf][32 * h + 16 * p + 4 * kb] * down;
+      }
+    }
+    u32x4 pf[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      float top = kPaNoMax;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float z = s[x][i >> 2][i & 3] * (k8 ? row_scale[x] * ks[i >> 2][i & 3] : row_scale[x]);
+        if (cut) z = 16 * (i >> 2) + 4 * kb + (i & 3) < left ? z : -__builtin_inff();
+        s[x][i >> 2][i & 3] = z;
+        top = fmaxf(top, z);
+      }
+      if (__any(top > m[x] + kPaSlack)) {
+        const float up = fmaxf(m[x], max_over_kb(top));
+        const float alpha = __builtin_amdgcn_exp2f(m[x] - up);
+        m[x] = up;
+        l[x] *= alpha;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[x][j] *= alpha;
+      }
+      if (k8 && rise > 0) {
+        const float alpha = rise > 126 ? 0.0f : as_f32((127 - rise) << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[x][j] *= alpha;
+      }
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(s[x][i >> 2][i & 3] - m[x]);
+        l[x] += w[i];
+        if (k8) w[i] *= vs[i >> 2][i & 3];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[x][i] = pack2<MT>(w[2 * i], w[2 * i + 1]);
+    }
+    u32x4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int in_page = 4 * kb + (i & 3);
+      v[i] = vt[(16 * (i >> 2) + in_page) * 16 + (n ^ in_page)];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      u32x4 lo, hi;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x05040100u);
+        hi[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x07060302u);
+      }
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        o[x][2 * c] = mfma16<MT>(lo, pf[x], o[x][2 * c]);
+        o[x][2 * c + 1] = mfma16<MT>(hi, pf[x], o[x][2 * c + 1]);
+      }
+    }
+  };
+
+  fetch(0, false);
+  stage(0, false);
+  fetch(0, true);
+  stage(0, true);
+  __syncthreads();
+  // all tiles but the last are whole, and a tile follows them
+  for (int t = 0; t + 1 < tiles; ++t) {
+    fetch(t + 1, false);
+    if (busy) products(t, 0, Never{});
+    stage(t + 1, false);
+    fetch(t + 1, true);
+    if (busy) products(t, 1, Never{});
+    stage(t + 1, true);
+    __syncthreads();
+  }
+  if (busy) {
+    products(tiles - 1, 0, Always{});
+    products(tiles - 1, 1, Always{});
+  }
+
+  const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const float total = sum_over_kb(l[x]);
+    const int row = row_of((wave * NQ + x) * 16 + n);
+    if (row < 0) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4)
+        put_row<QT>(a, row, part, parts, 32 * kb + 8 * i + j,
+                    f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]} * vfac, m[x], total);
+  }
+}
+
+// Ways to attend to a prefix part.
+enum PrefixMode { kStream16, kStream32, kStream64, kStaged };
+constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStream32 ? 32 : mode == kStream64 ? 64 : kStRows; }
+
+// Grid: the prefix parts (eight of (kv head, part, group), row tile, the next eight, ...: the row tiles
+// of a part run side by side on one XCD and find its K and V in that L2), then the own parts (kv head,
+// part, request, row tile).
+template <int QT, int KV, int MODE>
+__global__ __launch_bounds__(kPaThreads, MODE == kStream16 ? (KV == TWL_I8 ? 3 : 4) : 2) void prefix_attn_kernel(PrefixAttnArgs a) {
   const uint32_t parts = a.p_chunks + a.chunks;
   uint32_t id = blockIdx.x;
   if (id < a.p_blocks) {
+    const uint32_t tile = (id >> 3) % a.p_tiles;
+    id = (id >> 3) / a.p_tiles * 8 + (id & 7);
     const uint32_t kvh = id % a.num_kv_heads;
     id /= a.num_kv_heads;
-    const uint32_t c = id % a.p_chunks;
-    id /= a.p_chunks;
-    const uint32_t g = id % a.groups, tile = id / a.groups;
+    const uint32_t c = id % a.p_chunks, g = id / a.p_chunks;
+    if (g >= a.groups) return;              // the last eight may be short
     const int first = max(a.g_ptr[g], 0);
     const int members = min(min((int)a.batch, a.g_ptr[g + 1]) - first, (int)a.max_group);
-    const int rows = members * (int)a.G, row0 = (int)(tile * 16 * NQ * WR);
+    const int rows = members * (int)a.G, row0 = (int)tile * mode_rows(MODE);
     const int len = list_len(a.p_ptr, a.p_last, g, a.max_prefix);
     const int begin = (int)(c * a.p_chunk), end = min(len, begin + (int)a.p_chunk);
     if (begin >= end || row0 >= rows) return;
@@ -498,8 +744,13 @@ __global__ __launch_bounds__(kPaThreads) void prefix_attn_kernel(PrefixAttnArgs 
       const int b = lr / (int)a.G;
       return (int)((first + b) * a.num_q_heads + kvh * a.G) + lr - b * (int)a.G;
     };
-    attend_part<QT, KV, NQ, WR>(a, a.p_ids + a.p_ptr[g], a.p_ptr[g + 1] - a.p_ptr[g], begin, end,
-                                kvh, row_of, c, parts);
+    const int32_t* ids = a.p_ids + a.p_ptr[g];
+    const int num_ids = a.p_ptr[g + 1] - a.p_ptr[g];
+    if constexpr (MODE == kStaged)
+      attend_staged<QT, KV>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts);
+    else
+      attend_part<QT, KV, MODE == kStream16 ? 1 : 2, MODE == kStream64 ? 2 : 1>(a, ids, num_ids, begin, end, kvh,
+                                                                                row_of, c, parts);
   } else {
     id -= a.p_blocks;
     const uint32_t kvh = id % a.num_kv_heads;
@@ -575,7 +826,7 @@ __global__ __launch_bounds__(kPaThreads) void prefix_attn_merge_kernel(PrefixAtt
 
 // How a call is cut into workgroups: from the sizes alone, the same for the workspace and the launch.
 struct PrefixPlan {
-  uint32_t nq, wr;                          // sets of 16 rows per wavefront, wavefronts across rows
+  int mode;
   uint32_t p_chunk, p_chunks, p_tiles, chunk, chunks, tiles;
 };
 
@@ -601,10 +852,8 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
   PrefixPlan p{};
   const uint32_t G = num_q_heads / num_kv_heads;
   const uint64_t rows = (uint64_t)max_group * G;
-  p.nq = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p.wr = rows <= 64 ? 1 : rows <= 128 ? 2 : 4;
-  const uint32_t per = 16 * p.nq * p.wr;
-  p.p_tiles = (uint32_t)((rows + per - 1) / per);
+  p.mode = rows <= 16 ? kStream16 : rows <= 32 ? kStream32 : rows <= 64 ? kStream64 : kStaged;
+  p.p_tiles = (uint32_t)((rows + mode_rows(p.mode) - 1) / mode_rows(p.mode));
   p.tiles = (G + 15) / 16;
   cut_tokens(groups ? max_prefix : 0, (uint64_t)num_kv_heads * groups * p.p_tiles, 512, 128, &p.p_chunk,
              &p.p_chunks);
@@ -614,13 +863,12 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
 
 template <int QT, int KV>
 static void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& p, uint32_t blocks, hipStream_t st) {
-#define TWL_PA(NQ, WR) \
-  hipLaunchKernelGGL((prefix_attn_kernel<QT, KV, NQ, WR>), dim3(blocks), dim3(kPaThreads), 0, st, a)
-  if (a.p_chunks == 0 || p.nq == 1) TWL_PA(1, 1);
-  else if (p.nq == 2) TWL_PA(2, 1);
-  else if (p.wr == 1) TWL_PA(4, 1);
-  else if (p.wr == 2) TWL_PA(4, 2);
-  else TWL_PA(4, 4);
+#define TWL_PA(MODE) \
+  hipLaunchKernelGGL((prefix_attn_kernel<QT, KV, MODE>), dim3(blocks), dim3(kPaThreads), 0, st, a)
+  if (a.p_chunks == 0 || p.mode == kStream16) TWL_PA(kStream16);
+  else if (p.mode == kStream32) TWL_PA(kStream32);
+  else if (p.mode == kStream64) TWL_PA(kStream64);
+  else TWL_PA(kStaged);
 #undef TWL_PA
 }
 
@@ -678,7 +926,7 @@ extern "C" int twl_prefix_attn(
                                                         max_prefix_tokens, max_group_size, max_tokens);
   if (need && !workspace) return TWL_ENULL;
   if (workspace_bytes < need) return TWL_EINVAL;
-  const uint64_t p_blocks = (uint64_t)num_kv_heads * p.p_chunks * groups * p.p_tiles;
+  const uint64_t p_blocks = ((uint64_t)num_kv_heads * p.p_chunks * groups + 7) / 8 * 8 * p.p_tiles;
   const uint64_t blocks = p_blocks + (uint64_t)num_kv_heads * p.chunks * batch * p.tiles;
   if (blocks > 0x7FFFFFFFull) return TWL_EINVAL;
   const uint64_t parts = (uint64_t)p.p_chunks + p.chunks, rows = (uint64_t)batch * num_q_heads;
@@ -688,7 +936,10 @@ extern "C" int twl_prefix_attn(
   a.v = (const uint8_t*)v_cache; a.page_bytes = page_stride * eb; a.head_bytes = head_stride * eb;
   a.token_bytes = (uint32_t)(token_stride * eb); a.ks = k_scale; a.vs = v_scale;
   a.scale_page = scale_page_stride; a.scale_head = scale_head_stride;
-  a.scale_token = (uint32_t)scale_token_stride; a.num_pages = num_pages;
+  a.scale_token = (uint32_t)scale_token_stride;
+  a.scale_vec = scale_token_stride == 1 && ((scale_page_stride | scale_head_stride) & 3u) == 0 &&
+                ((((uintptr_t)k_scale) | ((uintptr_t)v_scale)) & 15u) == 0;
+  a.num_pages = num_pages;
   a.p_ids = prefix_page_indices; a.p_ptr = prefix_page_indptr; a.p_last = prefix_last_page_len;
   a.g_ptr = group_indptr; a.ids = kv_page_indices; a.ptr = kv_page_indptr; a.last = kv_last_page_len;
   a.batch = batch; a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads;
