@@ -7,9 +7,12 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._check import check_dim, check_dtype, check_input, check_same_device, dtype_code, ptr, stream_of
+from ._check import (check_dim, check_dtype, check_input, check_same_device, fine_rows, ptr,
+                     stream_and_switch)
 from .attention import _cache_strides
-from .quant_cache import check_page_table, check_quant_cache
+from .quant_cache import KV_FORMATS, check_page_table, check_quant_cache
+
+_QUERY_TYPES = {torch.float16: _lib.TWL_F16, torch.bfloat16: _lib.TWL_BF16}
 
 
 def prefix_attention_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, groups: int,
@@ -28,26 +31,46 @@ def _bound(value, name: str, least: int) -> int:
     return value
 
 
-def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_page_indptr,
-            kv_last_page_len, max_tokens, sm_scale, return_lse, out, workspace, what):
+def _fine(q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len) -> bool:
+    """Whether the operands are plainly right; if not, :func:`_check` finds out what is wrong."""
+    dev, cs = q.device, k_cache.stride()
+    if not (q.is_cuda and q.dim() == 3 and q.is_contiguous() and q.dtype in _QUERY_TYPES and len(cs) == 4
+            and v_cache.stride() == cs and cs[3] == 1 and v_cache.shape == k_cache.shape
+            and v_cache.dtype is k_cache.dtype and k_cache.device == dev and v_cache.device == dev):
+        return False
+    B, H, D = q.shape
+    pages, page, Hkv, Dk = k_cache.shape
+    if not (D == Dk == _lib.HEAD_DIM and page == _lib.PAGE and B and H and pages and Hkv and H % Hkv == 0
+            and kv_page_indptr.numel() == B + 1 and kv_last_page_len.numel() == B
+            and fine_rows(dev, torch.int32, kv_page_indices, kv_page_indptr, kv_last_page_len)):
+        return False
+    if k_scale is None:
+        return v_scale is None and k_cache.dtype is q.dtype
+    return (v_scale is not None and k_cache.dtype in KV_FORMATS and k_scale.dtype is torch.float32
+            and v_scale.dtype is torch.float32 and k_scale.shape == k_cache.shape[:3]
+            and v_scale.shape == k_scale.shape and k_scale.stride() == v_scale.stride()
+            and k_scale.device == dev and v_scale.device == dev)
+
+
+def _check(q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len) -> None:
     check_input(q, "q"); check_dim(3, q, "q")
     B, H, D = q.shape
     if D != _lib.HEAD_DIM:
         raise RuntimeError(f"head_dim must be {_lib.HEAD_DIM}, got {D}")
     if B == 0 or H == 0:
         raise RuntimeError("q must not be empty")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    if q.dtype not in _QUERY_TYPES:
         raise RuntimeError("q must be float16 or bfloat16")
     if (k_scale is None) != (v_scale is None):
         raise RuntimeError("k_scale and v_scale go together")
     if k_scale is None:
-        cs, ss, fmt = _cache_strides(k_cache, "k_cache"), (0, 0, 0), dtype_code(q.dtype, "q")
+        cs = _cache_strides(k_cache, "k_cache")
         if _cache_strides(v_cache, "v_cache") != cs or k_cache.shape != v_cache.shape:
             raise RuntimeError("k_cache and v_cache must share shape and strides")
         if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
             raise RuntimeError("q, k_cache and v_cache must share one dtype (8-bit pages need k_scale and v_scale)")
     else:
-        fmt, cs, ss = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
+        check_quant_cache(k_cache, v_cache, k_scale, v_scale)
     Hkv = k_cache.size(2)
     if Hkv == 0 or H % Hkv != 0:
         raise RuntimeError(f"num_q_heads {H} must be a multiple of num_kv_heads {Hkv}")
@@ -55,31 +78,48 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
         raise RuntimeError("the cache must hold a page")
     check_same_device(q, ("k_cache", k_cache), ("v_cache", v_cache))
     check_page_table(q, B, kv_page_indices, kv_page_indptr, kv_last_page_len)
+
+
+def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_page_indptr,
+            kv_last_page_len, max_tokens, sm_scale, return_lse, out, workspace, what):
+    """The launch; the operands have been checked."""
+    B, H, D = q.shape
+    Hkv, dev, dtype = k_cache.size(2), q.device, q.dtype
+    cs = k_cache.stride()
+    if k_scale is None:
+        ss, fmt = (0, 0, 0), _QUERY_TYPES[dtype]
+    else:
+        ss, fmt = k_scale.stride(), KV_FORMATS[k_cache.dtype]
+    stream, switch = stream_and_switch(dev)
+    if switch:
+        with torch.cuda.device(dev):
+            return _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_page_indptr,
+                           kv_last_page_len, max_tokens, sm_scale, return_lse, out, workspace, what)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        check_input(out, "out"); check_same_device(q, ("out", out))
+        if out.shape != q.shape or out.dtype != dtype:
+            raise RuntimeError("out must match q")
+    lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     p_ids, p_ptr, p_last, g_ptr, groups, max_prefix, max_group = prefix
-    dev = q.device
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty_like(q)
-        else:
-            check_input(out, "out"); check_same_device(q, ("out", out))
-            if out.shape != q.shape or out.dtype != q.dtype:
-                raise RuntimeError("out must match q")
-        lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
-        scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-        need = prefix_attention_workspace_bytes(B, H, Hkv, groups, max_prefix, max_group, max_tokens)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        else:
-            check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
-            if workspace.numel() < need or workspace.device != dev:
-                raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
-        rc = _lib.lib().twl_prefix_attn(
-            ptr(q), ptr(out), dtype_code(q.dtype, "q"), ptr(k_cache), ptr(v_cache), fmt, *cs,
-            ptr(k_scale), ptr(v_scale), *ss, k_cache.size(0), ptr(p_ids), ptr(p_ptr), ptr(p_last),
-            ptr(g_ptr), groups, max_prefix, max_group, ptr(kv_page_indices), ptr(kv_page_indptr),
-            ptr(kv_last_page_len), max_tokens, B, H, Hkv, scale, ptr(lse), ptr(workspace),
-            workspace.numel(), stream_of(q))
-    _lib.check(rc, what)
+    L = _lib.lib()
+    need = L.twl_prefix_attn_workspace_bytes(B, H, Hkv, groups, max_prefix, max_group, max_tokens)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
+        if workspace.numel() < need or workspace.device != dev:
+            raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
+    rc = L.twl_prefix_attn(
+        q.data_ptr(), out.data_ptr(), _QUERY_TYPES[dtype], k_cache.data_ptr(), v_cache.data_ptr(), fmt, cs[0], cs[1],
+        cs[2], ptr(k_scale), ptr(v_scale), *ss, k_cache.size(0), ptr(p_ids), ptr(p_ptr), ptr(p_last), ptr(g_ptr),
+        groups, max_prefix, max_group, kv_page_indices.data_ptr(), kv_page_indptr.data_ptr(),
+        kv_last_page_len.data_ptr(), max_tokens, B, H, Hkv, scale, ptr(lse), workspace.data_ptr(), workspace.numel(),
+        stream)
+    if rc:
+        _lib.check(rc, what)
     return (out, lse) if return_lse else out
 
 
@@ -102,6 +142,9 @@ def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     calls on one stream may share; by default a fresh one is allocated."""
     if k_scale is None or v_scale is None:
         raise RuntimeError("8-bit pages need k_scale and v_scale")
+    operands = (q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    if not _fine(*operands):
+        _check(*operands)
     return _attend(q, k_cache, v_cache, k_scale, v_scale, (None, None, None, None, 0, 0, 0),
                    kv_page_indices, kv_page_indptr, kv_last_page_len, _bound(max_tokens, "max_tokens", 1),
                    sm_scale, return_lse, out, workspace, "QuantPagedDecodeAttention")
@@ -131,14 +174,21 @@ def prefix_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     :func:`quant_paged_decode_attention`. ``max_prefix_tokens``, ``max_group_size`` and ``max_tokens``
     are upper bounds that size the launch: tokens beyond them are not attended to, members of a
     group beyond the second do not see its prefix. Returns ``out`` (and ``lse``) as there."""
-    check_input(group_indptr, "group_indptr"); check_dtype(group_indptr, torch.int32, "group_indptr")
-    groups = group_indptr.numel() - 1
-    if groups < 1 or groups > q.size(0):
-        raise RuntimeError("group_indptr must have groups + 1 elements, with 1 to batch groups")
-    check_same_device(q, ("group_indptr", group_indptr))
-    check_page_table(q, groups, prefix_page_indices, prefix_page_indptr, prefix_last_page_len, "prefix")
+    operands = (q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    if not _fine(*operands):
+        _check(*operands)
+    groups, batch = group_indptr.numel() - 1, q.size(0)
+    if not (1 <= groups <= batch and prefix_page_indptr.numel() == groups + 1
+            and prefix_last_page_len.numel() == groups
+            and fine_rows(q.device, torch.int32, group_indptr, prefix_page_indices, prefix_page_indptr,
+                          prefix_last_page_len)):
+        check_input(group_indptr, "group_indptr"); check_dtype(group_indptr, torch.int32, "group_indptr")
+        if groups < 1 or groups > batch:
+            raise RuntimeError("group_indptr must have groups + 1 elements, with 1 to batch groups")
+        check_same_device(q, ("group_indptr", group_indptr))
+        check_page_table(q, groups, prefix_page_indices, prefix_page_indptr, prefix_last_page_len, "prefix")
     max_group = _bound(max_group_size, "max_group_size", 1)
-    if max_group > q.size(0):
+    if max_group > batch:
         raise RuntimeError("max_group_size must not exceed the batch")
     prefix = (prefix_page_indices, prefix_page_indptr, prefix_last_page_len, group_indptr, groups,
               _bound(max_prefix_tokens, "max_prefix_tokens", 0), max_group)

@@ -6,18 +6,19 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ._check import (check_cuda, check_dim, check_dtype, check_input, check_same_device, dtype_code, ptr,
-                     stream_of)
+from ._check import (check_cuda, check_dim, check_dtype, check_input, check_same_device, dtype_code, fine_rows,
+                     stream_and_switch)
 from .attention import _cache_strides
 
-_FORMATS = {torch.int8: _lib.TWL_I8, torch.float8_e4m3fn: _lib.TWL_E4M3}
+_ROW_TYPES = {torch.float16: _lib.TWL_F16, torch.bfloat16: _lib.TWL_BF16}
+KV_FORMATS = {torch.int8: _lib.TWL_I8, torch.float8_e4m3fn: _lib.TWL_E4M3}
 
 
 def kv_format_code(dt: torch.dtype, name: str) -> int:
     """Library code of an 8-bit page format."""
-    if dt not in _FORMATS:
+    if dt not in KV_FORMATS:
         raise RuntimeError(f"{name}: 8-bit pages are int8 or float8_e4m3fn, got {dt}")
-    return _FORMATS[dt]
+    return KV_FORMATS[dt]
 
 
 def check_quant_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -58,6 +59,19 @@ def _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_las
     return batch
 
 
+def _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len) -> bool:
+    """Whether a cache and its tables are plainly right; if not, the checks above find out what is wrong."""
+    dev, cs, batch = k_cache.device, k_cache.stride(), token_indptr.numel() - 1
+    return (k_cache.is_cuda and len(cs) == 4 and cs[3] == 1 and k_cache.size(1) == _lib.PAGE
+            and k_cache.size(3) == _lib.HEAD_DIM and k_cache.dtype in KV_FORMATS and v_cache.dtype is k_cache.dtype
+            and v_cache.stride() == cs and v_cache.shape == k_cache.shape and v_cache.device == dev
+            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+            and k_scale.shape == k_cache.shape[:3] and v_scale.shape == k_scale.shape
+            and k_scale.stride() == v_scale.stride() and k_scale.device == dev and v_scale.device == dev
+            and batch >= 1 and kv_page_indptr.numel() == batch + 1 and kv_last_page_len.numel() == batch
+            and fine_rows(dev, torch.int32, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len))
+
+
 def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torch.Tensor,
                     k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, kv_page_indices: torch.Tensor,
@@ -72,27 +86,37 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
     last tokens of request b: the page table counts them already. Rows from ``token_indptr[B]`` on are
     ignored; rows that have no place in the table are skipped. A page that is written must belong
     to one request only. A row with a non-finite element reads back as NaN."""
-    fmt, cs, ss = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
-    Hkv = k_cache.size(2)
-    for name, t in (("k_new", k_new), ("v_new", v_new)):
-        check_cuda(t, name); check_dim(3, t, name)
-        if t.size(1) != Hkv or t.size(2) != _lib.HEAD_DIM or t.stride(2) != 1:
-            raise RuntimeError(f"{name} must be [T, {Hkv}, {_lib.HEAD_DIM}] with contiguous head_dim")
-        if t.dtype not in (torch.float16, torch.bfloat16):
-            raise RuntimeError(f"{name} must be float16 or bfloat16")
-    if v_new.shape != k_new.shape or v_new.stride() != k_new.stride() or v_new.dtype != k_new.dtype:
-        raise RuntimeError("k_new and v_new must share shape, dtype and strides")
-    batch = _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
-    check_same_device(k_cache, ("k_new", k_new), ("v_new", v_new))
+    if not _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len):
+        check_quant_cache(k_cache, v_cache, k_scale, v_scale)
+        _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    dev, Hkv, ns = k_cache.device, k_cache.size(2), k_new.stride()
+    if not (k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and len(ns) == 3 and ns[2] == 1 and k_new.dtype in _ROW_TYPES
+            and v_new.shape == k_new.shape and v_new.stride() == ns and v_new.dtype is k_new.dtype
+            and k_new.device == dev and v_new.device == dev):
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            check_cuda(t, name); check_dim(3, t, name)
+            if t.size(1) != Hkv or t.size(2) != _lib.HEAD_DIM or t.stride(2) != 1:
+                raise RuntimeError(f"{name} must be [T, {Hkv}, {_lib.HEAD_DIM}] with contiguous head_dim")
+            if t.dtype not in _ROW_TYPES:
+                raise RuntimeError(f"{name} must be float16 or bfloat16")
+        if v_new.shape != k_new.shape or v_new.stride() != k_new.stride() or v_new.dtype != k_new.dtype:
+            raise RuntimeError("k_new and v_new must share shape, dtype and strides")
+        check_same_device(k_cache, ("k_new", k_new), ("v_new", v_new))
     if k_new.size(0) == 0:
         return
-    with torch.cuda.device(k_cache.device):
-        rc = _lib.lib().twl_kv_quant_append(
-            ptr(k_new), ptr(v_new), dtype_code(k_new.dtype, "k_new"), k_new.stride(0), k_new.stride(1),
-            ptr(token_indptr), k_new.size(0), ptr(k_cache), ptr(v_cache), fmt, *cs, ptr(k_scale),
-            ptr(v_scale), *ss, k_cache.size(0), ptr(kv_page_indices), ptr(kv_page_indptr),
-            ptr(kv_last_page_len), batch, Hkv, stream_of(k_cache))
-    _lib.check(rc, "KvQuantAppend")
+    stream, switch = stream_and_switch(dev)
+    if switch:
+        with torch.cuda.device(dev):
+            return kv_quant_append(k_new, v_new, token_indptr, k_cache, v_cache, k_scale, v_scale, kv_page_indices,
+                                   kv_page_indptr, kv_last_page_len)
+    cs, ss = k_cache.stride(), k_scale.stride()
+    rc = _lib.lib().twl_kv_quant_append(
+        k_new.data_ptr(), v_new.data_ptr(), _ROW_TYPES[k_new.dtype], ns[0], ns[1], token_indptr.data_ptr(),
+        k_new.size(0), k_cache.data_ptr(), v_cache.data_ptr(), KV_FORMATS[k_cache.dtype], cs[0], cs[1], cs[2],
+        k_scale.data_ptr(), v_scale.data_ptr(), *ss, k_cache.size(0), kv_page_indices.data_ptr(),
+        kv_page_indptr.data_ptr(), kv_last_page_len.data_ptr(), token_indptr.numel() - 1, Hkv, stream)
+    if rc:
+        _lib.check(rc, "KvQuantAppend")
 
 
 def kv_quant_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -105,29 +129,36 @@ def kv_quant_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
     of them when ``token_indptr`` adds up the requests' lengths). Arguments as in
     :func:`kv_quant_append`. Rows from ``token_indptr[B]`` on are left as they were (undefined in
     outputs this call allocates); rows that have no place in the table are zeros."""
-    fmt, cs, ss = check_quant_cache(k_cache, v_cache, k_scale, v_scale)
-    Hkv = k_cache.size(2)
-    batch = _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
-    tokens = int(tokens)
+    if not _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len):
+        check_quant_cache(k_cache, v_cache, k_scale, v_scale)
+        _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    dev, Hkv, tokens = k_cache.device, k_cache.size(2), int(tokens)
     if tokens < 0:
         raise RuntimeError("tokens must not be negative")
-    code, dev = dtype_code(dtype, "dtype"), k_cache.device
-    outs = []
-    with torch.cuda.device(dev):
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t is None:
-                t = torch.empty((tokens, Hkv, _lib.HEAD_DIM), dtype=dtype, device=dev)
-            else:
-                check_input(t, name)
-                if tuple(t.shape) != (tokens, Hkv, _lib.HEAD_DIM) or t.dtype != dtype:
-                    raise RuntimeError(f"{name} must be [{tokens}, {Hkv}, {_lib.HEAD_DIM}] of {dtype}")
-                check_same_device(k_cache, (name, t))
-            outs.append(t)
-        if tokens == 0:
-            return outs[0], outs[1]
-        rc = _lib.lib().twl_kv_quant_read(
-            ptr(outs[0]), ptr(outs[1]), code, ptr(token_indptr), tokens, ptr(k_cache), ptr(v_cache), fmt,
-            *cs, ptr(k_scale), ptr(v_scale), *ss, k_cache.size(0), ptr(kv_page_indices),
-            ptr(kv_page_indptr), ptr(kv_last_page_len), batch, Hkv, stream_of(k_cache))
-    _lib.check(rc, "KvQuantRead")
-    return outs[0], outs[1]
+    code = dtype_code(dtype, "dtype")
+    stream, switch = stream_and_switch(dev)
+    if switch:
+        with torch.cuda.device(dev):
+            return kv_quant_read(k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len,
+                                 token_indptr, tokens, dtype, k_out, v_out)
+    shape = (tokens, Hkv, _lib.HEAD_DIM)
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is not None:
+            check_input(t, name); check_same_device(k_cache, (name, t))
+            if tuple(t.shape) != shape or t.dtype != dtype:
+                raise RuntimeError(f"{name} must be {list(shape)} of {dtype}")
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=dev)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=dtype, device=dev)
+    if tokens == 0:
+        return k_out, v_out
+    cs, ss = k_cache.stride(), k_scale.stride()
+    rc = _lib.lib().twl_kv_quant_read(
+        k_out.data_ptr(), v_out.data_ptr(), code, token_indptr.data_ptr(), tokens, k_cache.data_ptr(),
+        v_cache.data_ptr(), KV_FORMATS[k_cache.dtype], cs[0], cs[1], cs[2], k_scale.data_ptr(), v_scale.data_ptr(),
+        *ss, k_cache.size(0), kv_page_indices.data_ptr(), kv_page_indptr.data_ptr(), kv_last_page_len.data_ptr(),
+        token_indptr.numel() - 1, Hkv, stream)
+    if rc:
+        _lib.check(rc, "KvQuantRead")
+    return k_out, v_out

@@ -11,8 +11,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _lib
-from ._check import (check_dim, check_dtype, check_input, check_same_device, dtype_code, ptr,
-                     stream_of)
+from ._check import (check_dim, check_dtype, check_input, check_same_device, dtype_code, fine_rows, ptr,
+                     stream_and_switch, stream_of)
 
 _HIGH = {"first": _lib.TWL_HIGH_FIRST, "max": _lib.TWL_HIGH_MAX}
 
@@ -191,17 +191,18 @@ def softmax_top_p(scores: torch.Tensor, top_p: Union[torch.Tensor, float],
 
 
 def _row_filter(value, name: str, rows: int, ref: torch.Tensor, dtype: torch.dtype, lo: float, hi: float):
-    """A filter of :func:`sample_tokens`: one number for every row, or a tensor with one per row."""
+    """A filter of :func:`sample_tokens`: one number for every row, or a tensor with one per row.
+    Returns its pointer (0: a number) and the number."""
     if isinstance(value, torch.Tensor):
-        check_input(value, name); check_dtype(value, dtype, name)
-        check_same_device(ref, (name, value))
-        if value.numel() != rows:
+        if value.numel() != rows or not fine_rows(ref.device, dtype, value):
+            check_input(value, name); check_dtype(value, dtype, name)
+            check_same_device(ref, (name, value))
             raise RuntimeError(f"{name} tensor must have one element per row ({rows})")
-        return value, 0
-    value = int(value) if dtype == torch.int32 else float(value)
+        return value.data_ptr(), 0
+    value = int(value) if dtype is torch.int32 else float(value)
     if not lo <= value <= hi:
         raise RuntimeError(f"{name} must be in [{lo}, {hi}], got {value}")
-    return None, value
+    return 0, value
 
 
 def sample_tokens_workspace_bytes(rows: int, vocab: int) -> int:
@@ -235,32 +236,35 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
         raise RuntimeError("logits must have 1 to 65535 rows and 1 to 262144 columns")
     if vocab > 1 and logits.stride(1) != 1:
         raise RuntimeError("logits must be contiguous along the vocabulary")
-    code = dtype_code(logits.dtype, "logits")
-    check_input(u, "u"); check_dtype(u, torch.float32, "u"); check_same_device(logits, ("u", u))
-    if u.numel() != rows:
+    code, dev = dtype_code(logits.dtype, "logits"), logits.device
+    if u.numel() != rows or not fine_rows(dev, torch.float32, u):
+        check_input(u, "u"); check_dtype(u, torch.float32, "u"); check_same_device(logits, ("u", u))
         raise RuntimeError(f"u must have one element per row ({rows})")
     f32 = torch.float32
     t_arr, t_val = _row_filter(temperature, "temperature", rows, logits, f32, 0.0, 3e38)
     k_arr, k_val = _row_filter(top_k, "top_k", rows, logits, torch.int32, 0, 2 ** 31 - 1)
     p_arr, p_val = _row_filter(top_p, "top_p", rows, logits, f32, 0.0, 1.0)
     m_arr, m_val = _row_filter(min_p, "min_p", rows, logits, f32, 0.0, 1.0)
-    with torch.cuda.device(logits.device):
-        if out is None:
-            out = torch.empty(rows, dtype=torch.int64, device=logits.device)
-        else:
-            check_input(out, "out"); check_dtype(out, torch.int64, "out")
-            check_same_device(logits, ("out", out))
-            if out.numel() != rows:
-                raise RuntimeError(f"out must have one element per row ({rows})")
-        need = sample_tokens_workspace_bytes(rows, vocab)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        else:
-            check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
-            if workspace.numel() < need or workspace.device != logits.device:
-                raise RuntimeError(f"workspace must hold {need} bytes on {logits.device}")
-        rc = _lib.lib().twl_sample_tokens(
-            ptr(logits), code, logits.stride(0), rows, vocab, ptr(u), ptr(t_arr), t_val, ptr(k_arr), k_val,
-            ptr(p_arr), p_val, ptr(m_arr), m_val, ptr(out), ptr(workspace), workspace.numel(), stream_of(logits))
-    _lib.check(rc, "SampleTokens")
+    stream, switch = stream_and_switch(dev)
+    if switch:
+        with torch.cuda.device(dev):
+            return sample_tokens(logits, u, temperature, top_k, top_p, min_p, out, workspace)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    elif out.numel() != rows or not fine_rows(dev, torch.int64, out):
+        check_input(out, "out"); check_dtype(out, torch.int64, "out")
+        check_same_device(logits, ("out", out))
+        raise RuntimeError(f"out must have one element per row ({rows})")
+    need = sample_tokens_workspace_bytes(rows, vocab)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
+        if workspace.numel() < need or workspace.device != dev:
+            raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
+    rc = _lib.lib().twl_sample_tokens(
+        logits.data_ptr(), code, logits.stride(0), rows, vocab, u.data_ptr(), t_arr, t_val, k_arr, k_val, p_arr,
+        p_val, m_arr, m_val, out.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
+    if rc:
+        _lib.check(rc, "SampleTokens")
     return out
