@@ -71,16 +71,14 @@ struct SampleCut {
   int32_t bin, pad;
 };
 
-template <int DT>
-__device__ __forceinline__ float masked_logit(float x) {
-  return x != x ? -__builtin_inff() : x + 0.0f;   // NaN counts as masked; -0 ranks as +0
-}
+// NaN counts as masked; -0 ranks as +0
+__device__ __forceinline__ float masked_logit(float x) { return fmaxf(x, -__builtin_inff()) + 0.0f; }
 template <int DT>
 __device__ __forceinline__ float logit_at(const SampleArgs& a, uint32_t row, uint32_t i) {
   float x;
   if (DT == TWL_F32) x = ((const float*)a.logits)[row * a.row_stride + i];
   else x = bits16_to_f32<DT>(((const uint16_t*)a.logits)[row * a.row_stride + i]);
-  return masked_logit<DT>(x);
+  return masked_logit(x);
 }
 // Eight consecutive logits from i on; -inf behind the vocabulary.
 template <int DT>
@@ -96,7 +94,7 @@ __device__ __forceinline__ void logits8(const SampleArgs& a, uint32_t row, uint3
       unpack8<DT>(*(const u32x4*)p, x);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = masked_logit<DT>(x[j]);
+    for (int j = 0; j < 8; ++j) x[j] = masked_logit(x[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = i + j < a.vocab ? logit_at<DT>(a, row, i + j) : -__builtin_inff();
@@ -112,25 +110,51 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 }
 constexpr uint32_t kKeyNone = 0x007FFFFFu;     // key_of(-inf)
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v = max(v, (uint64_t)__shfl_xor(v, d));
-  return v;
+// ---- 64-bit values across a wavefront, by DPP (a scan step is a few cycles; through LDS it is a
+// hundred) ------------------------------------------------------------------------------------
+template <int CTRL, int ROW_MASK, class T>
+__device__ __forceinline__ T dpp64(T v) {        // 0 where there is no source
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)dpp<CTRL, ROW_MASK>(0, (int)(uint32_t)u);
+  const uint32_t hi = (uint32_t)dpp<CTRL, ROW_MASK>(0, (int)(uint32_t)(u >> 32));
+  return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
 }
 template <class T>
-__device__ __forceinline__ T wave_scan(T v) {   // inclusive, in lane order
-  const int lane = lane_id();
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const T x = __shfl_up(v, d);
-    if (lane >= d) v += x;
-  }
+__device__ __forceinline__ T lane63(T v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {    // inclusive, in lane order
+  T t;
+  t = dpp64<0x111, 0xF>(v); v += t;
+  t = dpp64<0x112, 0xF>(v); v += t;
+  t = dpp64<0x114, 0xF>(v); v += t;
+  t = dpp64<0x118, 0xF>(v); v += t;
+  t = dpp64<kDppBcast15, 0xA>(v); v += t;
+  t = dpp64<kDppBcast31, 0xC>(v); v += t;
   return v;
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return lane63(wave_scan(v)); }
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  v = max(v, dpp64<0x111, 0xF>(v));
+  v = max(v, dpp64<0x112, 0xF>(v));
+  v = max(v, dpp64<0x114, 0xF>(v));
+  v = max(v, dpp64<0x118, 0xF>(v));
+  v = max(v, dpp64<kDppBcast15, 0xA>(v));
+  v = max(v, dpp64<kDppBcast31, 0xC>(v));
+  return lane63(v);
+}
+__device__ __forceinline__ uint32_t wave_max32(uint32_t v) {
+  v = max(v, (uint32_t)dpp<0x111>(0, (int)v));
+  v = max(v, (uint32_t)dpp<0x112>(0, (int)v));
+  v = max(v, (uint32_t)dpp<0x114>(0, (int)v));
+  v = max(v, (uint32_t)dpp<0x118>(0, (int)v));
+  v = max(v, (uint32_t)dpp<kDppBcast15, 0xA>(0, (int)v));
+  v = max(v, (uint32_t)dpp<kDppBcast31, 0xC>(0, (int)v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // How a row is filtered.
@@ -152,35 +176,59 @@ __device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, uint32_t ro
   return f;
 }
 
-// w and its fixed-point form, for logits relative to `top`.
-//   2^z = 2^(n >> 6) * 2^((n & 63) / 64) * 2^f,   n = rint(64 z),  |f| <= 1/128
-// with the middle factor from a table and the last from its series to the fifth power
+// w and its fixed-point form, for logits relative to `top`. With z = 64 (x - top) log2(e) / T:
+//   2^(z / 64) = 2^(n >> 6) * 2^((n & 63) / 64) * 2^(f / 64),   n = rint(z),  |f| <= 1/2
+// with the middle factor from a table and the last from its series to the fifth power in f
 // (next term (ln 2 / 128)^6 / 720 < 4e-17).
 struct Weigher {
   const double* table;        // LDS, 2^(i / 64)
-  double top, per;            // per = log2(e) / T
-  __device__ __forceinline__ double z_of(float x) const { return x == top ? 0.0 : ((double)x - top) * per; }
-  __device__ __forceinline__ double exp2_of(double z) const {
-    z = fmax(z, -1000.0);
-    const double n = rint(z * 64.0);
-    const double f = fma(n, -1.0 / 64, z) * 0.693147180559945309417;
+  double top, per;            // per = 64 log2(e) / T
+  bool endless;               // the largest logit is infinite: it weighs 1, the others nothing
+  __device__ __forceinline__ Weigher(const double* t, float best, double T)
+      : table(t), top(best), per(92.3324826168936580 / T), endless(best == __builtin_inff()) {}
+  // x finite or -inf, not more than a few hundred T below top unless the result is not used
+  __device__ __forceinline__ double near(float x) const {
+    const double z = ((double)x - top) * per;
+    const double n = rint(z), f = z - n;
+    constexpr double c = 0.693147180559945309417 / 64;
     const int i = (int)n;
-    double y = fma(f, 1.0 / 120, 1.0 / 24);
-    y = fma(f, y, 1.0 / 6);
-    y = fma(f, y, 0.5);
-    y = fma(f, y, 1.0);
+    double y = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
+    y = fma(f, y, c * c * c / 6);
+    y = fma(f, y, c * c / 2);
+    y = fma(f, y, c);
     y = fma(f, y, 1.0);
     return __builtin_amdgcn_ldexp(y * table[i & 63], i >> 6);
   }
-  __device__ __forceinline__ double weight(float x) const { return exp2_of(z_of(x)); }
+  __device__ __forceinline__ double weight(float x) const {
+    if (endless) return x == __builtin_inff() ? 1.0 : 0.0;
+    return ((double)x - top) * per < -6400.0 ? 0.0 : near(x);
+  }
   static __device__ __forceinline__ uint64_t fixed(double w) {
     // adding 2^52 leaves the integer nearest w 2^45 in the low bits
-    return __builtin_bit_cast(uint64_t, fma(w, kSmpOne, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    return __builtin_bit_cast(uint64_t, fma(w, kSmpOne, 4503599627370496.0)) - 0x4330000000000000ull;
   }
   __device__ __forceinline__ uint64_t mass(float x) const { return fixed(weight(x)); }
 };
+__device__ const double kPow2[64] = {   // 2^(i / 64), rounded to nearest
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
+};
 __device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+  if (threadIdx.x < 64) table[threadIdx.x] = kPow2[threadIdx.x];
 }
 
 // Bins of width T / 16 from the best token's down: monotone in x, the same intervals for every slice.
@@ -195,11 +243,16 @@ __device__ __forceinline__ Binner binner(const RowFilter& f) {
   return Binner{fminf(fmaxf((float)(16.0 / f.T), 1e-37f), 1e30f)};
 }
 
+// Logits from here up weigh something; what is below weighs less than 2^-46 and may be left out.
+__device__ __forceinline__ float lowest_near(float top, double T) {
+  return fmaxf((float)((double)top - 40.0 * T), -__FLT_MAX__);
+}
+
 // ---- first launch ------------------------------------------------------------------------------
 template <int DT, int ITERS>
 __global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) {
   __shared__ uint64_t hist[kSmpBins];
-  __shared__ uint64_t wbest[kSmpWaves];
+  __shared__ uint32_t wbest[kSmpWaves], wat[kSmpWaves];
   __shared__ double table[64];
   const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const uint32_t first = slice * (ITERS * kSmpStep) + threadIdx.x * 8;
@@ -209,48 +262,78 @@ __global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) 
   const RowFilter f = row_filter(a, row);
   for (int i = threadIdx.x; i < kSmpBins; i += kSmpThreads) hist[i] = 0;
   fill_table(table);
-  // a thread's tokens ascend, so the first of equal ones is found by a strict comparison
   float m = -__builtin_inff();
-  uint32_t at = 0xFFFFFFFFu;
 #pragma unroll
   for (int t = 0; t < ITERS; ++t)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (x[t][j] > m) { m = x[t][j]; at = first + t * kSmpStep + j; }
-  uint64_t best = wave_max(((uint64_t)key_of(m) << 32) | (0xFFFFFFFFu - at));
-  if (lane_id() == 0) wbest[threadIdx.x / kWave] = best;
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, x[t][j]);
+  const uint32_t mine = wave_max32(key_of(m));
+  if (lane_id() == 0) wbest[threadIdx.x / kWave] = mine;
   __syncthreads();
+  uint32_t key = 0;
 #pragma unroll
-  for (int w = 0; w < kSmpWaves; ++w) best = max(best, wbest[w]);
+  for (int w = 0; w < kSmpWaves; ++w) key = max(key, wbest[w]);
   const size_t out = (size_t)row * a.slices + slice;
+  if (f.greedy) {
+    // where it is first
+    uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+    for (int t = ITERS - 1; t >= 0; --t)
+#pragma unroll
+      for (int j = 7; j >= 0; --j)
+        if (key_of(x[t][j]) == key) at = first + t * kSmpStep + j;
+    const uint32_t inv = wave_max32(0xFFFFFFFFu - at);
+    if (lane_id() == 0) wat[threadIdx.x / kWave] = inv;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t b = 0;
+      for (int w = 0; w < kSmpWaves; ++w) b = max(b, wat[w]);
+      a.best[out] = ((uint64_t)key << 32) | b;
+    }
+    return;
+  }
   if (threadIdx.x == 0) {
-    a.best[out] = best;
+    a.best[out] = (uint64_t)key << 32;
     if (slice == 0) a.cand_count[row] = 0;
   }
-  if (f.greedy || !(f.by_rank || f.by_mass) || (uint32_t)(best >> 32) <= kKeyNone) return;
-  const float top = key_value((uint32_t)(best >> 32));
-  const Weigher wt{table, top, 1.4426950408889634074 / f.T};
+  if (!(f.by_rank || f.by_mass) || key <= kKeyNone) return;
+  const float top = key_value(key);
+  const Weigher wt(table, top, f.T);
   const Binner bn = binner(f);
   const int top_bin = bn.bin(top);
+  const float low = lowest_near(top, f.T);
+  if (f.by_rank || wt.endless) {
 #pragma unroll
-  for (int t = 0; t < ITERS; ++t)
+    for (int t = 0; t < ITERS; ++t)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t rel = (uint32_t)(top_bin - bn.bin(x[t][j]));
-      if (rel < kSmpBins) {
-        const uint64_t v = f.by_rank ? (x[t][j] > -__builtin_inff() ? 1ull : 0ull) : wt.mass(x[t][j]);
-        atomicAdd((unsigned long long*)&hist[rel], (unsigned long long)v);
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t rel = (uint32_t)(top_bin - bn.bin(x[t][j]));
+        if (rel < kSmpBins && x[t][j] > -__builtin_inff())
+          atomicAdd((unsigned long long*)&hist[rel], f.by_rank ? 1ull : (unsigned long long)wt.mass(x[t][j]));
+      }
+  } else {
+#pragma unroll
+    for (int t = 0; t < ITERS; ++t) {
+      // eight at a time without a branch between them; saturated bins may hold anything, -inf among
+      // it, and `near` is for what is near
+      uint64_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = Weigher::fixed(wt.near(x[t][j]));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t rel = (uint32_t)(top_bin - bn.bin(x[t][j]));
+        if (rel < kSmpBins && x[t][j] >= low) atomicAdd((unsigned long long*)&hist[rel], (unsigned long long)v[j]);
       }
     }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < kSmpBins; i += kSmpThreads) a.hist[out * kSmpBins + i] = hist[i];
 }
 
-// best token of a row from its slices, by every thread
-__device__ __forceinline__ uint64_t row_best(const SampleArgs& a, uint32_t row) {
-  uint64_t b = 0;
-  for (uint32_t s = lane_id(); s < a.slices; s += kWave) b = max(b, a.best[(size_t)row * a.slices + s]);
-  return wave_max(b);
+// the best token of slice `lane` of a row (0: no such slice); there are at most kWave
+__device__ __forceinline__ uint64_t slice_best(const SampleArgs& a, uint32_t row) {
+  const uint32_t s = lane_id();
+  return s < a.slices ? a.best[(size_t)row * a.slices + s] : 0ull;
 }
 
 // ---- second launch -----------------------------------------------------------------------------
@@ -259,6 +342,8 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
   static_assert(kSmpBins == kSmpThreads, "one bin per thread");
   __shared__ uint64_t list[kSmpMaxCand];
   __shared__ double wsum[kSmpWaves], table[64];
+  __shared__ int slice_shift[64];
+  __shared__ double slice_weight[64];
   __shared__ double cut_before;
   __shared__ int cut_bin;
   __shared__ uint32_t list_n, list_at;
@@ -267,34 +352,41 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
   float x[ITERS][8];
 #pragma unroll
   for (int t = 0; t < ITERS; ++t) logits8<DT>(a, row, first + t * kSmpStep, x[t]);
+  const uint64_t mine_best = slice_best(a, row);
+  fill_table(table);
   const RowFilter f = row_filter(a, row);
-  const uint64_t best = row_best(a, row);
-  const uint32_t top_key = (uint32_t)(best >> 32);
+  const uint32_t top_key = (uint32_t)(wave_max(mine_best) >> 32);
   if (f.greedy || top_key <= kKeyNone) return;
   const float top = key_value(top_key);
   const Binner bn = binner(f);
   const int top_bin = bn.bin(top);
-  fill_table(table);
   if (threadIdx.x == 0) {
     list_n = 0;
     cut_bin = f.by_rank ? kSmpBins - 1 : kSmpBins;
     cut_before = 0.0;
   }
   __syncthreads();
-  const Weigher wt{table, top, 1.4426950408889634074 / f.T};
+  const Weigher wt(table, top, f.T);
+  const float low = lowest_near(top, f.T);
   double goal = (double)f.k;
   if (f.by_rank || f.by_mass) {
-    // this thread's bin of the row, from the slices in order
-    double v = 0.0;
-    for (uint32_t s = 0; s < a.slices; ++s) {
-      const size_t at = (size_t)row * a.slices + s;
-      const uint32_t key = (uint32_t)(a.best[at] >> 32);
-      if (key <= kKeyNone) continue;
+    // this thread's bin of the row, from the slices in order: their shifts and weights first, by one
+    // thread each, so that the loads of the bins do not wait for one another
+    if (threadIdx.x < a.slices) {
+      const uint32_t key = (uint32_t)(mine_best >> 32);
       const float stop = key_value(key);
-      const int64_t mine = (int64_t)threadIdx.x - ((int64_t)top_bin - bn.bin(stop));
-      if (mine < 0) continue;
-      const double h = (double)a.hist[at * kSmpBins + mine];
-      v += f.by_rank ? h : h * wt.weight(stop);
+      const bool used = key > kKeyNone;
+      slice_shift[threadIdx.x] = used ? (int)min((int64_t)top_bin - bn.bin(stop), (int64_t)kSmpBins) : kSmpBins;
+      slice_weight[threadIdx.x] = !used ? 0.0 : f.by_rank ? 1.0 : wt.weight(stop);
+    }
+    __syncthreads();
+    double v = 0.0;
+    const uint64_t* const bins = a.hist + (size_t)row * a.slices * kSmpBins;
+#pragma unroll 8
+    for (uint32_t s = 0; s < a.slices; ++s) {
+      const int mine = (int)threadIdx.x - slice_shift[s];
+      const uint64_t h = bins[s * kSmpBins + max(mine, 0)];
+      v += mine >= 0 ? (double)h * slice_weight[s] : 0.0;
     }
     const int wave = threadIdx.x / kWave;
     const double incl = wave_scan(v);
@@ -322,20 +414,28 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
 #pragma unroll
   for (int t = 0; t < ITERS; ++t) {
     uint64_t mine = 0;
+    int rel[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float y = x[t][j];
-      const int rel = top_bin - bn.bin(y);
-      if ((uint32_t)rel >= kSmpBins || !(y > -__builtin_inff())) continue;
-      if (rel == cut || (f.by_rank && rel < cut)) {
+      rel[j] = y >= low ? top_bin - bn.bin(y) : kSmpBins;
+      if (f.by_rank && rel[j] < cut) rel[j] = cut;
+    }
+    if (!f.by_rank) {
+      double w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = wt.endless ? wt.weight(x[t][j]) : wt.near(x[t][j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        mine += rel[j] < cut && (x[t][j] == top || !(w[j] < f.min_p)) ? Weigher::fixed(w[j]) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (rel[j] == cut && cut < kSmpBins) {
         const uint32_t at = atomicAdd(&list_n, 1u);
         if (at < kSmpMaxCand)
-          list[at] = ((uint64_t)key_of(y) << 32) | (0xFFFFFFFFu - (first + t * kSmpStep + j));
-      } else if (!f.by_rank && rel < cut) {
-        const double w = wt.weight(y);
-        if (y == top || !(w < f.min_p)) mine += Weigher::fixed(w);
+          list[at] = ((uint64_t)key_of(x[t][j]) << 32) | (0xFFFFFFFFu - (first + t * kSmpStep + j));
       }
-    }
     if (!f.by_rank) {
       const uint64_t s = wave_sum(mine);
       const uint32_t g = (first + t * kSmpStep) / kSmpSeg;
@@ -355,10 +455,12 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
 struct SampleShared {
   uint64_t seg[kSmpMaxVocab / kWave];   // generic: measure of every 64 tokens; else of every kSmpSeg
   uint64_t hist[2048];
-  uint64_t wsum[kSmpWaves];
+  uint32_t count[2048];
+  uint64_t left[kWave][2];
+  uint64_t wsum[kSmpWaves], wmin[kSmpWaves];
   double table[64];
-  uint32_t word[8];
-  uint64_t wide[4];
+  uint32_t word[2], members;
+  uint64_t wide[2];
 };
 // Sum of measure(i) over the row, by 64 tokens in sh.seg.
 template <class F>
@@ -529,46 +631,52 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared& sh, uint64_t v, uin
   return off + incl - v;
 }
 
-// Among the threads' values (those with a measure), the value at which the running measure, from the
-// largest value down, first reaches `target` (>= 1, <= the total), and the measure above it.
-__device__ __forceinline__ uint32_t value_reaching(SampleShared& sh, const uint32_t* val, const uint64_t* meas,
-                                                   uint64_t target, uint64_t& above) {
-  uint32_t lo = 0, hi = 0xFFFFFFFFu;
-  above = 0;
+// Among the threads' entries (those with a measure; no two alike), the entry at which the running measure,
+// from the largest entry down, first reaches `target` (>= 1, <= the total). A digit at a time of the
+// range that is in use, until at most a wavefront's worth is left, which is ranked directly.
+__device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint64_t* entry, const uint64_t* meas,
+                                                   uint64_t target) {
+  uint64_t lo = 0, hi = ~0ull, above = 0;
   for (;;) {
-    // the range that is in use: 16-bit logits and few candidates are through after a digit or two
-    uint32_t mn = 0xFFFFFFFFu, mx = 0;
+    uint64_t mx = 0, nmn = 0;
 #pragma unroll
     for (int j = 0; j < kSmpPerThread; ++j)
-      if (meas[j] && val[j] >= lo && val[j] <= hi) {
-        mn = min(mn, val[j]);
-        mx = max(mx, val[j]);
+      if (meas[j] && entry[j] >= lo && entry[j] <= hi) {
+        mx = max(mx, entry[j]);
+        nmn = max(nmn, ~entry[j]);
       }
-    uint32_t nmn = 0xFFFFFFFFu - mn;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      mx = max(mx, (uint32_t)__shfl_xor(mx, d));
-      nmn = max(nmn, (uint32_t)__shfl_xor(nmn, d));
+    mx = wave_max(mx);
+    nmn = wave_max(nmn);
+    if (lane_id() == 0) {
+      sh.wsum[threadIdx.x / kWave] = mx;
+      sh.wmin[threadIdx.x / kWave] = nmn;
     }
-    if (lane_id() == 0) sh.wsum[threadIdx.x / kWave] = ((uint64_t)mx << 32) | nmn;
-    for (int i = threadIdx.x; i < 2048; i += kSmpThreads) sh.hist[i] = 0;
+    for (int i = threadIdx.x; i < 2048; i += kSmpThreads) {
+      sh.hist[i] = 0;
+      sh.count[i] = 0;
+    }
+    if (threadIdx.x == 0) sh.members = 0;
     __syncthreads();
-    uint32_t top = 0, low = 0;
+    hi = 0;
+    lo = 0;
 #pragma unroll
     for (int w = 0; w < kSmpWaves; ++w) {
-      top = max(top, (uint32_t)(sh.wsum[w] >> 32));
-      low = max(low, (uint32_t)sh.wsum[w]);
+      hi = max(hi, sh.wsum[w]);
+      lo = max(lo, sh.wmin[w]);
     }
-    hi = top;
-    lo = 0xFFFFFFFFu - low;
-    __syncthreads();
-    if (lo >= hi) return hi;
-    const int bits = 32 - __builtin_clz(hi - lo);
-    const int shift = max(0, bits - 11);
+    lo = ~lo;
+    if (lo >= hi) {
+      __syncthreads();
+      return hi;
+    }
+    const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
 #pragma unroll
     for (int j = 0; j < kSmpPerThread; ++j)
-      if (meas[j] && val[j] >= lo && val[j] <= hi)
-        atomicAdd((unsigned long long*)&sh.hist[(hi - val[j]) >> shift], (unsigned long long)meas[j]);
+      if (meas[j] && entry[j] >= lo && entry[j] <= hi) {
+        const uint32_t digit = (uint32_t)((hi - entry[j]) >> shift);
+        atomicAdd((unsigned long long*)&sh.hist[digit], (unsigned long long)meas[j]);
+        atomicAdd(&sh.count[digit], 1u);
+      }
     __syncthreads();
     uint64_t m[4], s = 0, total;
 #pragma unroll
@@ -578,124 +686,122 @@ __device__ __forceinline__ uint32_t value_reaching(SampleShared& sh, const uint3
     for (int j = 0; j < 4; ++j) {
       if (run < target && run + m[j] >= target) {
         sh.word[0] = 4 * threadIdx.x + j;
+        sh.word[1] = sh.count[4 * threadIdx.x + j];
         sh.wide[0] = run;
       }
       run += m[j];
     }
     __syncthreads();
-    const uint32_t digit = sh.word[0];
+    const uint64_t digit = sh.word[0];
+    const uint32_t n = sh.word[1];
     above = sh.wide[0];
-    __syncthreads();
     hi -= digit << shift;
-    const uint32_t width = (1u << shift) - 1;
-    lo = max(lo, hi > width ? hi - width : 0u);
+    const uint64_t width = (1ull << shift) - 1;
+    const uint64_t least = hi > width ? hi - width : 0;   // one type on both sides of max, or it is the double's
+    lo = max(lo, least);
+    if (n <= kWave) {
+#pragma unroll
+      for (int j = 0; j < kSmpPerThread; ++j)
+        if (meas[j] && entry[j] >= lo && entry[j] <= hi) {
+          const uint32_t at = atomicAdd(&sh.members, 1u);
+          sh.left[at][0] = entry[j];
+          sh.left[at][1] = meas[j];
+        }
+      __syncthreads();
+      if (threadIdx.x < n) {
+        const uint64_t mine = sh.left[threadIdx.x][0];
+        uint64_t before = above;
+        for (uint32_t i = 0; i < n; ++i) before += sh.left[i][0] > mine ? sh.left[i][1] : 0;
+        if (before < target && before + sh.left[threadIdx.x][1] >= target) sh.wide[1] = mine;
+      }
+      __syncthreads();
+      const uint64_t got = sh.wide[1];
+      __syncthreads();
+      return got;
+    }
+    __syncthreads();
   }
 }
 
 template <int DT>
 __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) {
   __shared__ SampleShared sh;
-  const uint32_t row = blockIdx.x, V = a.vocab;
+  const uint32_t row = blockIdx.x, V = a.vocab, segs = (V + kSmpSeg - 1) / kSmpSeg;
+  // everything that does not depend on anything first: one round trip
+  uint64_t best = slice_best(a, row);
+  const uint32_t n = a.cand_count[row];
+  const SampleCut c = a.cut[row];
+  uint64_t seg = threadIdx.x < segs ? a.seg[(size_t)row * segs + threadIdx.x] : 0;
+  uint64_t entry[kSmpPerThread];          // key, then the complement of the index: larger is better ranked
+  entry[0] = threadIdx.x < a.cand_stride ? a.cand[(size_t)row * a.cand_stride + threadIdx.x] : 0;
+  const float u = a.u[row];
   const RowFilter f = row_filter(a, row);
-  const uint64_t best = row_best(a, row);
+  fill_table(sh.table);
+  best = wave_max(best);
   const uint32_t top_key = (uint32_t)(best >> 32);
   if (f.greedy || top_key <= kKeyNone) {
     if (threadIdx.x == 0) a.tokens[row] = top_key <= kKeyNone ? -1 : (int64_t)(0xFFFFFFFFu - (uint32_t)best);
     return;
   }
   const float top = key_value(top_key);
-  const Weigher wt{sh.table, top, 1.4426950408889634074 / f.T};
-  fill_table(sh.table);
-  const float u = a.u[row];
+  const Weigher wt(sh.table, top, f.T);
   auto aim = [&](uint64_t total) {
     const double at = (u > 0.0f ? fmin((double)u, 1.0) : 0.0) * (double)total;
     return min((uint64_t)at, total - 1);
   };
-  const uint32_t n = a.cand_count[row];
   __syncthreads();
   if (n > kSmpMaxCand) {
     const uint32_t token = pick_from_row<DT>(sh, a, row, f, wt, top_key, aim);
     if (threadIdx.x == 0) a.tokens[row] = token;
     return;
   }
-  const SampleCut c = a.cut[row];
-  uint32_t key[kSmpPerThread], inv[kSmpPerThread];      // complement of the index: larger is earlier
   uint64_t mass[kSmpPerThread];
 #pragma unroll
   for (int j = 0; j < kSmpPerThread; ++j) {
     const uint32_t i = j * kSmpThreads + threadIdx.x;
-    key[j] = 0;
-    inv[j] = 0;
-    mass[j] = 0;
-    if (i < n) {
-      const uint64_t e = a.cand[(size_t)row * a.cand_stride + i];
-      key[j] = (uint32_t)(e >> 32);
-      inv[j] = (uint32_t)e;
-      mass[j] = wt.mass(key_value(key[j]));
-    }
+    if (i >= n) entry[j] = 0;
+    else if (j > 0) entry[j] = a.cand[(size_t)row * a.cand_stride + i];
   }
-  // kept candidates: key above key_cut, or equal to it with a complement of at least inv_cut
-  uint32_t key_cut = 0, inv_cut = 0;
-  uint64_t one[kSmpPerThread], above;
+#pragma unroll
+  for (int j = 0; j < kSmpPerThread; ++j) mass[j] = entry[j] ? wt.mass(key_value((uint32_t)(entry[j] >> 32))) : 0;
+  // candidates from `cut` up are kept
+  uint64_t cut = 0;
   if (f.by_rank && (uint32_t)f.k < n) {
+    uint64_t one[kSmpPerThread];
 #pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j) one[j] = key[j] ? 1 : 0;
-    key_cut = value_reaching(sh, key, one, (uint64_t)f.k, above);
-    const uint64_t ties = (uint64_t)f.k - above;
+    for (int j = 0; j < kSmpPerThread; ++j) one[j] = entry[j] ? 1 : 0;
+    cut = entry_reaching(sh, entry, one, (uint64_t)f.k);
 #pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j) one[j] = key[j] == key_cut && key[j] ? 1 : 0;
-    inv_cut = value_reaching(sh, inv, one, ties, above);
-#pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j)
-      if (key[j] < key_cut || (key[j] == key_cut && inv[j] < inv_cut)) key[j] = 0;
+    for (int j = 0; j < kSmpPerThread; ++j) mass[j] = entry[j] < cut ? 0 : mass[j];
   }
   if (f.p < 1.0 && n > 0) {
     uint64_t mine = 0, total;
 #pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j) {
-      if (!key[j]) mass[j] = 0;
-      mine += mass[j];
-    }
+    for (int j = 0; j < kSmpPerThread; ++j) mine += mass[j];
     block_scan(sh, mine, total);
     const double goal = f.by_rank ? f.p * (double)total : c.goal - c.before;
     const uint64_t target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
-    if (target <= total) {
-      const uint32_t rank_cut = key_cut;
-      key_cut = value_reaching(sh, key, mass, target, above);
-      const uint64_t each = wt.mass(key_value(key_cut));
-      const uint64_t ties = (target - above + each - 1) / each;
-      uint64_t have = 0, all;
-#pragma unroll
-      for (int j = 0; j < kSmpPerThread; ++j) {
-        one[j] = key[j] == key_cut && key[j] ? 1 : 0;
-        have += one[j];
-      }
-      block_scan(sh, have, all);
-      if (ties < all) inv_cut = value_reaching(sh, inv, one, ties, above);
-      else if (key_cut != rank_cut) inv_cut = 0;        // else what top-k left of these
-#pragma unroll
-      for (int j = 0; j < kSmpPerThread; ++j)
-        if (key[j] < key_cut || (key[j] == key_cut && inv[j] < inv_cut)) key[j] = 0;
-    }
+    if (target <= total) cut = max(cut, entry_reaching(sh, entry, mass, target));
   }
   // ---- sums over kSmpSeg tokens, and the draw -------------------------------------------------
-  const uint32_t segs = (V + kSmpSeg - 1) / kSmpSeg;
-  if (threadIdx.x < segs) sh.seg[threadIdx.x] = f.by_rank ? 0 : a.seg[(size_t)row * segs + threadIdx.x];
+  if (threadIdx.x < segs) sh.seg[threadIdx.x] = f.by_rank ? 0 : seg;
   __syncthreads();
   auto passes = [&](uint32_t k, double w) { return k == top_key || !(w < f.min_p); };
 #pragma unroll
   for (int j = 0; j < kSmpPerThread; ++j)
-    if (key[j]) {
-      const double w = wt.weight(key_value(key[j]));
-      if (passes(key[j], w))
-        atomicAdd((unsigned long long*)&sh.seg[(0xFFFFFFFFu - inv[j]) / kSmpSeg], (unsigned long long)Weigher::fixed(w));
+    if (entry[j] && entry[j] >= cut) {
+      const uint32_t k = (uint32_t)(entry[j] >> 32);
+      const double w = wt.weight(key_value(k));
+      if (passes(k, w))
+        atomicAdd((unsigned long long*)&sh.seg[(0xFFFFFFFFu - (uint32_t)entry[j]) / kSmpSeg],
+                  (unsigned long long)Weigher::fixed(w));
     }
   __syncthreads();
-  const uint64_t mine = threadIdx.x < segs ? sh.seg[threadIdx.x] : 0;
+  seg = threadIdx.x < segs ? sh.seg[threadIdx.x] : 0;
   uint64_t total;
-  const uint64_t off = block_scan(sh, mine, total);
+  const uint64_t off = block_scan(sh, seg, total);
   const uint64_t target = aim(total);
-  if (off <= target && off + mine > target) {
+  if (off <= target && off + seg > target) {
     sh.word[0] = threadIdx.x;
     sh.wide[0] = off;
   }
@@ -710,10 +816,11 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int rel = top_bin - bn.bin(x[j]);
-    const uint32_t k = key_of(x[j]), comp = 0xFFFFFFFFu - (i0 + j);
+    const uint32_t k = key_of(x[j]);
+    const uint64_t e = ((uint64_t)k << 32) | (0xFFFFFFFFu - (i0 + j));
     bool in = k > kKeyNone && rel < kSmpBins;
     // tokens of the candidates' bins are kept by the exact cut, those above by their bin
-    if (rel == c.bin || (f.by_rank && rel < c.bin)) in = in && (k > key_cut || (k == key_cut && comp >= inv_cut));
+    if (rel == c.bin || (f.by_rank && rel < c.bin)) in = in && e >= cut;
     else in = in && rel < c.bin;
     const double w = wt.weight(x[j]);
     m[j] = in && passes(k, w) ? Weigher::fixed(w) : 0;
