@@ -64,11 +64,11 @@ struct SampleArgs {
   uint32_t* cand_count;       // [rows]
 };
 
-// What keep leaves for pick: the bin of the cut (bins run down from the best token's, 0), and for
-// top-p the mass above it and the mass to reach.
+// What keep leaves for pick. Tokens from `keep` up are kept, those from `cand` up to there are
+// candidates (a NaN: there are none); for top-p, the mass above the cut's bin and the mass to reach.
 struct SampleCut {
   double before, goal;
-  int32_t bin, pad;
+  float keep, cand;
 };
 
 // NaN counts as masked; -0 ranks as +0
@@ -176,36 +176,48 @@ __device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, uint32_t ro
   return f;
 }
 
-// w and its fixed-point form, for logits relative to `top`. With z = 64 (x - top) log2(e) / T:
+// a * b + c with c a constant of the scalar registers (the compiler takes the two-address form and
+// refills its accumulator with the constant each time)
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
+
+// w in units of 2^-45 and its fixed-point form, for logits relative to `top`. With
+// z = 64 (x - top) log2(e) / T:
 //   2^(z / 64) = 2^(n >> 6) * 2^((n & 63) / 64) * 2^(f / 64),   n = rint(z),  |f| <= 1/2
 // with the middle factor from a table and the last from its series to the fifth power in f
 // (next term (ln 2 / 128)^6 / 720 < 4e-17).
 struct Weigher {
-  const double* table;        // LDS, 2^(i / 64)
+  const double* table;        // LDS, 2^(45 + i / 64)
   double top, per;            // per = 64 log2(e) / T
   bool endless;               // the largest logit is infinite: it weighs 1, the others nothing
   __device__ __forceinline__ Weigher(const double* t, float best, double T)
       : table(t), top(best), per(92.3324826168936580 / T), endless(best == __builtin_inff()) {}
-  // x finite or -inf, not more than a few hundred T below top unless the result is not used
-  __device__ __forceinline__ double near(float x) const {
-    const double z = ((double)x - top) * per;
-    const double n = rint(z), f = z - n;
+  // any x where `endless` is not set. Rounding by adding 1.5 * 2^52 and scaling in the exponent field:
+  // the instructions made for either run at a quarter of an addition's rate
+  __device__ __forceinline__ double scaled(float x) const {
+    const double z = fmax(((double)x - top) * per, -4096.0);   // 2^-19 units for all that is further down
+    const double t = z + 6755399441055744.0;
+    const uint32_t i = (uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double f = z - (t - 6755399441055744.0);
     constexpr double c = 0.693147180559945309417 / 64;
-    const int i = (int)n;
-    double y = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
-    y = fma(f, y, c * c * c / 6);
-    y = fma(f, y, c * c / 2);
-    y = fma(f, y, c);
-    y = fma(f, y, 1.0);
-    return __builtin_amdgcn_ldexp(y * table[i & 63], i >> 6);
+    double y = fma_const(f, c * c * c * c * c / 120, c * c * c * c / 24);
+    y = fma_const(f, y, c * c * c / 6);
+    y = fma_const(f, y, c * c / 2);
+    y = fma_const(f, y, c);
+    y = fma(f, y, 1.0) * table[i & 63];
+    const uint64_t b = __builtin_bit_cast(uint64_t, y);
+    return __builtin_bit_cast(double, ((uint64_t)((uint32_t)(b >> 32) + ((i & ~63u) << 14)) << 32) | (uint32_t)b);
   }
-  __device__ __forceinline__ double weight(float x) const {
-    if (endless) return x == __builtin_inff() ? 1.0 : 0.0;
-    return ((double)x - top) * per < -6400.0 ? 0.0 : near(x);
+  __device__ __forceinline__ double weight(float x) const {     // in units of 2^-45
+    if (endless) return x == __builtin_inff() ? kSmpOne : 0.0;
+    return scaled(x);
   }
   static __device__ __forceinline__ uint64_t fixed(double w) {
-    // adding 2^52 leaves the integer nearest w 2^45 in the low bits
-    return __builtin_bit_cast(uint64_t, fma(w, kSmpOne, 4503599627370496.0)) - 0x4330000000000000ull;
+    // adding 2^52 leaves the nearest integer in the low bits
+    return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) - 0x4330000000000000ull;
   }
   __device__ __forceinline__ uint64_t mass(float x) const { return fixed(weight(x)); }
 };
@@ -228,24 +240,42 @@ __device__ const double kPow2[64] = {   // 2^(i / 64), rounded to nearest
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
 };
 __device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = kPow2[threadIdx.x];
+  if (threadIdx.x < 64) table[threadIdx.x] = kPow2[threadIdx.x] * kSmpOne;
 }
 
 // Bins of width T / 16 from the best token's down: monotone in x, the same intervals for every slice.
 struct Binner {
   float per;
   __device__ __forceinline__ int bin(float x) const {
-    return (int)fminf(fmaxf(floorf(x * per), -1073741824.0f), 1073741824.0f);
+    int b;                                        // floor and conversion in one; saturates
+    asm("v_cvt_flr_i32_f32 %0, %1" : "=v"(b) : "v"(x * per));
+    return b;
   }
+  // The least logit of bin b or above (NaN: no logit is), so that a pass over the tokens compares instead
+  // of binning: by halving, on the ordered bit patterns, an interval around the quotient or else all
+  __device__ __forceinline__ float edge(int64_t b) const {
+    if (b > 0x7FFFFFFFll) return __builtin_nanf("");
+    uint32_t lo = key_of(-__FLT_MAX__), hi = key_of(__FLT_MAX__);
+    if (b <= -0x80000000ll || bin(key_value(lo)) >= (int)b) return -__FLT_MAX__;
+    if (bin(key_value(hi)) < (int)b) return __builtin_inff();
+    const uint32_t near = key_of(fminf(fmaxf((float)b / per, -1e38f), 1e38f));
+    if (bin(key_value(near - 32)) < (int)b && bin(key_value(near + 32)) >= (int)b) {
+      lo = near - 32;
+      hi = near + 32;
+    }
+    while (hi - lo > 1) {                 // bin(lo) < b <= bin(hi)
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (bin(key_value(mid)) >= (int)b) hi = mid;
+      else lo = mid;
+    }
+    return key_value(hi);
+  }
+  // bins from the best token's down: a huge number, as unsigned, where the difference leaves 32 bits
+  __device__ __forceinline__ uint32_t below(int top_bin, float x) const { return (uint32_t)top_bin - (uint32_t)bin(x); }
 };
 __device__ __forceinline__ Binner binner(const RowFilter& f) {
   // bounded away from 0 and infinity, either of which could make a NaN of a logit
   return Binner{fminf(fmaxf((float)(16.0 / f.T), 1e-37f), 1e30f)};
-}
-
-// Logits from here up weigh something; what is below weighs less than 2^-46 and may be left out.
-__device__ __forceinline__ float lowest_near(float top, double T) {
-  return fmaxf((float)((double)top - 40.0 * T), -__FLT_MAX__);
 }
 
 // ---- first launch ------------------------------------------------------------------------------
@@ -301,30 +331,24 @@ __global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) 
   const Weigher wt(table, top, f.T);
   const Binner bn = binner(f);
   const int top_bin = bn.bin(top);
-  const float low = lowest_near(top, f.T);
   if (f.by_rank || wt.endless) {
 #pragma unroll
     for (int t = 0; t < ITERS; ++t)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t rel = (uint32_t)(top_bin - bn.bin(x[t][j]));
+        const uint32_t rel = bn.below(top_bin, x[t][j]);
         if (rel < kSmpBins && x[t][j] > -__builtin_inff())
           atomicAdd((unsigned long long*)&hist[rel], f.by_rank ? 1ull : (unsigned long long)wt.mass(x[t][j]));
       }
   } else {
 #pragma unroll
-    for (int t = 0; t < ITERS; ++t) {
-      // eight at a time without a branch between them; saturated bins may hold anything, -inf among
-      // it, and `near` is for what is near
-      uint64_t v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = Weigher::fixed(wt.near(x[t][j]));
+    for (int t = 0; t < ITERS; ++t)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t rel = (uint32_t)(top_bin - bn.bin(x[t][j]));
-        if (rel < kSmpBins && x[t][j] >= low) atomicAdd((unsigned long long*)&hist[rel], (unsigned long long)v[j]);
+        const uint32_t rel = bn.below(top_bin, x[t][j]);
+        const uint64_t v = Weigher::fixed(wt.scaled(x[t][j]));
+        if (rel < kSmpBins) atomicAdd((unsigned long long*)&hist[rel], (unsigned long long)v);
       }
-    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < kSmpBins; i += kSmpThreads) a.hist[out * kSmpBins + i] = hist[i];
@@ -346,6 +370,7 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
   __shared__ double slice_weight[64];
   __shared__ double cut_before;
   __shared__ int cut_bin;
+  __shared__ float cut_keep, cut_cand;
   __shared__ uint32_t list_n, list_at;
   const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const uint32_t first = slice * (ITERS * kSmpStep) + threadIdx.x * 8;
@@ -364,10 +389,11 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
     list_n = 0;
     cut_bin = f.by_rank ? kSmpBins - 1 : kSmpBins;
     cut_before = 0.0;
+    cut_keep = -__FLT_MAX__;              // without a cut: everything but -inf, and no candidates
+    cut_cand = __builtin_nanf("");
   }
   __syncthreads();
   const Weigher wt(table, top, f.T);
-  const float low = lowest_near(top, f.T);
   double goal = (double)f.k;
   if (f.by_rank || f.by_mass) {
     // this thread's bin of the row, from the slices in order: their shifts and weights first, by one
@@ -376,8 +402,8 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
       const uint32_t key = (uint32_t)(mine_best >> 32);
       const float stop = key_value(key);
       const bool used = key > kKeyNone;
-      slice_shift[threadIdx.x] = used ? (int)min((int64_t)top_bin - bn.bin(stop), (int64_t)kSmpBins) : kSmpBins;
-      slice_weight[threadIdx.x] = !used ? 0.0 : f.by_rank ? 1.0 : wt.weight(stop);
+      slice_shift[threadIdx.x] = used ? (int)min(bn.below(top_bin, stop), (uint32_t)kSmpBins) : kSmpBins;
+      slice_weight[threadIdx.x] = !used ? 0.0 : f.by_rank ? 1.0 : wt.weight(stop) / kSmpOne;
     }
     __syncthreads();
     double v = 0.0;
@@ -406,46 +432,66 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
     if (hit && lane_id() == __builtin_ctzll(hit)) atomicMin(&cut_bin, (int)threadIdx.x);
     __syncthreads();
     if ((int)threadIdx.x == cut_bin) cut_before = before;
+    if (threadIdx.x < 2 && cut_bin < kSmpBins) {
+      const float e = bn.edge((int64_t)top_bin - cut_bin + threadIdx.x);
+      if (threadIdx.x == 0) cut_cand = e;
+      else cut_keep = f.by_rank ? __builtin_nanf("") : e;
+    }
     __syncthreads();
   }
-  const int cut = cut_bin;
-  if (slice == 0 && threadIdx.x == 0) a.cut[row] = SampleCut{cut_before, goal, cut, 0};
-  const uint32_t segs = (a.vocab + kSmpSeg - 1) / kSmpSeg;
+  const float keep = cut_keep, cand = cut_cand;
+  if (slice == 0 && threadIdx.x == 0) a.cut[row] = SampleCut{cut_before, goal, keep, cand};
+  // candidates first: their place in the row's list is a round trip that the weights can hide
+  uint32_t hits[ITERS];                   // bit j: token j of the eight is a candidate
 #pragma unroll
   for (int t = 0; t < ITERS; ++t) {
-    uint64_t mine = 0;
-    int rel[8];
+    hits[t] = 0;
+    if (cand == cand) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float y = x[t][j];
-      rel[j] = y >= low ? top_bin - bn.bin(y) : kSmpBins;
-      if (f.by_rank && rel[j] < cut) rel[j] = cut;
-    }
-    if (!f.by_rank) {
-      double w[8];
+      for (int j = 0; j < 8; ++j) hits[t] |= x[t][j] >= cand && !(x[t][j] >= keep) ? 1u << j : 0u;
+      if (__any(hits[t] != 0)) {
+        const int n = __builtin_popcount(hits[t]), incl = wave_inclusive_scan(n);
+        int base = 0;
+        if (lane_id() == kWave - 1) base = (int)atomicAdd(&list_n, (uint32_t)incl);
+        uint32_t at = (uint32_t)(__builtin_amdgcn_readlane(base, kWave - 1) + incl - n);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = wt.endless ? wt.weight(x[t][j]) : wt.near(x[t][j]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        mine += rel[j] < cut && (x[t][j] == top || !(w[j] < f.min_p)) ? Weigher::fixed(w[j]) : 0;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (rel[j] == cut && cut < kSmpBins) {
-        const uint32_t at = atomicAdd(&list_n, 1u);
-        if (at < kSmpMaxCand)
-          list[at] = ((uint64_t)key_of(x[t][j]) << 32) | (0xFFFFFFFFu - (first + t * kSmpStep + j));
+        for (int j = 0; j < 8; ++j)
+          if (hits[t] & (1u << j)) {
+            if (at < kSmpMaxCand)
+              list[at] = ((uint64_t)key_of(x[t][j]) << 32) | (0xFFFFFFFFu - (first + t * kSmpStep + j));
+            ++at;
+          }
       }
-    if (!f.by_rank) {
-      const uint64_t s = wave_sum(mine);
-      const uint32_t g = (first + t * kSmpStep) / kSmpSeg;
-      if (lane_id() == 0 && g < segs) a.seg[(size_t)row * segs + g] = s;
     }
   }
   __syncthreads();
   const uint32_t n = list_n;
+  uint32_t row_at = 0;
+  if (threadIdx.x == 0 && n > 0) row_at = atomicAdd(&a.cand_count[row], n);
+  if (!f.by_rank) {
+    const double min_w = f.min_p > 0.0 ? f.min_p * kSmpOne : -1.0;
+    const uint32_t segs = (a.vocab + kSmpSeg - 1) / kSmpSeg;
+    auto sums = [&](auto weigh) {
+#pragma unroll
+      for (int t = 0; t < ITERS; ++t) {
+        uint64_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = x[t][j];
+          const double w = weigh(y);
+          const bool in = y >= keep && (w >= min_w || y == top);
+          mine += in ? Weigher::fixed(w) : 0;
+        }
+        const uint64_t s = wave_sum(mine);
+        const uint32_t g = (first + t * kSmpStep) / kSmpSeg;
+        if (lane_id() == 0 && g < segs) a.seg[(size_t)row * segs + g] = s;
+      }
+    };
+    if (wt.endless) sums([&](float y) { return wt.weight(y); });
+    else sums([&](float y) { return wt.scaled(y); });
+  }
   if (n == 0) return;
-  if (threadIdx.x == 0) list_at = atomicAdd(&a.cand_count[row], n);
+  if (threadIdx.x == 0) list_at = row_at;
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < min(n, kSmpMaxCand); i += kSmpThreads)
     if (list_at + i < a.cand_stride) a.cand[(size_t)row * a.cand_stride + list_at + i] = list[i];
@@ -607,7 +653,7 @@ __device__ uint32_t pick_from_row(SampleShared& sh, const SampleArgs& a, uint32_
     const uint32_t key = key_of(x);
     if (key < cut || (key == cut && i > last_tie)) return 0ull;
     const double w = wt.weight(x);
-    if (key != top_key && w < f.min_p) return 0ull;
+    if (key != top_key && w < f.min_p * kSmpOne) return 0ull;
     return (unsigned long long)Weigher::fixed(w);
   };
   const uint64_t total = measure_row(sh, V, kept);
@@ -635,13 +681,13 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared& sh, uint64_t v, uin
 // from the largest entry down, first reaches `target` (>= 1, <= the total). A digit at a time of the
 // range that is in use, until at most a wavefront's worth is left, which is ranked directly.
 __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint64_t* entry, const uint64_t* meas,
-                                                   uint64_t target) {
+                                                   uint32_t entries, uint64_t target) {
   uint64_t lo = 0, hi = ~0ull, above = 0;
-  for (;;) {
+  for (int digits = 0; digits < 7; ++digits) {   // a digit is 11 of 64 bits
     uint64_t mx = 0, nmn = 0;
 #pragma unroll
     for (int j = 0; j < kSmpPerThread; ++j)
-      if (meas[j] && entry[j] >= lo && entry[j] <= hi) {
+      if (j * kSmpThreads < entries && meas[j] && entry[j] >= lo && entry[j] <= hi) {
         mx = max(mx, entry[j]);
         nmn = max(nmn, ~entry[j]);
       }
@@ -672,7 +718,7 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint6
     const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
 #pragma unroll
     for (int j = 0; j < kSmpPerThread; ++j)
-      if (meas[j] && entry[j] >= lo && entry[j] <= hi) {
+      if (j * kSmpThreads < entries && meas[j] && entry[j] >= lo && entry[j] <= hi) {
         const uint32_t digit = (uint32_t)((hi - entry[j]) >> shift);
         atomicAdd((unsigned long long*)&sh.hist[digit], (unsigned long long)meas[j]);
         atomicAdd(&sh.count[digit], 1u);
@@ -702,7 +748,7 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint6
     if (n <= kWave) {
 #pragma unroll
       for (int j = 0; j < kSmpPerThread; ++j)
-        if (meas[j] && entry[j] >= lo && entry[j] <= hi) {
+        if (j * kSmpThreads < entries && meas[j] && entry[j] >= lo && entry[j] <= hi) {
           const uint32_t at = atomicAdd(&sh.members, 1u);
           sh.left[at][0] = entry[j];
           sh.left[at][1] = meas[j];
@@ -721,6 +767,7 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint6
     }
     __syncthreads();
   }
+  return hi;
 }
 
 template <int DT>
@@ -763,14 +810,15 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
     else if (j > 0) entry[j] = a.cand[(size_t)row * a.cand_stride + i];
   }
 #pragma unroll
-  for (int j = 0; j < kSmpPerThread; ++j) mass[j] = entry[j] ? wt.mass(key_value((uint32_t)(entry[j] >> 32))) : 0;
+  for (int j = 0; j < kSmpPerThread; ++j)
+    mass[j] = j * kSmpThreads < n && entry[j] ? wt.mass(key_value((uint32_t)(entry[j] >> 32))) : 0;
   // candidates from `cut` up are kept
   uint64_t cut = 0;
   if (f.by_rank && (uint32_t)f.k < n) {
     uint64_t one[kSmpPerThread];
 #pragma unroll
     for (int j = 0; j < kSmpPerThread; ++j) one[j] = entry[j] ? 1 : 0;
-    cut = entry_reaching(sh, entry, one, (uint64_t)f.k);
+    cut = entry_reaching(sh, entry, one, n, (uint64_t)f.k);
 #pragma unroll
     for (int j = 0; j < kSmpPerThread; ++j) mass[j] = entry[j] < cut ? 0 : mass[j];
   }
@@ -781,15 +829,16 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
     block_scan(sh, mine, total);
     const double goal = f.by_rank ? f.p * (double)total : c.goal - c.before;
     const uint64_t target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
-    if (target <= total) cut = max(cut, entry_reaching(sh, entry, mass, target));
+    if (target <= total) cut = max(cut, entry_reaching(sh, entry, mass, n, target));
   }
   // ---- sums over kSmpSeg tokens, and the draw -------------------------------------------------
   if (threadIdx.x < segs) sh.seg[threadIdx.x] = f.by_rank ? 0 : seg;
   __syncthreads();
-  auto passes = [&](uint32_t k, double w) { return k == top_key || !(w < f.min_p); };
+  const double min_w = f.min_p > 0.0 ? f.min_p * kSmpOne : -1.0;
+  auto passes = [&](uint32_t k, double w) { return k == top_key || w >= min_w; };
 #pragma unroll
   for (int j = 0; j < kSmpPerThread; ++j)
-    if (entry[j] && entry[j] >= cut) {
+    if (j * kSmpThreads < n && entry[j] && entry[j] >= cut) {
       const uint32_t k = (uint32_t)(entry[j] >> 32);
       const double w = wt.weight(key_value(k));
       if (passes(k, w))
@@ -807,21 +856,15 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
   }
   __syncthreads();
   if (threadIdx.x >= kWave) return;
-  const Binner bn = binner(f);
-  const int top_bin = bn.bin(top);
   const uint32_t i0 = sh.word[0] * kSmpSeg + lane_id() * 8;
   float x[8];
   logits8<DT>(a, row, i0, x);
   uint64_t m[8], sum = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int rel = top_bin - bn.bin(x[j]);
     const uint32_t k = key_of(x[j]);
     const uint64_t e = ((uint64_t)k << 32) | (0xFFFFFFFFu - (i0 + j));
-    bool in = k > kKeyNone && rel < kSmpBins;
-    // tokens of the candidates' bins are kept by the exact cut, those above by their bin
-    if (rel == c.bin || (f.by_rank && rel < c.bin)) in = in && e >= cut;
-    else in = in && rel < c.bin;
+    const bool in = x[j] >= c.keep || (x[j] >= c.cand && e >= cut);
     const double w = wt.weight(x[j]);
     m[j] = in && passes(k, w) ? Weigher::fixed(w) : 0;
     sum += m[j];
