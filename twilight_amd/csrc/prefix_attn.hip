@@ -44,6 +44,7 @@ constexpr int kPaWaves = kPaThreads / kWave;
 constexpr int kPaTile = 32;                 // tokens of one step of a wavefront
 constexpr float kPaNoMax = -3.0e38f;        // running maximum before the first token
 constexpr float kPaSlack = 8.0f;            // how far a logit may exceed it, in base 2
+constexpr uint32_t kPaMaxParts = 256;       // of one kind, per row
 constexpr float kLn2 = 0.693147180559945309f;
 
 struct PrefixAttnArgs {
@@ -152,12 +153,15 @@ __device__ __forceinline__ int group_of(const PrefixAttnArgs& a, uint32_t b) {
 template <int QT, bool PAIRED, bool TO_F16>
 __device__ __forceinline__ void load_query(const PrefixAttnArgs& a, int row, int kb, u32x4* qf, float& scale) {
   const uint16_t* src = a.q + (size_t)max(row, 0) * TWL_HEAD_DIM;
-  scale = a.scale_log2;
+  // positive, so that the largest product is the largest logit; not zero, so that a masked one stays masked
+  scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+  const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int d = PAIRED ? 64 * (j >> 1) + 16 * kb + 8 * (j & 1) : 32 * j + 8 * kb;
     qf[j] = *(const u32x4*)(src + d);
     if (row < 0) qf[j] = u32x4{0, 0, 0, 0};
+    else qf[j] ^= sign;
   }
   if (TO_F16 && QT == TWL_BF16) {
     float f[4][8];
@@ -195,13 +199,20 @@ __device__ __forceinline__ void put_row(const PrefixAttnArgs& a, int row, uint32
   if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : m * kLn2 + logf(l);
 }
 
+// What the wavefronts of a workgroup exchange at the end of a part.
+template <int NQ, int WR>
+struct PartLds {
+  float o[kPaWaves][16 * NQ][TWL_HEAD_DIM + 4];
+  float m[kPaWaves][16 * NQ], l[kPaWaves][16 * NQ], top[WR][16 * NQ], total[WR][16 * NQ];
+};
+
 // One workgroup's part: tokens [begin, end) of a page list (first id at `ids`, `num_ids` of them)
-// for kv head kvh, and 16 * NQ * WR query rows. The four wavefronts are WR sets of rows times
+// for kv head kvh, and 16 * NQ * WR query rows. The four wavefronts are WR (1 or 2) sets of rows times
 // 4 / WR interleaved sets of token tiles. row_of(local row) -> row of q / out, or -1.
 template <int QT, int KV, int NQ, int WR, class RowOf>
 __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32_t* ids, int num_ids,
                                             int begin, int end, uint32_t kvh, RowOf row_of,
-                                            uint32_t part, uint32_t parts) {
+                                            uint32_t part, uint32_t parts, uint8_t* pool) {
   constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
   constexpr int MT = k8 ? TWL_F16 : QT;
   constexpr int WT = kPaWaves / WR;
@@ -234,10 +245,11 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   const uint32_t voff = 4 * kb * a.token_bytes + (k8 ? 8 : 16) * n;
   const int tiles = (end - begin + kPaTile - 1) / kPaTile;
   int window = -1, held = 0;
-  // one tile; only the last one of a part can be cut short by the end of the list
-  auto step = [&](int t, auto last) {
-    constexpr bool cut = decltype(last)::value;
-    const int tok0 = begin + t * kPaTile;
+  struct Raw {                              // a tile as it comes from memory
+    u32x4 k[2][NKL], v[8];                  // V: eight tokens, 16 bytes (16-bit) or 8 (8-bit) each
+    float ks[2][4], vs[2][4];
+  };
+  auto fetch = [&](int t, Raw& raw) {
     // page ids come 64 at a time, one per lane (32 tiles)
     if ((t >> 5) != window) {
       window = t >> 5;
@@ -248,13 +260,10 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
     const uint32_t id1 = (uint32_t)__builtin_amdgcn_readlane(held, 2 * (t & 31) + 1);
     const uint8_t* kp[2] = {kbase + id0 * a.page_bytes, kbase + id1 * a.page_bytes};
     const uint8_t* vp[2] = {vbase + id0 * a.page_bytes, vbase + id1 * a.page_bytes};
-
-    u32x4 kr[2][NKL];
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int j = 0; j < NKL; ++j) kr[p][j] = load_kv<NT, u32x4>(kp[p] + koff + 64 * j);
-    float ks[2][4], vs[2][4];
+      for (int j = 0; j < NKL; ++j) raw.k[p][j] = load_kv<NT, u32x4>(kp[p] + koff + 64 * j);
     if (k8) {
       const float* sk = a.ks + kvh * a.scale_head;
       const float* sv = a.vs + kvh * a.scale_head;
@@ -264,27 +273,39 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         if (a.scale_vec) {
           const f32x4 x = *(const f32x4*)(sk + so), y = *(const f32x4*)(sv + so);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { ks[p][i] = x[i]; vs[p][i] = y[i]; }
+          for (int i = 0; i < 4; ++i) { raw.ks[p][i] = x[i]; raw.vs[p][i] = y[i]; }
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            ks[p][i] = sk[so + i * a.scale_token];
-            vs[p][i] = sv[so + i * a.scale_token];
+            raw.ks[p][i] = sk[so + i * a.scale_token];
+            raw.vs[p][i] = sv[so + i * a.scale_token];
           }
         }
       }
     }
-    u32x4 vr[8];                            // eight tokens, 16 bytes (16-bit) or 8 (8-bit) each
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint8_t* p = vp[i >> 2] + voff + (i & 3) * a.token_bytes;
       if (k8) {
         const u32x2 w = load_kv<NT, u32x2>(p);
-        vr[i].x = w.x;
-        vr[i].y = w.y;
+        raw.v[i].x = w.x;
+        raw.v[i].y = w.y;
       } else {
-        vr[i] = load_kv<NT, u32x4>(p);
+        raw.v[i] = load_kv<NT, u32x4>(p);
       }
+    }
+  };
+  // one tile; only the last one of a part can be cut short by the end of the list
+  auto step = [&](int t, const Raw& raw, auto last) {
+    constexpr bool cut = decltype(last)::value;
+    const int tok0 = begin + t * kPaTile;
+    float ks[2][4], vs[2][4];
+    u32x4 vr[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ks[i >> 2][i & 3] = raw.ks[i >> 2][i & 3];
+      vs[i >> 2][i & 3] = raw.vs[i >> 2][i & 3];
+      vr[i] = raw.v[i];
     }
 
     // ---- logits --------------------------------------------------------------------------------
@@ -299,11 +320,11 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
       for (int j = 0; j < 4; ++j) {
         u32x4 kf;
         if (k8) {
-          const u32x2 lo = widen4<KV>(kr[p][j >> 1][2 * (j & 1)]);
-          const u32x2 hi = widen4<KV>(kr[p][j >> 1][2 * (j & 1) + 1]);
+          const u32x2 lo = widen4<KV>(raw.k[p][j >> 1][2 * (j & 1)]);
+          const u32x2 hi = widen4<KV>(raw.k[p][j >> 1][2 * (j & 1) + 1]);
           kf = u32x4{lo.x, lo.y, hi.x, hi.y};
         } else {
-          kf = kr[p][j];
+          kf = raw.k[p][j];
         }
 #pragma unroll
         for (int x = 0; x < NQ; ++x) s[x][p] = mfma16<MT>(kf, qf[x][j], s[x][p]);
@@ -342,14 +363,15 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
     u32x4 pf[NQ];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      float top = kPaNoMax;
+      float top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float z = s[x][i >> 2][i & 3] * (k8 ? row_scale[x] * ks[i >> 2][i & 3] : row_scale[x]);
+        float z = k8 ? s[x][i >> 2][i & 3] * ks[i >> 2][i & 3] : s[x][i >> 2][i & 3];
         if (cut) z = tok0 + 16 * (i >> 2) + 4 * kb + (i & 3) < end ? z : -__builtin_inff();
         s[x][i >> 2][i & 3] = z;
         top = fmaxf(top, z);
       }
+      top *= row_scale[x];
       if (__any(top > m[x] + kPaSlack)) {
         const float up = fmaxf(m[x], max_over_kb(top));
         const float alpha = __builtin_amdgcn_exp2f(m[x] - up);
@@ -366,7 +388,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(s[x][i >> 2][i & 3] - m[x]);
+        w[i] = __builtin_amdgcn_exp2f(fmaf(s[x][i >> 2][i & 3], row_scale[x], -m[x]));
         l[x] += w[i];
         if (k8) w[i] *= vs[i >> 2][i & 3];
       }
@@ -416,19 +438,26 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
       }
     }
   };
+  // the next tile is on its way while this one is worked on
   const int whole = (end - begin) / kPaTile;
-  for (int t = wt; t < whole; t += WT) step(t, Never{});
-  if (whole < tiles && whole % WT == wt) step(whole, Always{});
+  Raw cur, next;
+  if (wt < tiles) fetch(wt, cur);
+  for (int t = wt; t < tiles; t += WT) {
+    if (t + WT < tiles) fetch(t + WT, next);
+    if (t < whole) step(t, cur, Never{});
+    else step(t, cur, Always{});
+    cur = next;
+  }
 
   // ---- join the wavefronts that share rows, and leave the part --------------------------------
   const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
-  __shared__ float lds_m[kPaWaves][ROWS], lds_l[kPaWaves][ROWS];
+  auto& lds = *(PartLds<NQ, WR>*)pool;
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
     l[x] = sum_over_kb(l[x]);
     if (kb == 0) {
-      lds_m[wave][16 * x + n] = m[x];
-      lds_l[wave][16 * x + n] = l[x];
+      lds.m[wave][16 * x + n] = m[x];
+      lds.l[wave][16 * x + n] = l[x];
     }
   }
   __syncthreads();
@@ -437,61 +466,41 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   for (int x = 0; x < NQ; ++x) {
     top[x] = kPaNoMax;
 #pragma unroll
-    for (int w = 0; w < WT; ++w) top[x] = fmaxf(top[x], lds_m[wr * WT + w][16 * x + n]);
+    for (int w = 0; w < WT; ++w) top[x] = fmaxf(top[x], lds.m[wr * WT + w][16 * x + n]);
     total[x] = 0.0f;
 #pragma unroll
     for (int w = 0; w < WT; ++w)
-      total[x] += lds_l[wr * WT + w][16 * x + n] * __builtin_amdgcn_exp2f(lds_m[wr * WT + w][16 * x + n] - top[x]);
+      total[x] += lds.l[wr * WT + w][16 * x + n] * __builtin_amdgcn_exp2f(lds.m[wr * WT + w][16 * x + n] - top[x]);
     const float f = __builtin_amdgcn_exp2f(m[x] - top[x]) * vfac;
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[x][j] *= f;
   }
-  if (WT == 1) {
-    // a lane holds 32 consecutive channels of its query's row
+  // every wavefront leaves its rows; 32 threads add and write one
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      const int row = row_of((wr * NQ + x) * 16 + n);
-      if (row >= 0) {
+  for (int x = 0; x < NQ; ++x)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 8; j += 4)
-            put_row<QT>(a, row, part, parts, 32 * kb + 8 * i + j,
-                        f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]}, top[x], total[x]);
-      }
-    }
-    return;
-  }
-  __shared__ float lds_o[WT > 1 ? WR : 1][WT > 1 ? ROWS : 1][TWL_HEAD_DIM + 4];
-  for (int w = 0; w < WT; ++w) {
-    if (wt == w) {
-#pragma unroll
-      for (int x = 0; x < NQ; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* p = &lds_o[wr][16 * x + n][32 * kb + 8 * i];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) p[j] = w == 0 ? o[x][j][i] : p[j] + o[x][j][i];
-        }
-    }
-    __syncthreads();
-  }
+      for (int j = 0; j < 8; j += 4)
+        *(f32x4*)&lds.o[wave][16 * x + n][32 * kb + 8 * i + j] =
+            f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]};
   // the maxima and sums of the joined rows
   if (wt == 0 && kb == 0) {
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      lds_m[wr][16 * x + n] = top[x];
-      lds_l[wr][16 * x + n] = total[x];
+      lds.top[wr][16 * x + n] = top[x];
+      lds.total[wr][16 * x + n] = total[x];
     }
   }
   __syncthreads();
-  // 32 threads write a row
   for (int r = threadIdx.x >> 5; r < ROWS * WR; r += kPaThreads / 32) {
     const int row = row_of(r);
     if (row < 0) continue;
-    const int c = 4 * (threadIdx.x & 31);
-    put_row<QT>(a, row, part, parts, c, *(const f32x4*)&lds_o[r / ROWS][r % ROWS][c], lds_m[r / ROWS][r % ROWS],
-                lds_l[r / ROWS][r % ROWS]);
+    const int c = 4 * (threadIdx.x & 31), g = r / ROWS;
+    f32x4 x = *(const f32x4*)&lds.o[g * WT][r % ROWS][c];
+#pragma unroll
+    for (int w = 1; w < WT; ++w) x += *(const f32x4*)&lds.o[g * WT + w][r % ROWS][c];
+    put_row<QT>(a, row, part, parts, c, x, lds.top[g][r % ROWS], lds.total[g][r % ROWS]);
   }
 }
 
@@ -499,23 +508,32 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 // tile of K and V from LDS. Streaming from L2 into every wavefront's registers would need
 // 16 KB of L1 traffic per 32 tokens and 32 rows, twice what the products take.
 //
-// Tiles of 64 tokens, two buffers: while the products of one run, the next is on its way into registers;
-// it is written to the other buffer after them, one barrier per tile. 8-bit pages are widened to fp16
-// on that way, once per workgroup. A row of 256 bytes holds its 16 chunks of 16 bytes at place
-// c ^ (row % 16): the K operand's loads (16 rows, one chunk) and the V operand's (one row, 16 chunks)
-// both touch every bank once.
+// Tiles of 64 tokens, two buffers: while the products of one run, the next one comes into registers; it
+// is written to the other buffer after them, one barrier per tile. 8-bit pages are widened to fp16
+// on that way, once per workgroup. The V operand comes out of LDS transposed (ds_read_b64_tr_b16: of the
+// 4 x 16 elements that 16 lanes name, four consecutive ones each, a lane gets one column), so that
+// product c takes channels 16 c .. 16 c + 15. A row of 256 bytes holds its 16 chunks of 16 bytes at place
+// c ^ f(row % 16), f(r) = 2 (r % 8) + r / 8: the K operand's loads (16 rows, one chunk) then touch every
+// bank once, and so do the transposing ones (four rows, two neighbouring chunks).
 constexpr int kStTile = 64, kStRows = 128;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+__device__ __forceinline__ int swizzle(int row) { return (row & 7) * 2 + ((row >> 3) & 1); }
+
+struct StagedLds {
+  u32x4 k[2][kStTile * 16], v[2][kStTile * 16];
+  float ks[2][kStTile], vs[2][kStTile];
+};
 
 template <int QT, int KV, class RowOf>
 __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int32_t* ids, int num_ids, int begin,
                                               int end, uint32_t kvh, int rows_here, RowOf row_of, uint32_t part,
-                                              uint32_t parts) {
+                                              uint32_t parts, uint8_t* pool) {
   constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
   constexpr int MT = k8 ? TWL_F16 : QT;
   constexpr int NQ = 2;
   constexpr int NL = k8 ? 2 : 4;            // 16-byte loads of K (and of V) per thread and tile
-  __shared__ u32x4 lds_k[2][kStTile * 16], lds_v[2][kStTile * 16];
-  __shared__ float lds_ks[2][k8 ? kStTile : 1], lds_vs[2][k8 ? kStTile : 1];
+  auto& lds = *(StagedLds*)pool;
   const int tx = threadIdx.x, lane = lane_id(), n = lane & 15, kb = lane >> 4, wave = tx / kWave;
   const bool busy = wave * 16 * NQ < rows_here;   // a wavefront without rows only stages
 
@@ -543,36 +561,35 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
   const int tok = k8 ? (tx >> 3) & 15 : tx >> 4, chunk = k8 ? tx & 7 : tx & 15;
   const uint32_t off = tok * a.token_bytes + 16 * chunk;
   int window = -1, held = 0;
-  u32x4 raw[NL];
-  float sc = 0.0f;
+  u32x4 kraw[NL], vraw[NL];
+  float sc = 0.0f;                          // wavefront 0: a scale of K, wavefront 1: of V
 
-  // One of K and V of tile t, into registers; and from there into LDS.
-  auto fetch = [&](int t, bool is_v) {
+  // Tile t into registers, and from there into LDS.
+  auto fetch = [&](int t) {
     if ((t >> 4) != window) {               // 64 page ids, 16 tiles
       window = t >> 4;
       const int at = min(begin / TWL_PAGE + window * kWave + lane, num_ids - 1);
       held = (int)min((uint32_t)ids[at], a.num_pages - 1);
     }
-    const uint8_t* const base = is_v ? vbase : kbase;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int pg = k8 ? 2 * i + __builtin_amdgcn_readfirstlane(tx >> 7) : i;
       const uint64_t id = (uint32_t)__builtin_amdgcn_readlane(held, 4 * (t & 15) + pg);
-      raw[i] = *(const u32x4*)(base + id * a.page_bytes + off);
+      kraw[i] = *(const u32x4*)(kbase + id * a.page_bytes + off);
+      vraw[i] = *(const u32x4*)(vbase + id * a.page_bytes + off);
     }
-    if (k8 && wave == 0) {                  // one scale per lane
+    if (k8 && wave < 2) {                   // one scale per lane
       const uint64_t id = (uint32_t)__shfl(held, 4 * (t & 15) + (lane >> 4));
-      sc = (is_v ? a.vs : a.ks)[id * a.scale_page + (lane & 15) * (size_t)a.scale_token + kvh * a.scale_head];
+      sc = (wave ? a.vs : a.ks)[id * a.scale_page + (lane & 15) * (size_t)a.scale_token + kvh * a.scale_head];
     }
   };
-  auto stage = [&](int t, bool is_v) {
+  auto stage = [&](int t) {
     const int left = end - begin - t * kStTile, buf = t & 1;
-    u32x4* const dst = (is_v ? lds_v : lds_k)[buf];
     if (left < kStTile) {
       // slots behind the last token hold whatever was there and must not reach a product
 #pragma unroll
       for (int i = 0; i < NL; ++i)
-        if (16 * (k8 ? 2 * i + (tx >> 7) : i) + tok >= left) raw[i] = u32x4{0, 0, 0, 0};
+        if (16 * (k8 ? 2 * i + (tx >> 7) : i) + tok >= left) kraw[i] = vraw[i] = u32x4{0, 0, 0, 0};
       if (lane >= left) sc = 0.0f;
     }
 #pragma unroll
@@ -581,22 +598,26 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
       if (k8) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const u32x2 lo = widen4<KV>(raw[i][2 * h]), hi = widen4<KV>(raw[i][2 * h + 1]);
-          dst[row * 16 + ((2 * chunk + h) ^ tok)] = u32x4{lo.x, lo.y, hi.x, hi.y};
+          const int at = row * 16 + ((2 * chunk + h) ^ swizzle(tok));
+          const u32x2 k0 = widen4<KV>(kraw[i][2 * h]), k1 = widen4<KV>(kraw[i][2 * h + 1]);
+          lds.k[buf][at] = u32x4{k0.x, k0.y, k1.x, k1.y};
+          const u32x2 v0 = widen4<KV>(vraw[i][2 * h]), v1 = widen4<KV>(vraw[i][2 * h + 1]);
+          lds.v[buf][at] = u32x4{v0.x, v0.y, v1.x, v1.y};
         }
       } else {
-        dst[row * 16 + (chunk ^ tok)] = raw[i];
+        lds.k[buf][row * 16 + (chunk ^ swizzle(tok))] = kraw[i];
+        lds.v[buf][row * 16 + (chunk ^ swizzle(tok))] = vraw[i];
       }
     }
-    if (k8 && wave == 0) (is_v ? lds_vs : lds_ks)[buf][lane] = sc;
+    if (k8 && wave < 2) (wave ? lds.vs : lds.ks)[buf][lane] = sc;
   };
 
   // the products of 32 tokens: pages 2 h and 2 h + 1 of tile t
   auto products = [&](int t, int h, auto last) {
     constexpr bool cut = decltype(last)::value;
     const int left = end - begin - t * kStTile - 32 * h, buf = t & 1;
-    const u32x4* const kt = lds_k[buf] + 512 * h;
-    const u32x4* const vt = lds_v[buf] + 512 * h;
+    const u32x4* const kt = lds.k[buf] + 512 * h;
+    const u32x4* const vt = lds.v[buf] + 512 * h;
     f32x4 s[NQ][2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -604,7 +625,7 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
       for (int x = 0; x < NQ; ++x) s[x][p] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u32x4 kf = kt[(16 * p + n) * 16 + ((4 * j + kb) ^ n)];
+        const u32x4 kf = kt[(16 * p + n) * 16 + ((4 * j + kb) ^ swizzle(n))];
 #pragma unroll
         for (int x = 0; x < NQ; ++x) s[x][p] = mfma16<MT>(kf, qf[x][j], s[x][p]);
       }
@@ -612,28 +633,29 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
     f32x4 ks[2], vs[2];
     int rise = 0;
     if (k8) {
-      const float top = wave_allreduce<OpMax>(fabsf(lds_vs[buf][32 * h + (lane & 31)]));
+      const float top = wave_allreduce<OpMax>(fabsf(lds.vs[buf][32 * h + (lane & 31)]));
       const int e = max(min((as_i32(top) >> 23) - 127, 126), vexp);
       rise = e - vexp;
       vexp = e;
       const float down = as_f32((127 - vexp) << 23);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        ks[p] = *(const f32x4*)&lds_ks[buf][32 * h + 16 * p + 4 * kb];
-        vs[p] = *(const f32x4*)&lds_vs[buf][32 * h + 16 * p + 4 * kb] * down;
+        ks[p] = *(const f32x4*)&lds.ks[buf][32 * h + 16 * p + 4 * kb];
+        vs[p] = *(const f32x4*)&lds.vs[buf][32 * h + 16 * p + 4 * kb] * down;
       }
     }
     u32x4 pf[NQ];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      float top = kPaNoMax;
+      float top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float z = s[x][i >> 2][i & 3] * (k8 ? row_scale[x] * ks[i >> 2][i & 3] : row_scale[x]);
+        float z = k8 ? s[x][i >> 2][i & 3] * ks[i >> 2][i & 3] : s[x][i >> 2][i & 3];
         if (cut) z = 16 * (i >> 2) + 4 * kb + (i & 3) < left ? z : -__builtin_inff();
         s[x][i >> 2][i & 3] = z;
         top = fmaxf(top, z);
       }
+      top *= row_scale[x];
       if (__any(top > m[x] + kPaSlack)) {
         const float up = fmaxf(m[x], max_over_kb(top));
         const float alpha = __builtin_amdgcn_exp2f(m[x] - up);
@@ -650,48 +672,40 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(s[x][i >> 2][i & 3] - m[x]);
+        w[i] = __builtin_amdgcn_exp2f(fmaf(s[x][i >> 2][i & 3], row_scale[x], -m[x]));
         l[x] += w[i];
         if (k8) w[i] *= vs[i >> 2][i & 3];
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[x][i] = pack2<MT>(w[2 * i], w[2 * i + 1]);
     }
-    u32x4 v[8];
+    // lane n names channels 16 c + 4 (n % 4) .. + 3 of token 4 kb + n / 4 of either page
+    const int vrow = 4 * kb + (n >> 2), half = n & 1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int in_page = 4 * kb + (i & 3);
-      v[i] = vt[(16 * (i >> 2) + in_page) * 16 + (n ^ in_page)];
-    }
+    for (int c = 0; c < 8; ++c) {
+      const int at = vrow * 16 + ((2 * c + ((n >> 1) & 1)) ^ swizzle(vrow));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)((const uint8_t*)(vt + at) + 8 * half));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)((const uint8_t*)(vt + 256 + at) + 8 * half));
+      const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+      const u32x4 vf = {l2.x, l2.y, h2.x, h2.y};
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      u32x4 lo, hi;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x05040100u);
-        hi[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x07060302u);
-      }
-#pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        o[x][2 * c] = mfma16<MT>(lo, pf[x], o[x][2 * c]);
-        o[x][2 * c + 1] = mfma16<MT>(hi, pf[x], o[x][2 * c + 1]);
-      }
+      for (int x = 0; x < NQ; ++x) o[x][c] = mfma16<MT>(vf, pf[x], o[x][c]);
     }
   };
 
-  fetch(0, false);
-  stage(0, false);
-  fetch(0, true);
-  stage(0, true);
+  // tile t + 2 is asked for as soon as t + 1 has left the registers: it has a whole tile's products to arrive
+  fetch(0);
+  stage(0);
+  if (tiles > 1) fetch(1);
   __syncthreads();
   // all tiles but the last are whole, and a tile follows them
   for (int t = 0; t + 1 < tiles; ++t) {
-    fetch(t + 1, false);
-    if (busy) products(t, 0, Never{});
-    stage(t + 1, false);
-    fetch(t + 1, true);
-    if (busy) products(t, 1, Never{});
-    stage(t + 1, true);
+    if (busy) {
+      products(t, 0, Never{});
+      products(t, 1, Never{});
+    }
+    stage(t + 1);
+    if (t + 2 < tiles) fetch(t + 2);
     __syncthreads();
   }
   if (busy) {
@@ -706,23 +720,25 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
     const int row = row_of((wave * NQ + x) * 16 + n);
     if (row < 0) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        put_row<QT>(a, row, part, parts, 32 * kb + 8 * i + j,
-                    f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]} * vfac, m[x], total);
+    for (int c = 0; c < 8; ++c) put_row<QT>(a, row, part, parts, 16 * c + 4 * kb, o[x][c] * vfac, m[x], total);
   }
 }
 
 // Ways to attend to a prefix part.
 enum PrefixMode { kStream16, kStream32, kStream64, kStaged };
+template <int MODE>
+struct ModeLds { using type = PartLds<MODE == kStream16 ? 1 : 2, MODE == kStream64 ? 2 : 1>; };
+template <>
+struct ModeLds<kStaged> { using type = StagedLds; };
+constexpr size_t larger(size_t x, size_t y) { return x > y ? x : y; }
 constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStream32 ? 32 : mode == kStream64 ? 64 : kStRows; }
 
 // Grid: the prefix parts (eight of (kv head, part, group), row tile, the next eight, ...: the row tiles
 // of a part run side by side on one XCD and find its K and V in that L2), then the own parts (kv head,
-// part, request, row tile).
+// request, row tile, part: the parts that only long requests have come last).
 template <int QT, int KV, int MODE>
-__global__ __launch_bounds__(kPaThreads, MODE == kStream16 ? (KV == TWL_I8 ? 3 : 4) : 2) void prefix_attn_kernel(PrefixAttnArgs a) {
+__global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnArgs a) {
+  __shared__ __align__(16) uint8_t pool[larger(sizeof(typename ModeLds<MODE>::type), sizeof(PartLds<1, 1>))];
   const uint32_t parts = a.p_chunks + a.chunks;
   uint32_t id = blockIdx.x;
   if (id < a.p_blocks) {
@@ -747,17 +763,17 @@ __global__ __launch_bounds__(kPaThreads, MODE == kStream16 ? (KV == TWL_I8 ? 3 :
     const int32_t* ids = a.p_ids + a.p_ptr[g];
     const int num_ids = a.p_ptr[g + 1] - a.p_ptr[g];
     if constexpr (MODE == kStaged)
-      attend_staged<QT, KV>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts);
+      attend_staged<QT, KV>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts, pool);
     else
       attend_part<QT, KV, MODE == kStream16 ? 1 : 2, MODE == kStream64 ? 2 : 1>(a, ids, num_ids, begin, end, kvh,
-                                                                                row_of, c, parts);
+                                                                                row_of, c, parts, pool);
   } else {
     id -= a.p_blocks;
     const uint32_t kvh = id % a.num_kv_heads;
     id /= a.num_kv_heads;
-    const uint32_t c = id % a.chunks;
-    id /= a.chunks;
-    const uint32_t b = id % a.batch, tile = id / a.batch;
+    const uint32_t b = id % a.batch;
+    id /= a.batch;
+    const uint32_t tile = id % a.tiles, c = id / a.tiles;
     const int row0 = (int)(tile * 16);
     const int len = list_len(a.ptr, a.last, b, a.max_tokens);
     const int begin = (int)(c * a.chunk), end = min(len, begin + (int)a.chunk);
@@ -773,19 +789,21 @@ __global__ __launch_bounds__(kPaThreads, MODE == kStream16 ? (KV == TWL_I8 ? 3 :
       return;
     }
     attend_part<QT, KV, 1, 1>(a, a.ids + a.ptr[b], a.ptr[b + 1] - a.ptr[b], begin, end, kvh, row_of,
-                              a.p_chunks + c, parts);
+                              a.p_chunks + c, parts, pool);
   }
 }
 
-// Joins the parts of a row: one wavefront per row, two channels per lane. Which parts exist follows
-// from the lengths alone, so the workspace needs no initial contents. Where a row has at most one part
-// (a prefix of one part and no own tokens, or neither) it only writes the rows that see no token.
+// Joins the parts of a row: one workgroup per row, 32 threads per part (four channels each), eight parts
+// at a time, so that the parts of a long context are not fetched one after another. Which parts exist
+// follows from the lengths alone, so the workspace needs no initial contents. Where a row has at most
+// one part (a prefix of one part and no own tokens, or neither) it only writes the rows that see no token.
 template <int QT>
 __global__ __launch_bounds__(kPaThreads) void prefix_attn_merge_kernel(PrefixAttnArgs a) {
-  const uint32_t row = blockIdx.x * kPaWaves + threadIdx.x / kWave;
-  if (row >= a.batch * a.num_q_heads) return;
-  const uint32_t b = row / a.num_q_heads, parts = a.p_chunks + a.chunks;
-  const int lane = lane_id();
+  constexpr int kLists = kPaThreads / 32;
+  __shared__ float weight[2 * kPaMaxParts];
+  __shared__ f32x4 sums[kLists][32];
+  const uint32_t row = blockIdx.x, b = row / a.num_q_heads, parts = a.p_chunks + a.chunks;
+  const int lane = lane_id(), list = threadIdx.x >> 5, c = threadIdx.x & 31;
   int np = 0;
   if (a.p_chunks) {
     const int g = group_of(a, b);
@@ -797,31 +815,32 @@ __global__ __launch_bounds__(kPaThreads) void prefix_attn_merge_kernel(PrefixAtt
   if (parts <= 1 && count > 0) return;      // the part has written the row
   const size_t at = (size_t)row * parts;
   auto slot = [&](int i) { return i < np ? i : (int)a.p_chunks + i - np; };
+  // every wavefront finds the maximum and the sum for itself; the first one shares the weights
   float top = kPaNoMax;
   for (int i = lane; i < count; i += kWave) top = fmaxf(top, a.ml[at + slot(i)].x);
   top = wave_allreduce<OpMax>(top);
   float l = 0.0f;
-  f32x2 acc = {0.0f, 0.0f};
-  for (int i0 = 0; i0 < count; i0 += kWave) {
-    float w = 0.0f;
-    if (i0 + lane < count) {
-      const f32x2 ml = a.ml[at + slot(i0 + lane)];
-      w = __builtin_amdgcn_exp2f(ml.x - top);
-      l += w * ml.y;
-    }
-    const int here = min(count - i0, kWave);
-#pragma unroll 4
-    for (int i = 0; i < here; ++i) {
-      const float wi = as_f32(__builtin_amdgcn_readlane(as_i32(w), i));
-      const f32x2 x = *(const f32x2*)(a.acc + (at + slot(i0 + i)) * TWL_HEAD_DIM + 2 * lane);
-      acc.x = fmaf(wi, x.x, acc.x);
-      acc.y = fmaf(wi, x.y, acc.y);
-    }
+  for (int i = lane; i < count; i += kWave) {
+    const f32x2 ml = a.ml[at + slot(i)];
+    const float w = __builtin_amdgcn_exp2f(ml.x - top);
+    l += w * ml.y;
+    if (threadIdx.x < kWave) weight[i] = w;
   }
   l = wave_allreduce<OpSum>(l);
+  __syncthreads();
+  f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = list; i < count; i += kLists)
+    acc += *(const f32x4*)(a.acc + (at + slot(i)) * TWL_HEAD_DIM + 4 * c) * weight[i];
+  sums[list][c] = acc;
+  __syncthreads();
+  if (list > 0) return;
+#pragma unroll
+  for (int i = 1; i < kLists; ++i) acc += sums[i][c];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *(uint32_t*)((uint16_t*)a.out + (size_t)row * TWL_HEAD_DIM + 2 * lane) = pack2<QT>(acc.x * inv, acc.y * inv);
-  if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : top * kLn2 + logf(l);
+  *(u32x2*)((uint16_t*)a.out + (size_t)row * TWL_HEAD_DIM + 4 * c) =
+      u32x2{pack2<QT>(acc[0] * inv, acc[1] * inv), pack2<QT>(acc[2] * inv, acc[3] * inv)};
+  if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : top * kLn2 + logf(l);
 }
 
 // How a call is cut into workgroups: from the sizes alone, the same for the workspace and the launch.
@@ -830,10 +849,10 @@ struct PrefixPlan {
   uint32_t p_chunk, p_chunks, p_tiles, chunk, chunks, tiles;
 };
 
-constexpr uint32_t kPaMaxParts = 256;       // of one kind, per row
 
-static void cut_tokens(uint32_t tokens, uint64_t others, uint32_t target, uint32_t least, uint32_t* chunk,
+static void cut_tokens(uint32_t tokens, uint64_t others, uint32_t target, uint32_t most, uint32_t* chunk,
                        uint32_t* chunks) {
+  const uint32_t least = kPaWaves * kPaTile;
   *chunk = 0;
   *chunks = 0;
   if (tokens == 0 || others == 0) return;
@@ -841,6 +860,7 @@ static void cut_tokens(uint32_t tokens, uint64_t others, uint32_t target, uint32
   if (want > kPaMaxParts) want = kPaMaxParts;
   if (want < 1) want = 1;
   uint64_t c = (tokens + want - 1) / want;
+  if (c > most && (tokens + most - 1) / most <= kPaMaxParts) c = most;
   c = (c + least - 1) / least * least;
   *chunk = (uint32_t)c;
   *chunks = (uint32_t)((tokens + c - 1) / c);
@@ -855,9 +875,10 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
   p.mode = rows <= 16 ? kStream16 : rows <= 32 ? kStream32 : rows <= 64 ? kStream64 : kStaged;
   p.p_tiles = (uint32_t)((rows + mode_rows(p.mode) - 1) / mode_rows(p.mode));
   p.tiles = (G + 15) / 16;
-  cut_tokens(groups ? max_prefix : 0, (uint64_t)num_kv_heads * groups * p.p_tiles, 512, 128, &p.p_chunk,
+  cut_tokens(groups ? max_prefix : 0, (uint64_t)num_kv_heads * groups * p.p_tiles, 512, 1u << 24, &p.p_chunk,
              &p.p_chunks);
-  cut_tokens(max_tokens, (uint64_t)num_kv_heads * batch * p.tiles, 1024, 128, &p.chunk, &p.chunks);
+  const uint64_t lists = (uint64_t)num_kv_heads * batch * p.tiles;
+  cut_tokens(max_tokens, lists, 512, lists < 256 ? 1u << 24 : 2048, &p.chunk, &p.chunks);
   return p;
 }
 
@@ -964,7 +985,7 @@ extern "C" int twl_prefix_attn(
     if (hipGetLastError() != hipSuccess) return TWL_ELAUNCH;
   }
   if (p.p_chunks == 0 && p.chunks == 1) return TWL_OK;   // every row is written by its one part
-  const dim3 mgrid((uint32_t)((rows + twl::kPaWaves - 1) / twl::kPaWaves));
+  const dim3 mgrid((uint32_t)rows);
   if (dtype == TWL_F16)
     hipLaunchKernelGGL((twl::prefix_attn_merge_kernel<TWL_F16>), mgrid, dim3(twl::kPaThreads), 0, st, a);
   else
