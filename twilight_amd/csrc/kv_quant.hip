@@ -32,7 +32,6 @@ struct KvQuantArgs {
   const int32_t* kv_page_indptr;
   const int32_t* kv_last_page_len;
   uint32_t tokens, batch, num_kv_heads, num_pages;
-  uint64_t rows;                                // tokens * num_kv_heads
 };
 
 constexpr int kQuantThreads = 256;
@@ -83,7 +82,10 @@ __device__ __forceinline__ uint32_t row_amax_bits(const float* x) {
   return (uint32_t)m;
 }
 
-// codes of a lane's 8 channels, and the row's scale
+// codes of a lane's 8 channels, and the row's scale. x / scale as IEEE division rounds it, for the price
+// of one division per row: with r the correctly rounded 1 / scale and q0 = x r, one correction
+// q0 + r (x - q0 scale) in fused multiply-adds is the correctly rounded quotient (Markstein's
+// theorem), as long as the remainder is representable; rows too small for that divide.
 template <int FMT>
 __device__ __forceinline__ u32x2 quantise8(const float* x, float& scale) {
   const uint32_t amax = row_amax_bits(x);
@@ -94,8 +96,17 @@ __device__ __forceinline__ u32x2 quantise8(const float* x, float& scale) {
   }
   scale = fmaxf(as_f32(amax) / (FMT == TWL_I8 ? 127.0f : 448.0f), kQuantMinScale);
   float y[8];
+  if (scale >= 8.0779357e-28f) {            // 2^-90: good for quotients from 2^-13 on, smaller ones are code 0
+    const float r = 1.0f / scale;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = x[i] / scale;
+    for (int i = 0; i < 8; ++i) {
+      const float q = x[i] * r;
+      y[i] = copysignf(fmaf(fmaf(-q, scale, x[i]), r, q), x[i]);   // the correction loses the sign of -0
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i] / scale;
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t w = 0;
@@ -114,26 +125,44 @@ __device__ __forceinline__ u32x2 quantise8(const float* x, float& scale) {
   return codes;
 }
 
-template <int DT, int FMT>
+// Heads per row of 16 lanes: a bulk call takes four, so that finding the token's place is paid once and
+// eight loads are on their way; a decode step takes one and spreads wider.
+template <int HB>
+__device__ __forceinline__ bool token_and_head(const KvQuantArgs& a, uint32_t& t, uint32_t& h) {
+  const uint32_t sets = (a.num_kv_heads + HB - 1) / HB;
+  const uint64_t at = (uint64_t)blockIdx.x * (kQuantThreads / 16) + threadIdx.x / 16;
+  t = (uint32_t)(at / sets);
+  h = (uint32_t)(at - (uint64_t)t * sets) * HB;
+  return t < a.tokens;
+}
+
+template <int DT, int FMT, int HB>
 __global__ __launch_bounds__(kQuantThreads) void kv_quant_append_kernel(KvQuantArgs a) {
-  const uint64_t row = (uint64_t)blockIdx.x * (kQuantThreads / 16) + threadIdx.x / 16;
   const int sub = threadIdx.x & 15;
-  if (row >= a.rows) return;
-  const uint32_t t = (uint32_t)(row / a.num_kv_heads), h = (uint32_t)(row - (uint64_t)t * a.num_kv_heads);
-  const size_t src = t * a.dense_token + h * a.dense_head + 8 * sub;
-  const u32x4 kb = *(const u32x4*)((const uint16_t*)a.k_dense + src);
-  const u32x4 vb = *(const u32x4*)((const uint16_t*)a.v_dense + src);
+  uint32_t t, h;
+  if (!token_and_head<HB>(a, t, h)) return;
+  u32x4 kb[HB], vb[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    const size_t src = t * a.dense_token + min(h + i, a.num_kv_heads - 1) * a.dense_head + 8 * sub;
+    kb[i] = __builtin_nontemporal_load((const u32x4*)((const uint16_t*)a.k_dense + src));
+    vb[i] = __builtin_nontemporal_load((const u32x4*)((const uint16_t*)a.v_dense + src));
+  }
   uint32_t page, slot;
   if (find_row(a, t, page, slot) != kRowPlaced) return;
-  const size_t dst = page * a.page_stride + slot * a.token_stride + h * a.head_stride + 8 * sub;
-  const size_t sdst = page * a.scale_page + slot * a.scale_token + h * a.scale_head;
-  float x[8], scale;
-  unpack8<DT>(kb, x);
-  *(u32x2*)(a.k_cache + dst) = quantise8<FMT>(x, scale);
-  if (sub == 0) a.k_scale[sdst] = scale;
-  unpack8<DT>(vb, x);
-  *(u32x2*)(a.v_cache + dst) = quantise8<FMT>(x, scale);
-  if (sub == 0) a.v_scale[sdst] = scale;
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    if (h + i >= a.num_kv_heads) break;
+    const size_t dst = page * a.page_stride + slot * a.token_stride + (h + i) * a.head_stride + 8 * sub;
+    const size_t sdst = page * a.scale_page + slot * a.scale_token + (h + i) * a.scale_head;
+    float x[8], scale;
+    unpack8<DT>(kb[i], x);
+    *(u32x2*)(a.k_cache + dst) = quantise8<FMT>(x, scale);
+    if (sub == 0) a.k_scale[sdst] = scale;
+    unpack8<DT>(vb[i], x);
+    *(u32x2*)(a.v_cache + dst) = quantise8<FMT>(x, scale);
+    if (sub == 0) a.v_scale[sdst] = scale;
+  }
 }
 
 // the values a lane's 8 codes stand for
@@ -168,27 +197,38 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float* x) {
   }
 }
 
-template <int DT, int FMT>
+template <int DT, int FMT, int HB>
 __global__ __launch_bounds__(kQuantThreads) void kv_quant_read_kernel(KvQuantArgs a) {
-  const uint64_t row = (uint64_t)blockIdx.x * (kQuantThreads / 16) + threadIdx.x / 16;
   const int sub = threadIdx.x & 15;
-  if (row >= a.rows) return;
-  const uint32_t t = (uint32_t)(row / a.num_kv_heads), h = (uint32_t)(row - (uint64_t)t * a.num_kv_heads);
+  uint32_t t, h;
+  if (!token_and_head<HB>(a, t, h)) return;
   uint32_t page, slot;
   const int where = find_row(a, t, page, slot);
   if (where == kRowBehind) return;
-  float k[8] = {}, v[8] = {};
+  u32x2 kc[HB] = {}, vc[HB] = {};
+  float ks[HB] = {}, vs[HB] = {};
   if (where == kRowPlaced) {
-    const size_t src = page * a.page_stride + slot * a.token_stride + h * a.head_stride + 8 * sub;
-    const size_t ssrc = page * a.scale_page + slot * a.scale_token + h * a.scale_head;
-    const u32x2 kc = *(const u32x2*)(a.k_cache + src), vc = *(const u32x2*)(a.v_cache + src);
-    const float ks = a.k_scale[ssrc], vs = a.v_scale[ssrc];
-    dequantise8<FMT>(kc, ks, k);
-    dequantise8<FMT>(vc, vs, v);
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      const uint32_t hh = min(h + i, a.num_kv_heads - 1);
+      const size_t src = page * a.page_stride + slot * a.token_stride + hh * a.head_stride + 8 * sub;
+      const size_t ssrc = page * a.scale_page + slot * a.scale_token + hh * a.scale_head;
+      kc[i] = *(const u32x2*)(a.k_cache + src);
+      vc[i] = *(const u32x2*)(a.v_cache + src);
+      ks[i] = a.k_scale[ssrc];
+      vs[i] = a.v_scale[ssrc];
+    }
   }
-  const size_t dst = (size_t)row * TWL_HEAD_DIM + 8 * sub;
-  store8<DT>((void*)a.k_dense, dst, k);
-  store8<DT>((void*)a.v_dense, dst, v);
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    if (h + i >= a.num_kv_heads) break;
+    float x[8];
+    const size_t dst = ((size_t)t * a.num_kv_heads + h + i) * TWL_HEAD_DIM + 8 * sub;
+    dequantise8<FMT>(kc[i], ks[i], x);
+    store8<DT>((void*)a.k_dense, dst, x);
+    dequantise8<FMT>(vc[i], vs[i], x);
+    store8<DT>((void*)a.v_dense, dst, x);
+  }
 }
 
 // Checks that both directions share; fills everything but the dense side.
@@ -215,8 +255,16 @@ int kv_quant_args(KvQuantArgs& a, uint8_t* k_cache, uint8_t* v_cache, int format
   a.scale_head = scale_head; a.token_indptr = token_indptr; a.kv_page_indices = kv_page_indices;
   a.kv_page_indptr = kv_page_indptr; a.kv_last_page_len = kv_last_page_len; a.tokens = tokens;
   a.batch = batch; a.num_kv_heads = num_kv_heads; a.num_pages = num_pages;
-  a.rows = (uint64_t)tokens * num_kv_heads;
   return TWL_OK;
+}
+
+// Heads per row of 16 lanes, and the grid: four where that leaves two full loads of the chip (2 x 256
+// compute units x 8 workgroups of 16 rows).
+static bool quant_grid(const KvQuantArgs& a, dim3& grid) {
+  const uint64_t four = ((uint64_t)a.tokens * ((a.num_kv_heads + 3) / 4) + 15) / 16;
+  const bool bulk = a.num_kv_heads >= 4 && four >= 4096;
+  grid = dim3((uint32_t)(bulk ? four : ((uint64_t)a.tokens * a.num_kv_heads + 15) / 16));
+  return bulk;
 }
 
 }  // namespace twl
@@ -241,9 +289,13 @@ extern "C" int twl_kv_quant_append(
   if ((new_token_stride | new_head_stride) & 7u) return TWL_EALIGN;   // 16-byte loads
   if ((((uintptr_t)k_new) | ((uintptr_t)v_new)) & 15u) return TWL_EALIGN;
   a.k_dense = k_new; a.v_dense = v_new; a.dense_token = new_token_stride; a.dense_head = new_head_stride;
-  const dim3 grid((uint32_t)((a.rows + 15) / 16)), block(twl::kQuantThreads);
-#define TWL_APPEND(DT, FMT) \
-  hipLaunchKernelGGL((twl::kv_quant_append_kernel<DT, FMT>), grid, block, 0, (hipStream_t)stream, a)
+  dim3 grid, block(twl::kQuantThreads);
+  const bool bulk = twl::quant_grid(a, grid);
+#define TWL_APPEND(DT, FMT)                                                                                        \
+  do {                                                                                                             \
+    if (bulk) hipLaunchKernelGGL((twl::kv_quant_append_kernel<DT, FMT, 4>), grid, block, 0, (hipStream_t)stream, a); \
+    else hipLaunchKernelGGL((twl::kv_quant_append_kernel<DT, FMT, 1>), grid, block, 0, (hipStream_t)stream, a);      \
+  } while (0)
   if (dtype == TWL_F16) { if (format == TWL_I8) TWL_APPEND(TWL_F16, TWL_I8); else TWL_APPEND(TWL_F16, TWL_E4M3); }
   else { if (format == TWL_I8) TWL_APPEND(TWL_BF16, TWL_I8); else TWL_APPEND(TWL_BF16, TWL_E4M3); }
 #undef TWL_APPEND
@@ -268,9 +320,13 @@ extern "C" int twl_kv_quant_read(
   if (rc != TWL_OK) return rc;
   if ((((uintptr_t)k_out) | ((uintptr_t)v_out)) & 15u) return TWL_EALIGN;
   a.k_dense = k_out; a.v_dense = v_out;
-  const dim3 grid((uint32_t)((a.rows + 15) / 16)), block(twl::kQuantThreads);
-#define TWL_READ(DT, FMT) \
-  hipLaunchKernelGGL((twl::kv_quant_read_kernel<DT, FMT>), grid, block, 0, (hipStream_t)stream, a)
+  dim3 grid, block(twl::kQuantThreads);
+  const bool bulk = twl::quant_grid(a, grid);
+#define TWL_READ(DT, FMT)                                                                                        \
+  do {                                                                                                           \
+    if (bulk) hipLaunchKernelGGL((twl::kv_quant_read_kernel<DT, FMT, 4>), grid, block, 0, (hipStream_t)stream, a); \
+    else hipLaunchKernelGGL((twl::kv_quant_read_kernel<DT, FMT, 1>), grid, block, 0, (hipStream_t)stream, a);      \
+  } while (0)
 #define TWL_READ_DT(FMT)                            \
   if (dtype == TWL_F16) TWL_READ(TWL_F16, FMT);     \
   else if (dtype == TWL_BF16) TWL_READ(TWL_BF16, FMT); \

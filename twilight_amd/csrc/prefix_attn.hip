@@ -123,9 +123,10 @@ __device__ __forceinline__ u32x2 widen4(uint32_t w) {
   return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 
-template <bool NT, class T>
+// K and V of a streamed part are read once
+template <class T>
 __device__ __forceinline__ T load_kv(const uint8_t* p) {
-  return NT ? __builtin_nontemporal_load((const T*)p) : *(const T*)p;
+  return __builtin_nontemporal_load((const T*)p);
 }
 
 // Tokens of a page list, bounded by what the caller sized the launch for.
@@ -200,33 +201,31 @@ __device__ __forceinline__ void put_row(const PrefixAttnArgs& a, int row, uint32
 }
 
 // What the wavefronts of a workgroup exchange at the end of a part.
-template <int NQ, int WR>
+template <int NQ>
 struct PartLds {
   float o[kPaWaves][16 * NQ][TWL_HEAD_DIM + 4];
-  float m[kPaWaves][16 * NQ], l[kPaWaves][16 * NQ], top[WR][16 * NQ], total[WR][16 * NQ];
+  float m[kPaWaves][16 * NQ], l[kPaWaves][16 * NQ], top[16 * NQ], total[16 * NQ];
 };
 
 // One workgroup's part: tokens [begin, end) of a page list (first id at `ids`, `num_ids` of them)
-// for kv head kvh, and 16 * NQ * WR query rows. The four wavefronts are WR (1 or 2) sets of rows times
-// 4 / WR interleaved sets of token tiles. row_of(local row) -> row of q / out, or -1.
-template <int QT, int KV, int NQ, int WR, class RowOf>
+// for kv head kvh, and 16 * NQ query rows; the four wavefronts take every fourth tile each.
+// row_of(local row) -> row of q / out, or -1.
+template <int QT, int KV, int NQ, class RowOf>
 __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32_t* ids, int num_ids,
                                             int begin, int end, uint32_t kvh, RowOf row_of,
                                             uint32_t part, uint32_t parts, uint8_t* pool) {
   constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
   constexpr int MT = k8 ? TWL_F16 : QT;
-  constexpr int WT = kPaWaves / WR;
   constexpr int ROWS = 16 * NQ;
-  constexpr bool NT = WR == 1;              // several sets of rows read the pages again
   constexpr int NKL = k8 ? 2 : 4;           // 16-byte loads of K per lane and page
   const int lane = lane_id(), n = lane & 15, kb = lane >> 4;
-  const int wave = threadIdx.x / kWave, wr = wave / WT, wt = wave % WT;
+  const int wave = threadIdx.x / kWave;
 
   u32x4 qf[NQ][4];
   float row_scale[NQ];
 #pragma unroll
   for (int x = 0; x < NQ; ++x)
-    load_query<QT, k8, k8>(a, row_of((wr * NQ + x) * 16 + n), kb, qf[x], row_scale[x]);
+    load_query<QT, k8, k8>(a, row_of(x * 16 + n), kb, qf[x], row_scale[x]);
 
   f32x4 o[NQ][8];
   float m[NQ], l[NQ];
@@ -263,7 +262,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int j = 0; j < NKL; ++j) raw.k[p][j] = load_kv<NT, u32x4>(kp[p] + koff + 64 * j);
+      for (int j = 0; j < NKL; ++j) raw.k[p][j] = load_kv<u32x4>(kp[p] + koff + 64 * j);
     if (k8) {
       const float* sk = a.ks + kvh * a.scale_head;
       const float* sv = a.vs + kvh * a.scale_head;
@@ -287,11 +286,11 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
     for (int i = 0; i < 8; ++i) {
       const uint8_t* p = vp[i >> 2] + voff + (i & 3) * a.token_bytes;
       if (k8) {
-        const u32x2 w = load_kv<NT, u32x2>(p);
+        const u32x2 w = load_kv<u32x2>(p);
         raw.v[i].x = w.x;
         raw.v[i].y = w.y;
       } else {
-        raw.v[i] = load_kv<NT, u32x4>(p);
+        raw.v[i] = load_kv<u32x4>(p);
       }
     }
   };
@@ -441,9 +440,9 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   // the next tile is on its way while this one is worked on
   const int whole = (end - begin) / kPaTile;
   Raw cur, next;
-  if (wt < tiles) fetch(wt, cur);
-  for (int t = wt; t < tiles; t += WT) {
-    if (t + WT < tiles) fetch(t + WT, next);
+  if (wave < tiles) fetch(wave, cur);
+  for (int t = wave; t < tiles; t += kPaWaves) {
+    if (t + kPaWaves < tiles) fetch(t + kPaWaves, next);
     if (t < whole) step(t, cur, Never{});
     else step(t, cur, Always{});
     cur = next;
@@ -451,7 +450,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 
   // ---- join the wavefronts that share rows, and leave the part --------------------------------
   const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
-  auto& lds = *(PartLds<NQ, WR>*)pool;
+  auto& lds = *(PartLds<NQ>*)pool;
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
     l[x] = sum_over_kb(l[x]);
@@ -466,11 +465,11 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   for (int x = 0; x < NQ; ++x) {
     top[x] = kPaNoMax;
 #pragma unroll
-    for (int w = 0; w < WT; ++w) top[x] = fmaxf(top[x], lds.m[wr * WT + w][16 * x + n]);
+    for (int w = 0; w < kPaWaves; ++w) top[x] = fmaxf(top[x], lds.m[w][16 * x + n]);
     total[x] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WT; ++w)
-      total[x] += lds.l[wr * WT + w][16 * x + n] * __builtin_amdgcn_exp2f(lds.m[wr * WT + w][16 * x + n] - top[x]);
+    for (int w = 0; w < kPaWaves; ++w)
+      total[x] += lds.l[w][16 * x + n] * __builtin_amdgcn_exp2f(lds.m[w][16 * x + n] - top[x]);
     const float f = __builtin_amdgcn_exp2f(m[x] - top[x]) * vfac;
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[x][j] *= f;
@@ -485,22 +484,22 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         *(f32x4*)&lds.o[wave][16 * x + n][32 * kb + 8 * i + j] =
             f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]};
   // the maxima and sums of the joined rows
-  if (wt == 0 && kb == 0) {
+  if (wave == 0 && kb == 0) {
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      lds.top[wr][16 * x + n] = top[x];
-      lds.total[wr][16 * x + n] = total[x];
+      lds.top[16 * x + n] = top[x];
+      lds.total[16 * x + n] = total[x];
     }
   }
   __syncthreads();
-  for (int r = threadIdx.x >> 5; r < ROWS * WR; r += kPaThreads / 32) {
+  for (int r = threadIdx.x >> 5; r < ROWS; r += kPaThreads / 32) {
     const int row = row_of(r);
     if (row < 0) continue;
-    const int c = 4 * (threadIdx.x & 31), g = r / ROWS;
-    f32x4 x = *(const f32x4*)&lds.o[g * WT][r % ROWS][c];
+    const int c = 4 * (threadIdx.x & 31);
+    f32x4 x = *(const f32x4*)&lds.o[0][r][c];
 #pragma unroll
-    for (int w = 1; w < WT; ++w) x += *(const f32x4*)&lds.o[g * WT + w][r % ROWS][c];
-    put_row<QT>(a, row, part, parts, c, x, lds.top[g][r % ROWS], lds.total[g][r % ROWS]);
+    for (int w = 1; w < kPaWaves; ++w) x += *(const f32x4*)&lds.o[w][r][c];
+    put_row<QT>(a, row, part, parts, c, x, lds.top[r], lds.total[r]);
   }
 }
 
@@ -725,20 +724,20 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
 }
 
 // Ways to attend to a prefix part.
-enum PrefixMode { kStream16, kStream32, kStream64, kStaged };
+enum PrefixMode { kStream16, kStream32, kStaged };
 template <int MODE>
-struct ModeLds { using type = PartLds<MODE == kStream16 ? 1 : 2, MODE == kStream64 ? 2 : 1>; };
+struct ModeLds { using type = PartLds<MODE == kStream16 ? 1 : 2>; };
 template <>
 struct ModeLds<kStaged> { using type = StagedLds; };
 constexpr size_t larger(size_t x, size_t y) { return x > y ? x : y; }
-constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStream32 ? 32 : mode == kStream64 ? 64 : kStRows; }
+constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStream32 ? 32 : kStRows; }
 
 // Grid: the prefix parts (eight of (kv head, part, group), row tile, the next eight, ...: the row tiles
 // of a part run side by side on one XCD and find its K and V in that L2), then the own parts (kv head,
 // request, row tile, part: the parts that only long requests have come last).
 template <int QT, int KV, int MODE>
 __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnArgs a) {
-  __shared__ __align__(16) uint8_t pool[larger(sizeof(typename ModeLds<MODE>::type), sizeof(PartLds<1, 1>))];
+  __shared__ __align__(16) uint8_t pool[larger(sizeof(typename ModeLds<MODE>::type), sizeof(PartLds<1>))];
   const uint32_t parts = a.p_chunks + a.chunks;
   uint32_t id = blockIdx.x;
   if (id < a.p_blocks) {
@@ -765,8 +764,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnAr
     if constexpr (MODE == kStaged)
       attend_staged<QT, KV>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts, pool);
     else
-      attend_part<QT, KV, MODE == kStream16 ? 1 : 2, MODE == kStream64 ? 2 : 1>(a, ids, num_ids, begin, end, kvh,
-                                                                                row_of, c, parts, pool);
+      attend_part<QT, KV, MODE == kStream16 ? 1 : 2>(a, ids, num_ids, begin, end, kvh, row_of, c, parts, pool);
   } else {
     id -= a.p_blocks;
     const uint32_t kvh = id % a.num_kv_heads;
@@ -788,7 +786,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnAr
             put_row<QT>(a, row_of(r), 0, 1, 4 * (threadIdx.x & 31), f32x4{0, 0, 0, 0}, 0.0f, 0.0f);
       return;
     }
-    attend_part<QT, KV, 1, 1>(a, a.ids + a.ptr[b], a.ptr[b + 1] - a.ptr[b], begin, end, kvh, row_of,
+    attend_part<QT, KV, 1>(a, a.ids + a.ptr[b], a.ptr[b + 1] - a.ptr[b], begin, end, kvh, row_of,
                               a.p_chunks + c, parts, pool);
   }
 }
@@ -872,7 +870,7 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
   PrefixPlan p{};
   const uint32_t G = num_q_heads / num_kv_heads;
   const uint64_t rows = (uint64_t)max_group * G;
-  p.mode = rows <= 16 ? kStream16 : rows <= 32 ? kStream32 : rows <= 64 ? kStream64 : kStaged;
+  p.mode = rows <= 16 ? kStream16 : rows <= 32 ? kStream32 : kStaged;
   p.p_tiles = (uint32_t)((rows + mode_rows(p.mode) - 1) / mode_rows(p.mode));
   p.tiles = (G + 15) / 16;
   cut_tokens(groups ? max_prefix : 0, (uint64_t)num_kv_heads * groups * p.p_tiles, 512, 1u << 24, &p.p_chunk,
@@ -888,7 +886,6 @@ static void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& p, uint32_t
   hipLaunchKernelGGL((prefix_attn_kernel<QT, KV, MODE>), dim3(blocks), dim3(kPaThreads), 0, st, a)
   if (a.p_chunks == 0 || p.mode == kStream16) TWL_PA(kStream16);
   else if (p.mode == kStream32) TWL_PA(kStream32);
-  else if (p.mode == kStream64) TWL_PA(kStream64);
   else TWL_PA(kStaged);
 #undef TWL_PA
 }
