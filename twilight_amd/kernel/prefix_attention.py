@@ -101,13 +101,13 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
         check_input(out, "out"); check_same_device(q, ("out", out))
         if out.shape != q.shape or out.dtype != dtype:
             raise RuntimeError("out must match q")
-    lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     p_ids, p_ptr, p_last, g_ptr, groups, max_prefix, max_group = prefix
     L = _lib.lib()
     need = L.twl_prefix_attn_workspace_bytes(B, H, Hkv, groups, max_prefix, max_group, max_tokens)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     else:
         check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
         if workspace.numel() < need or workspace.device != dev:
@@ -116,8 +116,7 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
         q.data_ptr(), out.data_ptr(), _QUERY_TYPES[dtype], k_cache.data_ptr(), v_cache.data_ptr(), fmt, cs[0], cs[1],
         cs[2], ptr(k_scale), ptr(v_scale), *ss, k_cache.size(0), ptr(p_ids), ptr(p_ptr), ptr(p_last), ptr(g_ptr),
         groups, max_prefix, max_group, kv_page_indices.data_ptr(), kv_page_indptr.data_ptr(),
-        kv_last_page_len.data_ptr(), max_tokens, B, H, Hkv, scale, ptr(lse), workspace.data_ptr(), workspace.numel(),
-        stream)
+        kv_last_page_len.data_ptr(), max_tokens, B, H, Hkv, scale, ptr(lse), ptr(workspace), need, stream)
     if rc:
         _lib.check(rc, what)
     return (out, lse) if return_lse else out
