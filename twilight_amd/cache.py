@@ -7,30 +7,20 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .kernel import kv_append, kv_shadow_build, meta_planes_build
+from .kernel import kv_append, kv_quant_append, kv_quant_read, kv_shadow_build, meta_planes_build
 
 PAGE = _lib.PAGE
 HEAD_DIM = _lib.HEAD_DIM
 
 
-class PagedKVCache:
-    """K / V pages ``[num_pages, 16, Hkv, 128]`` (fp16 or bf16) plus ``k_int4``
-    ``[num_pages, Hkv, 1280]`` and ``meta`` ``[num_pages, Hkv, 512]`` (uint8 records), and the
-    CSR page table of the current batch (``kv_page_indices``, ``kv_page_indptr``,
-    ``kv_last_page_len``; the layout benchmark/efficiency/bench_gemv.py:425-431 builds)."""
+class _PageTable:
+    """CSR page table of the current batch (``kv_page_indices``, ``kv_page_indptr``, ``kv_last_page_len``;
+    the layout benchmark/efficiency/bench_gemv.py:425-431 builds) with its host mirror."""
 
-    def __init__(self, num_pages: int, num_kv_heads: int, dtype: torch.dtype, device):
-        if dtype not in (torch.float16, torch.bfloat16):
-            raise RuntimeError("PagedKVCache dtype must be float16 or bfloat16")
-        self.num_pages, self.num_kv_heads, self.dtype = num_pages, num_kv_heads, dtype
-        self.device = torch.device(device)
-        shape = (num_pages, PAGE, num_kv_heads, HEAD_DIM)
-        self.k_cache = torch.zeros(shape, dtype=dtype, device=self.device)
-        self.v_cache = torch.zeros(shape, dtype=dtype, device=self.device)
-        self.k_int4 = torch.zeros((num_pages, num_kv_heads, _lib.INT4_RECORD_BYTES),
-                                  dtype=torch.uint8, device=self.device)
-        self.meta = torch.zeros((num_pages, num_kv_heads, _lib.META_RECORD_BYTES),
-                                dtype=torch.uint8, device=self.device)
+    device: torch.device
+    meta_planes: Optional[torch.Tensor] = None
+
+    def _no_table(self) -> None:
         self.kv_page_indices: Optional[torch.Tensor] = None
         self.kv_page_indptr: Optional[torch.Tensor] = None
         self.kv_last_page_len: Optional[torch.Tensor] = None
@@ -39,12 +29,7 @@ class PagedKVCache:
         self._room = 0         # appends that surely fit every request's last page
         self._append_key = None
         self._table_cap = 0    # pages per request of a fixed-address page table (0: not fixed)
-        # Quest metadata in plane layout [slots, Hkv, 128, 2, cap] (see enable_planes) and the
-        # slot of every request of the batch (None: slot = position in the batch)
-        self.meta_planes: Optional[torch.Tensor] = None
-        self.plane_slots: Optional[torch.Tensor] = None
 
-    # ---- page table ---------------------------------------------------------------------------
     def set_page_table(self, kv_page_indices: torch.Tensor, kv_page_indptr: torch.Tensor,
                        kv_last_page_len: torch.Tensor) -> None:
         self.kv_page_indices = kv_page_indices.to(self.device, torch.int32).contiguous()
@@ -86,12 +71,86 @@ class PagedKVCache:
     def batch(self) -> int:
         return self.kv_page_indptr.numel() - 1
 
-    # ---- filling ------------------------------------------------------------------------------
     @property
     def max_seq_len(self) -> int:
         """Longest request of the batch in tokens (host-side count, no device read)."""
         return max(self._seq_lens) if self._seq_lens else 0
 
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, free_pages: Optional[list] = None) -> None:
+        """Decode append of one token per request: ``k_new`` / ``v_new`` [B, Hkv, 128]. Extends the
+        page table when a request's last page is full (taking ids from ``free_pages``; host-side
+        bookkeeping only, nothing is read back from the device), then one kernel writes the token
+        and updates the lengths (and, beside 16-bit pages, the shadow records). The two halves are also callable on their
+        own: :meth:`advance_host` every step before a recorded step is replayed,
+        :meth:`append_device` inside the recorded step."""
+        self.advance_host(free_pages)
+        self.append_device(k_new, v_new)
+
+    def advance_host(self, free_pages: Optional[list] = None) -> None:
+        """Host half of :meth:`append`: make room for one more token per request (a new page from
+        ``free_pages`` where the last one is full) and count the token."""
+        B = self.batch
+        per_req, last = self._per_req, self._last
+        grew = False
+        if self._room <= 0:  # some request may have filled its last page
+            for b in range(B):
+                if last[b] == PAGE:
+                    if not free_pages:
+                        raise RuntimeError("PagedKVCache.append: no free page left")
+                    per_req[b].append(int(free_pages.pop(0)))
+                    last[b] = 0
+                    grew = True
+            self._room = PAGE - max(last)
+        if grew:  # a request took a new page: the CSR arrays change shape, lengths are re-sent
+            flat = [p for r in per_req for p in r]
+            ptr = [0]
+            for r in per_req:
+                ptr.append(ptr[-1] + len(r))
+            if self._table_cap:
+                if max(len(r) for r in per_req) > self._table_cap:
+                    raise RuntimeError("PagedKVCache.append: request outgrew reserve_page_table")
+                self.kv_page_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
+                self.kv_page_indptr.copy_(torch.tensor(ptr, dtype=torch.int32))
+            else:
+                self.kv_page_indices = torch.tensor(flat, dtype=torch.int32, device=self.device)
+                self.kv_page_indptr = torch.tensor(ptr, dtype=torch.int32, device=self.device)
+                self.max_pages_per_req = max(len(r) for r in per_req)
+            if self.meta_planes is not None and self.max_pages_per_req > self.meta_planes.size(4):
+                raise RuntimeError("PagedKVCache.append: request outgrew the plane buffer "
+                                   "(enable_planes with a larger cap_pages)")
+            # same tensor object every step, so cached argument blocks of the layer stay valid
+            self.kv_last_page_len.copy_(torch.tensor(last, dtype=torch.int32))
+        self._room -= 1
+        for b in range(B):
+            last[b] += 1
+            self._seq_lens[b] += 1
+
+
+class PagedKVCache(_PageTable):
+    """K / V pages ``[num_pages, 16, Hkv, 128]`` (fp16 or bf16) plus ``k_int4``
+    ``[num_pages, Hkv, 1280]`` and ``meta`` ``[num_pages, Hkv, 512]`` (uint8 records), and the
+    CSR page table of the current batch (``kv_page_indices``, ``kv_page_indptr``,
+    ``kv_last_page_len``; the layout benchmark/efficiency/bench_gemv.py:425-431 builds)."""
+
+    def __init__(self, num_pages: int, num_kv_heads: int, dtype: torch.dtype, device):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError("PagedKVCache dtype must be float16 or bfloat16")
+        self.num_pages, self.num_kv_heads, self.dtype = num_pages, num_kv_heads, dtype
+        self.device = torch.device(device)
+        shape = (num_pages, PAGE, num_kv_heads, HEAD_DIM)
+        self.k_cache = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.v_cache = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.k_int4 = torch.zeros((num_pages, num_kv_heads, _lib.INT4_RECORD_BYTES),
+                                  dtype=torch.uint8, device=self.device)
+        self.meta = torch.zeros((num_pages, num_kv_heads, _lib.META_RECORD_BYTES),
+                                dtype=torch.uint8, device=self.device)
+        self._no_table()
+        # Quest metadata in plane layout [slots, Hkv, 128, 2, cap] (see enable_planes) and the
+        # slot of every request of the batch (None: slot = position in the batch)
+        self.meta_planes: Optional[torch.Tensor] = None
+        self.plane_slots: Optional[torch.Tensor] = None
+
+    # ---- filling ------------------------------------------------------------------------------
     def rebuild_shadow(self, page_ids: Optional[torch.Tensor] = None,
                        valid_len: Optional[torch.Tensor] = None) -> None:
         """(Re)build INT4 records and Quest metadata of ``page_ids`` (default: every page, all 16
@@ -186,55 +245,6 @@ class PagedKVCache:
             c.enable_planes(plane_pages)
         return c
 
-    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, free_pages: Optional[list] = None) -> None:
-        """Decode append of one token per request: ``k_new`` / ``v_new`` [B, Hkv, 128]. Extends the
-        page table when a request's last page is full (taking ids from ``free_pages``; host-side
-        bookkeeping only, nothing is read back from the device), then one kernel writes the token
-        and updates the shadow records and the lengths. The two halves are also callable on their
-        own: :meth:`advance_host` every step before a recorded step is replayed,
-        :meth:`append_device` inside the recorded step."""
-        self.advance_host(free_pages)
-        self.append_device(k_new, v_new)
-
-    def advance_host(self, free_pages: Optional[list] = None) -> None:
-        """Host half of :meth:`append`: make room for one more token per request (a new page from
-        ``free_pages`` where the last one is full) and count the token."""
-        B = self.batch
-        per_req, last = self._per_req, self._last
-        grew = False
-        if self._room <= 0:  # some request may have filled its last page
-            for b in range(B):
-                if last[b] == PAGE:
-                    if not free_pages:
-                        raise RuntimeError("PagedKVCache.append: no free page left")
-                    per_req[b].append(int(free_pages.pop(0)))
-                    last[b] = 0
-                    grew = True
-            self._room = PAGE - max(last)
-        if grew:  # a request took a new page: the CSR arrays change shape, lengths are re-sent
-            flat = [p for r in per_req for p in r]
-            ptr = [0]
-            for r in per_req:
-                ptr.append(ptr[-1] + len(r))
-            if self._table_cap:
-                if max(len(r) for r in per_req) > self._table_cap:
-                    raise RuntimeError("PagedKVCache.append: request outgrew reserve_page_table")
-                self.kv_page_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
-                self.kv_page_indptr.copy_(torch.tensor(ptr, dtype=torch.int32))
-            else:
-                self.kv_page_indices = torch.tensor(flat, dtype=torch.int32, device=self.device)
-                self.kv_page_indptr = torch.tensor(ptr, dtype=torch.int32, device=self.device)
-                self.max_pages_per_req = max(len(r) for r in per_req)
-            if self.meta_planes is not None and self.max_pages_per_req > self.meta_planes.size(4):
-                raise RuntimeError("PagedKVCache.append: request outgrew the plane buffer "
-                                   "(enable_planes with a larger cap_pages)")
-            # same tensor object every step, so cached argument blocks of the layer stay valid
-            self.kv_last_page_len.copy_(torch.tensor(last, dtype=torch.int32))
-        self._room -= 1
-        for b in range(B):
-            last[b] += 1
-            self._seq_lens[b] += 1
-
     def append_device(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         """Device half of :meth:`append`: one launch writes the token of every request at the
         position the device-side lengths give (and adds one to them), its INT4 codes and the
@@ -275,3 +285,70 @@ class PagedKVCache:
                     0 if planes is None else planes.size(0),
                     torch.cuda.current_stream(self.device).cuda_stream)
             _lib.check(rc, "KvAppend")
+
+
+class QuantPagedKVCache(_PageTable):
+    """K / V pages held in 8 bits: ``k_cache`` / ``v_cache`` [num_pages, 16, Hkv, 128] of ``int8`` or
+    ``float8_e4m3fn`` codes (views; in memory a page keeps a head's 16 tokens together) and
+    ``k_scale`` / ``v_scale`` fp32 [num_pages, 16, Hkv], with the page table and the decode append of
+    :class:`PagedKVCache`. For dense decode: :func:`twilight_amd.kernel.quant_paged_decode_attention`
+    and :func:`~twilight_amd.kernel.prefix_paged_decode_attention` read it in place."""
+
+    def __init__(self, num_pages: int, num_kv_heads: int, fmt: torch.dtype, device):
+        if fmt not in (torch.int8, torch.float8_e4m3fn):
+            raise RuntimeError("QuantPagedKVCache holds int8 or float8_e4m3fn codes")
+        self.num_pages, self.num_kv_heads, self.dtype = num_pages, num_kv_heads, fmt
+        self.device = torch.device(device)
+        shape = (num_pages, num_kv_heads, PAGE)
+
+        def pool(*more, dtype):
+            return torch.zeros(shape + more, dtype=dtype, device=self.device).transpose(1, 2)
+
+        self.k_cache, self.v_cache = (pool(HEAD_DIM, dtype=torch.uint8).view(fmt) for _ in range(2))
+        self.k_scale, self.v_scale = (pool(dtype=torch.float32) for _ in range(2))
+        self._one_each: Optional[torch.Tensor] = None
+        self._no_table()
+
+    @property
+    def pools(self):
+        """``(k_cache, v_cache, k_scale, v_scale)``, as the ops take them."""
+        return self.k_cache, self.v_cache, self.k_scale, self.v_scale
+
+    @property
+    def table(self):
+        """``(kv_page_indices, kv_page_indptr, kv_last_page_len)``, as the ops take them."""
+        return self.kv_page_indices, self.kv_page_indptr, self.kv_last_page_len
+
+    @classmethod
+    def from_dense(cls, k: torch.Tensor, v: torch.Tensor, fmt: torch.dtype, device,
+                   spare_pages: int = 0) -> "QuantPagedKVCache":
+        """Quantise dense ``k`` / ``v`` [B, Hkv, N, 128] (fp16 / bf16) into pages (prefill fill)."""
+        B, Hkv, N, D = k.shape
+        if D != HEAD_DIM or v.shape != k.shape:
+            raise RuntimeError("k and v must be [B, Hkv, N, 128]")
+        npg = (N + PAGE - 1) // PAGE
+        c = cls(B * npg + spare_pages, Hkv, fmt, device)
+        c.set_page_table(torch.arange(B * npg, dtype=torch.int32), (torch.arange(B + 1) * npg).to(torch.int32),
+                         torch.full((B,), N - (npg - 1) * PAGE, dtype=torch.int32))
+        rows = [x.to(c.device).transpose(1, 2).reshape(B * N, Hkv, D) for x in (k, v)]
+        ptr = (torch.arange(B + 1) * N).to(c.device, torch.int32)
+        kv_quant_append(rows[0], rows[1], ptr, *c.pools, *c.table)
+        return c
+
+    def append_device(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+        """Device half of :meth:`append`: count one token per request and write it, ``k_new`` / ``v_new``
+        [B, Hkv, 128] (fp16 / bf16). :meth:`advance_host` must have made room for it."""
+        if self._one_each is None or self._one_each.numel() != self.batch + 1:
+            self._one_each = torch.arange(self.batch + 1, dtype=torch.int32, device=self.device)
+        self.kv_last_page_len.add_(1)
+        if k_new.stride() != v_new.stride() or k_new.stride(-1) != 1:
+            k_new, v_new = k_new.contiguous(), v_new.contiguous()
+        kv_quant_append(k_new, v_new, self._one_each, *self.pools, *self.table)
+
+    def read(self, dtype: torch.dtype = torch.bfloat16):
+        """The values of every request's tokens, ``(k, v)`` [sum of lengths, Hkv, 128] in order."""
+        ptr = [0]
+        for n in self._seq_lens:
+            ptr.append(ptr[-1] + n)
+        indptr = torch.tensor(ptr, dtype=torch.int32, device=self.device)
+        return kv_quant_read(*self.pools, *self.table, indptr, ptr[-1], dtype=dtype)

@@ -20,9 +20,11 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from . import _lib
-from .cache import PagedKVCache
+from .cache import PagedKVCache, QuantPagedKVCache
 from .kernel.attention import (group_attention_workspace_bytes, group_paged_decode_attention,
                                rope_qk_)
+from .kernel.prefix_attention import (prefix_attention_workspace_bytes,
+                                      quant_paged_decode_attention)
 from .layer import TwilightDecodeLayer, parse_sparse_config
 
 PAGE = _lib.PAGE
@@ -161,7 +163,8 @@ class _LayerState:
 
     def __init__(self, cfg: dict, reserve_tokens: int, budget_info: Optional[HistoryBudgetInfo],
                  keep_hf_cache: bool, score_info: Optional[HistoryAccumulatedScoreInfo] = None,
-                 dense: bool = False):
+                 dense: bool = False, dense_kv: Optional[torch.dtype] = None):
+        self.dense_kv = dense_kv  # 8-bit format of a dense layer's pages (None: the model's dtype)
         self.cfg, self.reserve_tokens, self.budget_info = cfg, reserve_tokens, budget_info
         self.keep_hf_cache, self.score_info = keep_hf_cache, score_info
         self.dense = dense        # a layer the configuration leaves dense, served from paged K / V
@@ -189,14 +192,19 @@ def fill_from_prefill(st: _LayerState, k: torch.Tensor, v: torch.Tensor, num_q_h
     # plane-layout metadata next to the records: the one-launch selector reads half the bytes from
     # it (with GQA it is used at the batch sizes where that launch runs, the records otherwise)
     planes = npg + spare_per_req
-    st.cache = PagedKVCache.from_dense(k, v, k.device, spare_pages=B * spare_per_req,
-                                       plane_pages=None if st.dense else planes)
+    if st.dense_kv is not None:
+        st.cache = QuantPagedKVCache.from_dense(k, v, st.dense_kv, k.device, spare_pages=B * spare_per_req)
+    else:
+        st.cache = PagedKVCache.from_dense(k, v, k.device, spare_pages=B * spare_per_req,
+                                           plane_pages=None if st.dense else planes)
     st.free = list(range(B * npg, B * (npg + spare_per_req)))
     st.seq_len = N
     if st.dense:
         st.max_tokens = (npg + spare_per_req) * PAGE
-        st.workspace = torch.empty(group_attention_workspace_bytes(
-            B, num_q_heads, k.shape[1], st.max_tokens, False), dtype=torch.uint8, device=k.device)
+        need = group_attention_workspace_bytes(B, num_q_heads, k.shape[1], st.max_tokens, False) \
+            if st.dense_kv is None else \
+            prefix_attention_workspace_bytes(B, num_q_heads, k.shape[1], 0, 0, 0, st.max_tokens)
+        st.workspace = torch.empty(need, dtype=torch.uint8, device=k.device)
         return
     st.layer = TwilightDecodeLayer(st.cache, num_q_heads, reserve_pages=npg + spare_per_req, **st.cfg)
 
@@ -272,11 +280,14 @@ def _twilight_attention_forward(self, hidden_states, position_embeddings=None, a
         st.cache.append(k[:, :, 0], v[:, :, 0], st.free)
         st.seq_len += 1
     if st.dense:
-        c = st.cache
-        out = group_paged_decode_attention(
-            q[:, :, 0].contiguous(), c.k_cache, c.v_cache, c.kv_page_indices, c.kv_page_indptr,
-            c.kv_last_page_len, max_tokens=st.max_tokens, sm_scale=getattr(self, "scaling", None),
-            workspace=st.workspace)
+        c, args = st.cache, dict(max_tokens=st.max_tokens, sm_scale=getattr(self, "scaling", None),
+                                 workspace=st.workspace)
+        if st.dense_kv is not None:
+            out = quant_paged_decode_attention(q[:, :, 0].contiguous(), *c.pools, *c.table, **args)
+        else:
+            out = group_paged_decode_attention(
+                q[:, :, 0].contiguous(), c.k_cache, c.v_cache, c.kv_page_indices, c.kv_page_indptr,
+                c.kv_last_page_len, **args)
         return self.o_proj(out.reshape(B, 1, -1)), None
     out = st.layer(q[:, :, 0].contiguous())           # [B, H, 128]
     if st.budget_info is not None and not st.recorded:
@@ -293,7 +304,8 @@ def enable_sparse_attention(model, sparse_config: Dict, enable_budget_info: bool
                             enable_score_info: bool = False, reserve_tokens: int = 4096,
                             high: str = "max", keep_hf_cache: bool = True,
                             dense_layers: str = "model",
-                            group_select: bool = False) -> Tuple[Optional[HistoryBudgetInfo],
+                            group_select: bool = False,
+                            dense_kv: str = "model") -> Tuple[Optional[HistoryBudgetInfo],
                                        Optional[HistoryAccumulatedScoreInfo]]:
     """Patch every Llama / Mistral attention module of ``model`` (twilight/pyimpl/attention.py:
     351-418, 481-493). ``sparse_config`` is the reference's JSON template
@@ -322,6 +334,11 @@ def enable_sparse_attention(model, sparse_config: Dict, enable_budget_info: bool
     skip = 2 if sparse_config.get("skip_first_two_layers", True) else 0
     if dense_layers not in ("model", "paged"):
         raise RuntimeError(f"dense_layers must be 'model' or 'paged', got {dense_layers!r}")
+    formats = {"model": None, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+    if dense_kv not in formats:
+        raise RuntimeError(f"dense_kv must be 'model', 'int8' or 'e4m3', got {dense_kv!r}")
+    if dense_kv != "model" and dense_layers != "paged":
+        raise RuntimeError("dense_kv needs dense_layers='paged'")
     if not keep_hf_cache and skip == 0:
         raise RuntimeError("keep_hf_cache=False needs skip_first_two_layers")
     budget_info = HistoryBudgetInfo() if enable_budget_info else None
@@ -339,7 +356,8 @@ def enable_sparse_attention(model, sparse_config: Dict, enable_budget_info: bool
             continue
         module._twilight_state = _LayerState(dict(cfg), reserve_tokens,
                                              None if dense else budget_info, keep_hf_cache,
-                                             None if dense else score_info, dense=dense)
+                                             None if dense else score_info, dense=dense,
+                                             dense_kv=formats[dense_kv] if dense else None)
         module._twilight_orig_forward = module.forward
         module.forward = types.MethodType(_twilight_attention_forward, module)
         patched += 1
