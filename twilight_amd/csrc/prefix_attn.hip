@@ -45,6 +45,7 @@ constexpr int kPaTile = 32;                 // tokens of one step of a wavefront
 constexpr float kPaNoMax = -3.0e38f;        // running maximum before the first token
 constexpr float kPaSlack = 8.0f;            // how far a logit may exceed it, in base 2
 constexpr uint32_t kPaMaxParts = 256;       // of one kind, per row
+constexpr float kPaLeastScale = 1.17549435e-38f;   // 2^-126: -inf times it is -inf
 constexpr float kLn2 = 0.693147180559945309f;
 
 struct PrefixAttnArgs {
@@ -154,14 +155,16 @@ __device__ __forceinline__ int group_of(const PrefixAttnArgs& a, uint32_t b) {
 template <int QT, bool PAIRED, bool TO_F16>
 __device__ __forceinline__ void load_query(const PrefixAttnArgs& a, int row, int kb, u32x4* qf, float& scale) {
   const uint16_t* src = a.q + (size_t)max(row, 0) * TWL_HEAD_DIM;
-  // positive, so that the largest product is the largest logit; not zero, so that a masked one stays masked
-  scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+  // positive, so that the largest product is the largest logit and a masked one stays masked: a negative
+  // scale turns the query, a scale of zero clears it
+  const bool flat = a.scale_log2 == 0.0f;
+  scale = flat ? 1.0f : fabsf(a.scale_log2);
   const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int d = PAIRED ? 64 * (j >> 1) + 16 * kb + 8 * (j & 1) : 32 * j + 8 * kb;
     qf[j] = *(const u32x4*)(src + d);
-    if (row < 0) qf[j] = u32x4{0, 0, 0, 0};
+    if (row < 0 || flat) qf[j] = u32x4{0, 0, 0, 0};
     else qf[j] ^= sign;
   }
   if (TO_F16 && QT == TWL_BF16) {
@@ -182,6 +185,7 @@ __device__ __forceinline__ void load_query(const PrefixAttnArgs& a, int row, int
 #pragma unroll
       for (int i = 0; i < 4; ++i) qf[j][i] = pack2<TWL_F16>(f[j][2 * i] * down, f[j][2 * i + 1] * down);
   }
+  scale = fmaxf(scale, kPaLeastScale);
 }
 
 // Four channels of a row's part: into the workspace, or, where a row has one part, the answer.
@@ -847,7 +851,6 @@ struct PrefixPlan {
   uint32_t p_chunk, p_chunks, p_tiles, chunk, chunks, tiles;
 };
 
-
 static void cut_tokens(uint32_t tokens, uint64_t others, uint32_t target, uint32_t most, uint32_t* chunk,
                        uint32_t* chunks) {
   const uint32_t least = kPaWaves * kPaTile;
@@ -936,7 +939,7 @@ extern "C" int twl_prefix_attn(
   if (groups && (max_group_size == 0 || max_group_size > batch)) return TWL_EINVAL;
   if (max_tokens > (1u << 24) || max_prefix_tokens > (1u << 24)) return TWL_EINVAL;
   if (token_stride > (1u << 24) || scale_token_stride > (1u << 24)) return TWL_EINVAL;
-  if (!(sm_scale == sm_scale)) return TWL_EINVAL;
+  if (!(sm_scale - sm_scale == 0.0f)) return TWL_EINVAL;   // infinite or NaN
   const uint64_t align = k8 ? 15u : 7u;     // 16-byte loads of a token's channels
   if ((page_stride | token_stride | head_stride) & align) return TWL_EALIGN;
   if ((((uintptr_t)q) | ((uintptr_t)k_cache) | ((uintptr_t)v_cache) | ((uintptr_t)workspace)) & 15u)
@@ -952,7 +955,7 @@ extern "C" int twl_prefix_attn(
   if (workspace_bytes < need) return TWL_EINVAL;
   const uint64_t p_blocks = ((uint64_t)num_kv_heads * p.p_chunks * groups + 7) / 8 * 8 * p.p_tiles;
   const uint64_t blocks = p_blocks + (uint64_t)num_kv_heads * p.chunks * batch * p.tiles;
-  if (blocks > 0x7FFFFFFFull) return TWL_EINVAL;
+  if (blocks > 0xFFFFFFull) return TWL_EINVAL;   // 2^32 threads
   const uint64_t parts = (uint64_t)p.p_chunks + p.chunks, rows = (uint64_t)batch * num_q_heads;
   twl::PrefixAttnArgs a{};
   const uint64_t eb = k8 ? 1 : 2;
