@@ -126,3 +126,29 @@ def test_quant_cache_shares_the_page_table(hip_lib):
     c.advance_host(free)
     assert c.kv_page_indices.tolist() == [0, 4, 1] and c.kv_last_page_len.tolist() == [0, 3] and free == [5]
     assert c._seq_lens == [17, 4]
+
+
+def test_calls_too_large_for_one_launch_and_scales_that_are_no_number(hip_lib):
+    # 2^28 rows of 16 lanes are 2^32 threads
+    assert _append(hip_lib, tokens=1 << 26, hkv=4) == -2 and _read(hip_lib, tokens=1 << 26, hkv=4) == -2
+    assert _attn(hip_lib, scale=float("inf")) == -2 and _attn(hip_lib, scale=float("-inf")) == -2
+
+
+def test_arguments_that_are_no_tensors(hip_lib):
+    pools, table, i32 = _cpu_cache()
+    q = torch.zeros(1, 4, 128, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="[Tt]ensor"):
+        K.quant_paged_decode_attention(None, *pools, *table, max_tokens=3)
+    with pytest.raises(RuntimeError, match="[Tt]ensor"):
+        K.quant_paged_decode_attention(q, [1], *pools[1:], *table, max_tokens=3)
+    with pytest.raises(RuntimeError, match="[Tt]ensor"):
+        K.kv_quant_read(None, *pools[1:], *table, i32(0, 3), 3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        K.kv_quant_append(None, None, [0, 3], *pools, *table)
+
+
+def test_quant_cache_counts_its_appends_with_the_table(hip_lib):
+    # the row counts of an append exist before a step is recorded, not from the recording on
+    c = QuantPagedKVCache(6, 2, torch.float8_e4m3fn, "cpu")
+    c.set_page_table(torch.tensor([0, 1, 2]), torch.tensor([0, 1, 2, 3]), torch.tensor([16, 3, 1]))
+    assert c._one_each.tolist() == [0, 1, 2, 3]

@@ -306,8 +306,13 @@ class QuantPagedKVCache(_PageTable):
 
         self.k_cache, self.v_cache = (pool(HEAD_DIM, dtype=torch.uint8).view(fmt) for _ in range(2))
         self.k_scale, self.v_scale = (pool(dtype=torch.float32) for _ in range(2))
-        self._one_each: Optional[torch.Tensor] = None
+        self._one_each: Optional[torch.Tensor] = None   # one new token per request, of an append
         self._no_table()
+
+    def set_page_table(self, kv_page_indices: torch.Tensor, kv_page_indptr: torch.Tensor,
+                       kv_last_page_len: torch.Tensor) -> None:
+        super().set_page_table(kv_page_indices, kv_page_indptr, kv_last_page_len)
+        self._one_each = torch.arange(self.batch + 1, dtype=torch.int32, device=self.device)
 
     @property
     def pools(self):
@@ -338,8 +343,6 @@ class QuantPagedKVCache(_PageTable):
     def append_device(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         """Device half of :meth:`append`: count one token per request and write it, ``k_new`` / ``v_new``
         [B, Hkv, 128] (fp16 / bf16). :meth:`advance_host` must have made room for it."""
-        if self._one_each is None or self._one_each.numel() != self.batch + 1:
-            self._one_each = torch.arange(self.batch + 1, dtype=torch.int32, device=self.device)
         self.kv_last_page_len.add_(1)
         if k_new.stride() != v_new.stride() or k_new.stride(-1) != 1:
             k_new, v_new = k_new.contiguous(), v_new.contiguous()

@@ -245,7 +245,7 @@ int kv_quant_args(KvQuantArgs& a, uint8_t* k_cache, uint8_t* v_cache, int format
   if (tokens == 0 || batch == 0 || num_kv_heads == 0 || num_pages == 0 || tokens > 0x7FFFFFFFu ||
       num_pages > 0x7FFFFFFFu)
     return TWL_EINVAL;
-  if (((uint64_t)tokens * num_kv_heads + 15) / 16 > 0x7FFFFFFFull) return TWL_EINVAL;
+  if (((uint64_t)tokens * num_kv_heads + 15) / 16 > 0xFFFFFFull) return TWL_EINVAL;   // 2^32 threads
   if ((page_stride | token_stride | head_stride) & 7u) return TWL_EALIGN;
   if ((((uintptr_t)k_cache) | ((uintptr_t)v_cache)) & 7u) return TWL_EALIGN;
   if ((((uintptr_t)k_scale) | ((uintptr_t)v_scale)) & 3u) return TWL_EALIGN;

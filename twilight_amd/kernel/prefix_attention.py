@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._check import (check_dim, check_dtype, check_input, check_same_device, fine_rows, ptr,
+from ._check import (check_cuda, check_dim, check_dtype, check_input, check_same_device, fine_rows, ptr,
                      stream_and_switch)
 from .attention import _cache_strides
 from .quant_cache import KV_FORMATS, check_page_table, check_quant_cache
@@ -33,23 +33,26 @@ def _bound(value, name: str, least: int) -> int:
 
 def _fine(q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len) -> bool:
     """Whether the operands are plainly right; if not, :func:`_check` finds out what is wrong."""
-    dev, cs = q.device, k_cache.stride()
-    if not (q.is_cuda and q.dim() == 3 and q.is_contiguous() and q.dtype in _QUERY_TYPES and len(cs) == 4
-            and v_cache.stride() == cs and cs[3] == 1 and v_cache.shape == k_cache.shape
-            and v_cache.dtype is k_cache.dtype and k_cache.device == dev and v_cache.device == dev):
+    try:
+        dev, cs = q.device, k_cache.stride()
+        if not (q.is_cuda and q.dim() == 3 and q.is_contiguous() and q.dtype in _QUERY_TYPES and len(cs) == 4
+                and v_cache.stride() == cs and cs[3] == 1 and v_cache.shape == k_cache.shape
+                and v_cache.dtype is k_cache.dtype and k_cache.device == dev and v_cache.device == dev):
+            return False
+        B, H, D = q.shape
+        pages, page, Hkv, Dk = k_cache.shape
+        if not (D == Dk == _lib.HEAD_DIM and page == _lib.PAGE and B and H and pages and Hkv and H % Hkv == 0
+                and kv_page_indptr.numel() == B + 1 and kv_last_page_len.numel() == B
+                and fine_rows(dev, torch.int32, kv_page_indices, kv_page_indptr, kv_last_page_len)):
+            return False
+        if k_scale is None:
+            return v_scale is None and k_cache.dtype is q.dtype
+        return (v_scale is not None and k_cache.dtype in KV_FORMATS and k_scale.dtype is torch.float32
+                and v_scale.dtype is torch.float32 and k_scale.shape == k_cache.shape[:3]
+                and v_scale.shape == k_scale.shape and k_scale.stride() == v_scale.stride()
+                and k_scale.device == dev and v_scale.device == dev)
+    except AttributeError:                    # no tensor
         return False
-    B, H, D = q.shape
-    pages, page, Hkv, Dk = k_cache.shape
-    if not (D == Dk == _lib.HEAD_DIM and page == _lib.PAGE and B and H and pages and Hkv and H % Hkv == 0
-            and kv_page_indptr.numel() == B + 1 and kv_last_page_len.numel() == B
-            and fine_rows(dev, torch.int32, kv_page_indices, kv_page_indptr, kv_last_page_len)):
-        return False
-    if k_scale is None:
-        return v_scale is None and k_cache.dtype is q.dtype
-    return (v_scale is not None and k_cache.dtype in KV_FORMATS and k_scale.dtype is torch.float32
-            and v_scale.dtype is torch.float32 and k_scale.shape == k_cache.shape[:3]
-            and v_scale.shape == k_scale.shape and k_scale.stride() == v_scale.stride()
-            and k_scale.device == dev and v_scale.device == dev)
 
 
 def _check(q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len) -> None:
@@ -176,6 +179,11 @@ def prefix_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     operands = (q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len)
     if not _fine(*operands):
         _check(*operands)
+    tables = (("group_indptr", group_indptr), ("prefix_page_indices", prefix_page_indices),
+              ("prefix_page_indptr", prefix_page_indptr), ("prefix_last_page_len", prefix_last_page_len))
+    for name, t in tables:
+        if not isinstance(t, torch.Tensor):
+            check_cuda(t, name)
     groups, batch = group_indptr.numel() - 1, q.size(0)
     if not (1 <= groups <= batch and prefix_page_indptr.numel() == groups + 1
             and prefix_last_page_len.numel() == groups

@@ -61,15 +61,18 @@ def _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_las
 
 def _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len) -> bool:
     """Whether a cache and its tables are plainly right; if not, the checks above find out what is wrong."""
-    dev, cs, batch = k_cache.device, k_cache.stride(), token_indptr.numel() - 1
-    return (k_cache.is_cuda and len(cs) == 4 and cs[3] == 1 and k_cache.size(1) == _lib.PAGE
-            and k_cache.size(3) == _lib.HEAD_DIM and k_cache.dtype in KV_FORMATS and v_cache.dtype is k_cache.dtype
-            and v_cache.stride() == cs and v_cache.shape == k_cache.shape and v_cache.device == dev
-            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
-            and k_scale.shape == k_cache.shape[:3] and v_scale.shape == k_scale.shape
-            and k_scale.stride() == v_scale.stride() and k_scale.device == dev and v_scale.device == dev
-            and batch >= 1 and kv_page_indptr.numel() == batch + 1 and kv_last_page_len.numel() == batch
-            and fine_rows(dev, torch.int32, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len))
+    try:
+        dev, cs, batch = k_cache.device, k_cache.stride(), token_indptr.numel() - 1
+        return (k_cache.is_cuda and len(cs) == 4 and cs[3] == 1 and k_cache.size(1) == _lib.PAGE
+                and k_cache.size(3) == _lib.HEAD_DIM and k_cache.dtype in KV_FORMATS and v_cache.dtype is k_cache.dtype
+                and v_cache.stride() == cs and v_cache.shape == k_cache.shape and v_cache.device == dev
+                and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+                and k_scale.shape == k_cache.shape[:3] and v_scale.shape == k_scale.shape
+                and k_scale.stride() == v_scale.stride() and k_scale.device == dev and v_scale.device == dev
+                and batch >= 1 and kv_page_indptr.numel() == batch + 1 and kv_last_page_len.numel() == batch
+                and fine_rows(dev, torch.int32, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len))
+    except AttributeError:                    # no tensor
+        return False
 
 
 def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torch.Tensor,
@@ -89,6 +92,9 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
     if not _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len):
         check_quant_cache(k_cache, v_cache, k_scale, v_scale)
         _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
+    for name, t in (("k_new", k_new), ("v_new", v_new)):
+        if not isinstance(t, torch.Tensor):
+            check_cuda(t, name)
     dev, Hkv, ns = k_cache.device, k_cache.size(2), k_new.stride()
     if not (k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and len(ns) == 3 and ns[2] == 1 and k_new.dtype in _ROW_TYPES
             and v_new.shape == k_new.shape and v_new.stride() == ns and v_new.dtype is k_new.dtype

@@ -237,7 +237,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     if vocab > 1 and logits.stride(1) != 1:
         raise RuntimeError("logits must be contiguous along the vocabulary")
     code, dev = dtype_code(logits.dtype, "logits"), logits.device
-    if u.numel() != rows or not fine_rows(dev, torch.float32, u):
+    if not isinstance(u, torch.Tensor) or u.numel() != rows or not fine_rows(dev, torch.float32, u):
         check_input(u, "u"); check_dtype(u, torch.float32, "u"); check_same_device(logits, ("u", u))
         raise RuntimeError(f"u must have one element per row ({rows})")
     f32 = torch.float32
