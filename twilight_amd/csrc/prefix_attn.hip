@@ -68,7 +68,7 @@ struct PrefixAttnArgs {
   uint32_t max_prefix, max_group, max_tokens;
   uint32_t p_chunk, p_chunks, p_tiles;      // prefix: tokens per part, parts, row tiles per group
   uint32_t chunk, chunks, tiles;            // own tokens: the same
-  uint32_t p_blocks;                        // workgroups of the prefix parts, first in the grid
+  uint32_t own_blocks;                      // workgroups of the own parts, first in the grid
   float scale_log2;
   float* acc;                               // [rows, parts, 128]
   f32x2* ml;                                // [rows, parts]
@@ -736,15 +736,19 @@ struct ModeLds<kStaged> { using type = StagedLds; };
 constexpr size_t larger(size_t x, size_t y) { return x > y ? x : y; }
 constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStream32 ? 32 : kStRows; }
 
-// Grid: the prefix parts (eight of (kv head, part, group), row tile, the next eight, ...: the row tiles
-// of a part run side by side on one XCD and find its K and V in that L2), then the own parts (kv head,
-// request, row tile, part: the parts that only long requests have come last).
+// Grid: the own parts (kv head, request, row tile, part: the parts that only long requests have come last),
+// then the prefix parts (eight of (kv head, part, group), row tile, the next eight, ...: the row tiles of a
+// part run side by side on one XCD and find its K and V in that L2). Own parts wait for memory where
+// prefix parts compute, so each compute unit's first prefix part overlaps with its last own ones (64 samples
+// of a 32768-token prompt, up to 4000 tokens of their own: 202 us with the prefix first, 183 so; 4 samples
+// of 16384, up to 1000: 40 and 35.5; 20 of 16384, up to 100: 32 and 30).
 template <int QT, int KV, int MODE>
 __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnArgs a) {
   __shared__ __align__(16) uint8_t pool[larger(sizeof(typename ModeLds<MODE>::type), sizeof(PartLds<1>))];
   const uint32_t parts = a.p_chunks + a.chunks;
   uint32_t id = blockIdx.x;
-  if (id < a.p_blocks) {
+  if (id >= a.own_blocks) {
+    id -= a.own_blocks;
     const uint32_t tile = (id >> 3) % a.p_tiles;
     id = (id >> 3) / a.p_tiles * 8 + (id & 7);
     const uint32_t kvh = id % a.num_kv_heads;
@@ -770,12 +774,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnAr
     else
       attend_part<QT, KV, MODE == kStream16 ? 1 : 2>(a, ids, num_ids, begin, end, kvh, row_of, c, parts, pool);
   } else {
-    id -= a.p_blocks;
     const uint32_t kvh = id % a.num_kv_heads;
     id /= a.num_kv_heads;
     const uint32_t b = id % a.batch;
     id /= a.batch;
     const uint32_t tile = id % a.tiles, c = id / a.tiles;
+    if (c >= a.chunks) return;              // the last eight may be short
     const int row0 = (int)(tile * 16);
     const int len = list_len(a.ptr, a.last, b, a.max_tokens);
     const int begin = (int)(c * a.chunk), end = min(len, begin + (int)a.chunk);
@@ -881,11 +885,14 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
              &p.p_chunks);
   // Own tokens: about two workgroups per compute unit (at 32k tokens, 8 requests, 8 kv heads: 512 of them
   // 98 us, 1024 106, 2048 105; a workgroup's start and end cost what it does not stream), but where the
-  // requests alone are that many, parts of 2048 tokens at most, since their lengths may differ (16
-  // requests of up to 8191 tokens, 32 kv heads: 144 -> 121 us). Up to 1024 tokens are one part: the
-  // merge is a launch of its own (1000 tokens: 20.6 -> 17.9 us).
-  const uint64_t lists = max_tokens <= 1024 ? 512 : (uint64_t)num_kv_heads * batch * p.tiles;
-  cut_tokens(max_tokens, lists, 512, lists < 256 ? 1u << 24 : 2048, &p.chunk, &p.chunks);
+  // requests alone are half of that, parts of 2048 tokens at most, since their lengths may differ (16
+  // requests of up to 8191 tokens, 32 kv heads: 144 -> 121 us). Without a prefix, up to 1024 tokens are
+  // one part: the merge is a launch of its own (1000 tokens: 20.6 -> 17.9 us). Beside prefix parts it runs
+  // in any case and few requests are cut like longer ones (4 samples of 16384 tokens, up to 1000 of their
+  // own: 35.5 -> 27 us), but 256 lists fill the chip as they are (264 of up to 300: 50.5 -> 47.5).
+  const uint64_t lists = (uint64_t)num_kv_heads * batch * p.tiles;
+  const bool whole = p.p_chunks ? lists >= 256 : max_tokens <= 1024;
+  cut_tokens(max_tokens, whole ? 512 : lists, 512, lists < 256 ? 1u << 24 : 2048, &p.chunk, &p.chunks);
   return p;
 }
 
@@ -954,7 +961,8 @@ extern "C" int twl_prefix_attn(
   if (need && !workspace) return TWL_ENULL;
   if (workspace_bytes < need) return TWL_EINVAL;
   const uint64_t p_blocks = ((uint64_t)num_kv_heads * p.p_chunks * groups + 7) / 8 * 8 * p.p_tiles;
-  const uint64_t blocks = p_blocks + (uint64_t)num_kv_heads * p.chunks * batch * p.tiles;
+  const uint64_t own_blocks = ((uint64_t)num_kv_heads * p.chunks * batch * p.tiles + 7) / 8 * 8;
+  const uint64_t blocks = p_blocks + own_blocks;
   if (blocks > 0xFFFFFFull) return TWL_EINVAL;   // 2^32 threads
   const uint64_t parts = (uint64_t)p.p_chunks + p.chunks, rows = (uint64_t)batch * num_q_heads;
   twl::PrefixAttnArgs a{};
@@ -973,7 +981,7 @@ extern "C" int twl_prefix_attn(
   a.G = num_q_heads / num_kv_heads; a.groups = groups; a.max_prefix = max_prefix_tokens;
   a.max_group = max_group_size; a.max_tokens = max_tokens; a.p_chunk = p.p_chunk;
   a.p_chunks = p.p_chunks; a.p_tiles = p.p_tiles; a.chunk = p.chunk; a.chunks = p.chunks;
-  a.tiles = p.tiles; a.p_blocks = (uint32_t)p_blocks;
+  a.tiles = p.tiles; a.own_blocks = (uint32_t)own_blocks;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.acc = (float*)workspace;
   a.ml = (twl::f32x2*)((float*)workspace + rows * parts * TWL_HEAD_DIM);
