@@ -38,8 +38,7 @@ constexpr double kSmpOne = 35184372088832.0;   // 2^45: the weight 1
 constexpr int kSmpBins = 512;
 constexpr int kSmpSeg = 512;                   // tokens of one running sum: a wavefront, 8 a lane
 constexpr int kSmpStep = kSmpThreads * 8;      // tokens of one pass of a workgroup
-constexpr int kSmpPerThread = 16;
-constexpr uint32_t kSmpMaxCand = kSmpThreads * kSmpPerThread;
+constexpr uint32_t kSmpMaxCand = 8192;
 
 struct SampleArgs {
   const void* logits;
@@ -408,11 +407,20 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
     __syncthreads();
     double v = 0.0;
     const uint64_t* const bins = a.hist + (size_t)row * a.slices * kSmpBins;
-#pragma unroll 8
-    for (uint32_t s = 0; s < a.slices; ++s) {
-      const int mine = (int)threadIdx.x - slice_shift[s];
-      const uint64_t h = bins[s * kSmpBins + max(mine, 0)];
-      v += mine >= 0 ? (double)h * slice_weight[s] : 0.0;
+    // eight loads at a time; every one is used, if with weight 0, or the compiler makes branches of them
+    // that wait for one another (one row of 128256 in 32 slices: 33 us so, 27 like this)
+    for (uint32_t s0 = 0; s0 < a.slices; s0 += 8) {
+      uint64_t h[8];
+      double w[8];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t s = min(s0 + j, a.slices - 1);
+        const int mine = (int)threadIdx.x - slice_shift[s];
+        h[j] = bins[s * kSmpBins + max(mine, 0)];
+        w[j] = mine >= 0 && s0 + j < a.slices ? slice_weight[s] : 0.0;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v += (double)h[j] * w[j];
     }
     const int wave = threadIdx.x / kWave;
     const double incl = wave_scan(v);
@@ -498,11 +506,15 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
 }
 
 // ---- third launch ------------------------------------------------------------------------------
+// Sums by digit are kept in copies, one per lane of 16: equal logits are common (a bf16 logit near 4 has 16
+// of them per unit) and atomics on one address go one after another.
+constexpr int kSmpDigitBits = 7, kSmpCopies = 16, kSmpSlots = kSmpCopies << kSmpDigitBits;
 struct SampleShared {
+  uint64_t list[kSmpMaxCand];           // key, then the complement of the index: larger is better ranked
   uint64_t seg[kSmpMaxVocab / kWave];   // generic: measure of every 64 tokens; else of every kSmpSeg
-  uint64_t hist[2048];
-  uint32_t count[2048];
-  uint64_t left[kWave][2];
+  uint64_t hist[kSmpSlots];
+  uint32_t count[kSmpSlots];
+  uint64_t left[kWave][2], before[kWave];
   uint64_t wsum[kSmpWaves], wmin[kSmpWaves];
   double table[64];
   uint32_t word[2], members;
@@ -677,65 +689,80 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared& sh, uint64_t v, uin
   return off + incl - v;
 }
 
-// Among the threads' entries (those with a measure; no two alike), the entry at which the running measure,
-// from the largest entry down, first reaches `target` (>= 1, <= the total). A digit at a time of the
-// range that is in use, until at most a wavefront's worth is left, which is ranked directly.
-__device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint64_t* entry, const uint64_t* meas,
-                                                   uint32_t entries, uint64_t target) {
-  uint64_t lo = 0, hi = ~0ull, above = 0;
-  for (int digits = 0; digits < 7; ++digits) {   // a digit is 11 of 64 bits
-    uint64_t mx = 0, nmn = 0;
-#pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j)
-      if (j * kSmpThreads < entries && meas[j] && entry[j] >= lo && entry[j] <= hi) {
-        mx = max(mx, entry[j]);
-        nmn = max(nmn, ~entry[j]);
+// Among the entries of sh.list in [lo, hi] (no two alike), the one at which the running measure, from the
+// largest entry down, first reaches `target` (>= 1, <= the total). A digit at a time, of the bounds and
+// then of the range that is in use, until at most a wavefront's worth is left, which is ranked directly.
+// Expects and leaves the digits' sums, the members and their ranks cleared. Loops are not unrolled: a
+// workgroup goes through this code once, and fetching it is what takes the time (62 KB of code with the
+// entries in registers).
+template <class F>
+__device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, uint32_t entries, F meas, uint64_t target,
+                                                   uint64_t lo, uint64_t hi) {
+  uint64_t above = 0;
+#pragma unroll 1
+  for (int digits = 0; digits < 11; ++digits) {   // a digit is 7 of 64 bits, the first one of the bounds
+    if (digits > 0) {
+      uint64_t mx = 0, nmn = 0;
+#pragma unroll 1
+      for (uint32_t i = threadIdx.x; i < entries; i += kSmpThreads) {
+        const uint64_t e = sh.list[i];
+        if (e >= lo && e <= hi) {
+          mx = max(mx, e);
+          nmn = max(nmn, ~e);
+        }
       }
-    mx = wave_max(mx);
-    nmn = wave_max(nmn);
-    if (lane_id() == 0) {
-      sh.wsum[threadIdx.x / kWave] = mx;
-      sh.wmin[threadIdx.x / kWave] = nmn;
-    }
-    for (int i = threadIdx.x; i < 2048; i += kSmpThreads) {
-      sh.hist[i] = 0;
-      sh.count[i] = 0;
-    }
-    if (threadIdx.x == 0) sh.members = 0;
-    __syncthreads();
-    hi = 0;
-    lo = 0;
-#pragma unroll
-    for (int w = 0; w < kSmpWaves; ++w) {
-      hi = max(hi, sh.wsum[w]);
-      lo = max(lo, sh.wmin[w]);
-    }
-    lo = ~lo;
-    if (lo >= hi) {
+      mx = wave_max(mx);
+      nmn = wave_max(nmn);
+      if (lane_id() == 0) {
+        sh.wsum[threadIdx.x / kWave] = mx;
+        sh.wmin[threadIdx.x / kWave] = nmn;
+      }
       __syncthreads();
-      return hi;
-    }
-    const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 11);
+      hi = 0;
+      lo = 0;
 #pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j)
-      if (j * kSmpThreads < entries && meas[j] && entry[j] >= lo && entry[j] <= hi) {
-        const uint32_t digit = (uint32_t)((hi - entry[j]) >> shift);
-        atomicAdd((unsigned long long*)&sh.hist[digit], (unsigned long long)meas[j]);
-        atomicAdd(&sh.count[digit], 1u);
+      for (int w = 0; w < kSmpWaves; ++w) {
+        hi = max(hi, sh.wsum[w]);
+        lo = max(lo, sh.wmin[w]);
       }
+      lo = ~lo;
+      if (lo >= hi) {
+        __syncthreads();
+        return hi;
+      }
+    }
+    const int shift = max(0, 64 - __builtin_clzll(hi - lo) - kSmpDigitBits);
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < entries; i += kSmpThreads) {
+      const uint64_t e = sh.list[i];
+      if (e >= lo && e <= hi) {
+        const uint32_t at = (uint32_t)((hi - e) >> shift) * kSmpCopies + lane_id() % kSmpCopies;
+        atomicAdd((unsigned long long*)&sh.hist[at], (unsigned long long)meas(e));
+        atomicAdd(&sh.count[at], 1u);
+      }
+    }
     __syncthreads();
-    uint64_t m[4], s = 0, total;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s += m[j] = sh.hist[4 * threadIdx.x + j];
-    uint64_t run = block_scan(sh, s, total) + above;
+    // a digit's copies are read by four neighbouring lanes
+    static_assert(kSmpSlots == 4 * kSmpThreads && kSmpCopies == 16, "four slots a thread, four threads a digit");
+    uint64_t s = 0, total;
+    uint32_t c = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (run < target && run + m[j] >= target) {
-        sh.word[0] = 4 * threadIdx.x + j;
-        sh.word[1] = sh.count[4 * threadIdx.x + j];
-        sh.wide[0] = run;
-      }
-      run += m[j];
+      s += sh.hist[4 * threadIdx.x + j];
+      c += sh.count[4 * threadIdx.x + j];
+      sh.hist[4 * threadIdx.x + j] = 0;
+      sh.count[4 * threadIdx.x + j] = 0;
+    }
+    s += dpp64<kDppXor1, 0xF>(s);
+    s += dpp64<kDppXor2, 0xF>(s);
+    c += (uint32_t)dpp<kDppXor1>(0, (int)c);
+    c += (uint32_t)dpp<kDppXor2>(0, (int)c);
+    const bool lead = threadIdx.x % 4 == 0;
+    const uint64_t run = block_scan(sh, lead ? s : 0, total) + above;
+    if (lead && run < target && run + s >= target) {
+      sh.word[0] = threadIdx.x / 4;
+      sh.word[1] = c;
+      sh.wide[0] = run;
     }
     __syncthreads();
     const uint64_t digit = sh.word[0];
@@ -746,20 +773,35 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, const uint6
     const uint64_t least = hi > width ? hi - width : 0;   // one type on both sides of max, or it is the double's
     lo = max(lo, least);
     if (n <= kWave) {
-#pragma unroll
-      for (int j = 0; j < kSmpPerThread; ++j)
-        if (j * kSmpThreads < entries && meas[j] && entry[j] >= lo && entry[j] <= hi) {
+#pragma unroll 1
+      for (uint32_t i = threadIdx.x; i < entries; i += kSmpThreads) {
+        const uint64_t e = sh.list[i];
+        if (e >= lo && e <= hi) {
           const uint32_t at = atomicAdd(&sh.members, 1u);
-          sh.left[at][0] = entry[j];
-          sh.left[at][1] = meas[j];
+          sh.left[at][0] = e;
+          sh.left[at][1] = meas(e);
         }
+      }
+      __syncthreads();
+      // the measure in front of every member, an eighth of the members per wavefront
+      const uint32_t member = threadIdx.x % kWave, first = threadIdx.x / kWave * (kWave / kSmpWaves);
+      if (member < n) {
+        const uint64_t mine = sh.left[member][0];
+        uint64_t before = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kWave / kSmpWaves; ++i) {
+          const uint64_t e = sh.left[first + i][0], w = sh.left[first + i][1];
+          before += first + i < n && e > mine ? w : 0;
+        }
+        if (before) atomicAdd((unsigned long long*)&sh.before[member], (unsigned long long)before);
+      }
       __syncthreads();
       if (threadIdx.x < n) {
-        const uint64_t mine = sh.left[threadIdx.x][0];
-        uint64_t before = above;
-        for (uint32_t i = 0; i < n; ++i) before += sh.left[i][0] > mine ? sh.left[i][1] : 0;
-        if (before < target && before + sh.left[threadIdx.x][1] >= target) sh.wide[1] = mine;
+        const uint64_t before = above + sh.before[threadIdx.x];
+        sh.before[threadIdx.x] = 0;
+        if (before < target && before + sh.left[threadIdx.x][1] >= target) sh.wide[1] = sh.left[threadIdx.x][0];
       }
+      if (threadIdx.x == 0) sh.members = 0;
       __syncthreads();
       const uint64_t got = sh.wide[1];
       __syncthreads();
@@ -779,11 +821,17 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
   const uint32_t n = a.cand_count[row];
   const SampleCut c = a.cut[row];
   uint64_t seg = threadIdx.x < segs ? a.seg[(size_t)row * segs + threadIdx.x] : 0;
-  uint64_t entry[kSmpPerThread];          // key, then the complement of the index: larger is better ranked
-  entry[0] = threadIdx.x < a.cand_stride ? a.cand[(size_t)row * a.cand_stride + threadIdx.x] : 0;
+  const uint64_t* const cand = a.cand + (size_t)row * a.cand_stride;
+  const uint64_t first = threadIdx.x < a.cand_stride ? cand[threadIdx.x] : 0;
   const float u = a.u[row];
   const RowFilter f = row_filter(a, row);
   fill_table(sh.table);
+  for (int i = threadIdx.x; i < kSmpSlots; i += kSmpThreads) {
+    sh.hist[i] = 0;
+    sh.count[i] = 0;
+  }
+  if (threadIdx.x < kWave) sh.before[threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.members = 0;
   best = wave_max(best);
   const uint32_t top_key = (uint32_t)(best >> 32);
   if (f.greedy || top_key <= kKeyNone) {
@@ -802,49 +850,48 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
     if (threadIdx.x == 0) a.tokens[row] = token;
     return;
   }
-  uint64_t mass[kSmpPerThread];
-#pragma unroll
-  for (int j = 0; j < kSmpPerThread; ++j) {
-    const uint32_t i = j * kSmpThreads + threadIdx.x;
-    if (i >= n) entry[j] = 0;
-    else if (j > 0) entry[j] = a.cand[(size_t)row * a.cand_stride + i];
-  }
-#pragma unroll
-  for (int j = 0; j < kSmpPerThread; ++j)
-    mass[j] = j * kSmpThreads < n && entry[j] ? wt.mass(key_value((uint32_t)(entry[j] >> 32))) : 0;
-  // candidates from `cut` up are kept
-  uint64_t cut = 0;
-  if (f.by_rank && (uint32_t)f.k < n) {
-    uint64_t one[kSmpPerThread];
-#pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j) one[j] = entry[j] ? 1 : 0;
-    cut = entry_reaching(sh, entry, one, n, (uint64_t)f.k);
-#pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j) mass[j] = entry[j] < cut ? 0 : mass[j];
-  }
-  if (f.p < 1.0 && n > 0) {
-    uint64_t mine = 0, total;
-#pragma unroll
-    for (int j = 0; j < kSmpPerThread; ++j) mine += mass[j];
-    block_scan(sh, mine, total);
-    const double goal = f.by_rank ? f.p * (double)total : c.goal - c.before;
-    const uint64_t target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
-    if (target <= total) cut = max(cut, entry_reaching(sh, entry, mass, n, target));
-  }
-  // ---- sums over kSmpSeg tokens, and the draw -------------------------------------------------
+  sh.list[threadIdx.x] = first;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x + kSmpThreads; i < n; i += kSmpThreads) sh.list[i] = cand[i];
   if (threadIdx.x < segs) sh.seg[threadIdx.x] = f.by_rank ? 0 : seg;
   __syncthreads();
+  auto mass_of = [&](uint64_t e) { return wt.mass(key_value((uint32_t)(e >> 32))); };
+  // candidates from `cut` up are kept. All of them lie between the edges of the cut's bin, or (top-k) up to
+  // the best
+  const uint64_t least = (uint64_t)key_of(c.cand) << 32;
+  const uint64_t most = c.keep == c.keep ? ((uint64_t)key_of(c.keep) << 32) - 1 : ((uint64_t)top_key << 32) | 0xFFFFFFFFu;
+  uint64_t cut = 0;
+#pragma unroll 1
+  for (int by_mass = 0; by_mass < 2; ++by_mass) {
+    uint64_t target = (uint64_t)f.k;
+    if (by_mass) {
+      if (!(f.p < 1.0) || n == 0) break;
+      uint64_t mine = 0, total;
+#pragma unroll 1
+      for (uint32_t i = threadIdx.x; i < n; i += kSmpThreads) mine += sh.list[i] >= cut ? mass_of(sh.list[i]) : 0;
+      block_scan(sh, mine, total);
+      const double goal = f.by_rank ? f.p * (double)total : c.goal - c.before;
+      target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
+      if (target > total) break;
+    } else if (!f.by_rank || (uint32_t)f.k >= n) {
+      continue;
+    }
+    const uint64_t reached = entry_reaching(sh, n, [&](uint64_t e) { return by_mass ? mass_of(e) : 1ull; }, target,
+                                            max(cut, least), most);
+    cut = max(cut, reached);
+  }
+  // ---- sums over kSmpSeg tokens, and the draw -------------------------------------------------
   const double min_w = f.min_p > 0.0 ? f.min_p * kSmpOne : -1.0;
   auto passes = [&](uint32_t k, double w) { return k == top_key || w >= min_w; };
-#pragma unroll
-  for (int j = 0; j < kSmpPerThread; ++j)
-    if (j * kSmpThreads < n && entry[j] && entry[j] >= cut) {
-      const uint32_t k = (uint32_t)(entry[j] >> 32);
-      const double w = wt.weight(key_value(k));
-      if (passes(k, w))
-        atomicAdd((unsigned long long*)&sh.seg[(0xFFFFFFFFu - (uint32_t)entry[j]) / kSmpSeg],
-                  (unsigned long long)Weigher::fixed(w));
-    }
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x; i < n; i += kSmpThreads) {
+    const uint64_t e = sh.list[i];
+    const uint32_t k = (uint32_t)(e >> 32);
+    const double w = wt.weight(key_value(k));
+    if (e >= cut && passes(k, w))
+      atomicAdd((unsigned long long*)&sh.seg[(0xFFFFFFFFu - (uint32_t)e) / kSmpSeg],
+                (unsigned long long)Weigher::fixed(w));
+  }
   __syncthreads();
   seg = threadIdx.x < segs ? sh.seg[threadIdx.x] : 0;
   uint64_t total;
@@ -883,12 +930,17 @@ struct SamplePlan {
   uint32_t slices, iters;
   uint64_t best, hist, seg, cand, cut, count, bytes;   // offsets into the workspace
 };
-// Slices of 4096, 8192 or 16384 tokens: as large as leaves about two workgroups per compute unit.
+// Slices of 4096, 8192 or 16384 tokens: as large as leaves a workgroup per compute unit, or two where a row
+// has few slices. Every slice reads the bins of all the row's slices, which is what many of them cost (63
+// rows of 128256: 504 workgroups of 8 slices a row 49 us, 1008 of 16 55; 24 rows: 38 and 48; but 128 rows of
+// 32000: 256 workgroups of 2 slices a row 37 us, 512 of 4 35).
 static SamplePlan sample_plan(uint32_t rows, uint32_t vocab) {
   SamplePlan p{};
-  p.iters = 4;
-  while (p.iters > 1 && (uint64_t)rows * ((vocab + p.iters * kSmpStep - 1) / (p.iters * kSmpStep)) < 512) p.iters >>= 1;
-  p.slices = (vocab + p.iters * kSmpStep - 1) / (p.iters * kSmpStep);
+  for (p.iters = 4;; p.iters >>= 1) {
+    p.slices = (vocab + p.iters * kSmpStep - 1) / (p.iters * kSmpStep);
+    const uint64_t groups = (uint64_t)rows * p.slices;
+    if (p.iters == 1 || groups >= 512 || (groups >= 256 && p.slices >= 4)) break;
+  }
   const uint64_t r = rows, segs = (vocab + kSmpSeg - 1) / kSmpSeg;
   p.best = 0;
   p.hist = p.best + r * p.slices * 8;
