@@ -13,6 +13,10 @@
 // and a call can be repeated. 16 lanes share a row (8 channels a lane: one 16-byte load, one
 // 8-byte store) and find its request with a 16-way search, so up to 16 requests cost one load
 // round trip and 256 cost two.
+//
+// Bound by memory: 32768 bf16 tokens of 32 heads, 814 MB either way, are written in 165 us (4.9 TB/s) and read
+// in 175 (4.6), where a large copy reaches 5.2 TB/s. A decode step of 8 requests and 8 heads is a chain of
+// loads and takes 3.4 us to write, 2.8 to read.
 #include "twl_common.h"
 
 namespace twl {
@@ -259,7 +263,8 @@ int kv_quant_args(KvQuantArgs& a, uint8_t* k_cache, uint8_t* v_cache, int format
 }
 
 // Heads per row of 16 lanes, and the grid: four where that leaves two full loads of the chip (2 x 256
-// compute units x 8 workgroups of 16 rows).
+// compute units x 8 workgroups of 16 rows). One head and four, to write and to read: 32768 tokens of 32 heads
+// 189 and 224 us, 166 and 176; 32768 of 8 heads 56 and 42, 51 and 36; 4096 of 8 heads 10.6 and 7.8, 10.8 and 7.5.
 static bool quant_grid(const KvQuantArgs& a, dim3& grid) {
   const uint64_t four = ((uint64_t)a.tokens * ((a.num_kv_heads + 3) / 4) + 15) / 16;
   const bool bulk = a.num_kv_heads >= 4 && four >= 4096;
