@@ -8,7 +8,7 @@
 // with the queries of all its requests as the columns of one matrix product, and the requests' own
 // tokens are ordinary parts beside it.
 //
-// One wavefront works on tiles of 32 tokens (two pages) and NQ sets of 16 query rows, without LDS
+// One wavefront works on tiles of 32 tokens (two pages) and 16 query rows, without LDS
 // and without moving anything between lanes. With n = lane % 16, kb = lane / 16:
 //   S^T = K Q^T   A operand: token n of a page, 8 channels per lane; B operand: query n. A lane of
 //                 the result holds query n's logits of tokens 4 kb + i of either page.
@@ -210,41 +210,32 @@ __device__ __forceinline__ void put_row(const PrefixAttnArgs& a, int row, uint32
 }
 
 // What the wavefronts of a workgroup exchange at the end of a part.
-template <int NQ>
 struct PartLds {
-  float o[kPaWaves][16 * NQ][TWL_HEAD_DIM + 4];
-  float m[kPaWaves][16 * NQ], l[kPaWaves][16 * NQ], top[16 * NQ], total[16 * NQ];
+  float o[kPaWaves][16][TWL_HEAD_DIM + 4];
+  float m[kPaWaves][16], l[kPaWaves][16], top[16], total[16];
 };
 
 // One workgroup's part: tokens [begin, end) of a page list (first id at `ids`, `num_ids` of them)
-// for kv head kvh, and 16 * NQ query rows; the four wavefronts take every fourth tile each.
+// for kv head kvh, and 16 query rows; the four wavefronts take every fourth tile each.
 // row_of(local row) -> row of q / out, or -1.
-template <int QT, int KV, int NQ, class RowOf>
+template <int QT, int KV, class RowOf>
 __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32_t* ids, int num_ids,
                                             int begin, int end, uint32_t kvh, RowOf row_of,
                                             uint32_t part, uint32_t parts, uint8_t* pool) {
   constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
   constexpr int MT = k8 ? TWL_F16 : QT;
-  constexpr int ROWS = 16 * NQ;
   constexpr int NKL = k8 ? 2 : 4;           // 16-byte loads of K per lane and page
   const int lane = lane_id(), n = lane & 15, kb = lane >> 4;
   const int wave = threadIdx.x / kWave;
 
-  u32x4 qf[NQ][4];
-  float row_scale[NQ];
-#pragma unroll
-  for (int x = 0; x < NQ; ++x)
-    load_query<QT, k8, k8>(a, row_of(x * 16 + n), kb, qf[x], row_scale[x]);
+  u32x4 qf[4];
+  float row_scale;
+  load_query<QT, k8, k8>(a, row_of(n), kb, qf, row_scale);
 
-  f32x4 o[NQ][8];
-  float m[NQ], l[NQ];
+  f32x4 o[8];
+  float m = kPaNoMax, l = 0.0f;
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    m[x] = kPaNoMax;
-    l[x] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[x][j] = f32x4{0, 0, 0, 0};
-  }
+  for (int j = 0; j < 8; ++j) o[j] = f32x4{0, 0, 0, 0};
   int vexp = -126;                          // V scales so far are below 2^(vexp + 1)
 
   const uint8_t* const kbase = a.k + kvh * a.head_bytes;
@@ -317,11 +308,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
     }
 
     // ---- logits --------------------------------------------------------------------------------
-    f32x4 s[NQ][2];
-#pragma unroll
-    for (int x = 0; x < NQ; ++x)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) s[x][p] = f32x4{0, 0, 0, 0};
+    f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -334,8 +321,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         } else {
           kf = raw.k[p][j];
         }
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) s[x][p] = mfma16<MT>(kf, qf[x][j], s[x][p]);
+        s[p] = mfma16<MT>(kf, qf[j], s[p]);
       }
 
     if (cut) {
@@ -368,41 +354,38 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
       for (int i = 0; i < 8; ++i) vs[i >> 2][i & 3] *= down;
     }
 
-    u32x4 pf[NQ];
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float z = k8 ? s[x][i >> 2][i & 3] * ks[i >> 2][i & 3] : s[x][i >> 2][i & 3];
-        if (cut) z = tok0 + 16 * (i >> 2) + 4 * kb + (i & 3) < end ? z : -__builtin_inff();
-        s[x][i >> 2][i & 3] = z;
-        top = fmaxf(top, z);
-      }
-      top *= row_scale[x];
-      if (__any(top > m[x] + kPaSlack)) {
-        const float up = fmaxf(m[x], max_over_kb(top));
-        const float alpha = __builtin_amdgcn_exp2f(m[x] - up);
-        m[x] = up;
-        l[x] *= alpha;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[x][j] *= alpha;
-      }
-      if (k8 && rise > 0) {
-        const float alpha = rise > 126 ? 0.0f : as_f32((127 - rise) << 23);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[x][j] *= alpha;
-      }
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(fmaf(s[x][i >> 2][i & 3], row_scale[x], -m[x]));
-        l[x] += w[i];
-        if (k8) w[i] *= vs[i >> 2][i & 3];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pf[x][i] = pack2<MT>(w[2 * i], w[2 * i + 1]);
+    for (int i = 0; i < 8; ++i) {
+      float z = k8 ? s[i >> 2][i & 3] * ks[i >> 2][i & 3] : s[i >> 2][i & 3];
+      if (cut) z = tok0 + 16 * (i >> 2) + 4 * kb + (i & 3) < end ? z : -__builtin_inff();
+      s[i >> 2][i & 3] = z;
+      top = fmaxf(top, z);
     }
+    top *= row_scale;
+    if (__any(top > m + kPaSlack)) {
+      const float up = fmaxf(m, max_over_kb(top));
+      const float alpha = __builtin_amdgcn_exp2f(m - up);
+      m = up;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] *= alpha;
+    }
+    if (k8 && rise > 0) {
+      const float alpha = rise > 126 ? 0.0f : as_f32((127 - rise) << 23);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] *= alpha;
+    }
+    float w[8];
+    u32x4 pf;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], row_scale, -m));
+      l += w[i];
+      if (k8) w[i] *= vs[i >> 2][i & 3];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pf[i] = pack2<MT>(w[2 * i], w[2 * i + 1]);
 
     // ---- O^T += V^T P^T ------------------------------------------------------------------------
     if (k8) {
@@ -425,8 +408,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         for (int j = 0; j < 4; ++j) {
           const u32x2 lo = widen4<KV>(by_ch[0][j]), hi = widen4<KV>(by_ch[1][j]);
           const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-          for (int x = 0; x < NQ; ++x) o[x][4 * c + j] = mfma16<MT>(vf, pf[x], o[x][4 * c + j]);
+          o[4 * c + j] = mfma16<MT>(vf, pf, o[4 * c + j]);
         }
       }
     } else {
@@ -438,11 +420,8 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
           lo[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c], vr[2 * i][c], 0x05040100u);
           hi[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c], vr[2 * i][c], 0x07060302u);
         }
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-          o[x][2 * c] = mfma16<MT>(lo, pf[x], o[x][2 * c]);
-          o[x][2 * c + 1] = mfma16<MT>(hi, pf[x], o[x][2 * c + 1]);
-        }
+        o[2 * c] = mfma16<MT>(lo, pf, o[2 * c]);
+        o[2 * c + 1] = mfma16<MT>(hi, pf, o[2 * c + 1]);
       }
     }
   };
@@ -459,49 +438,32 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 
   // ---- join the wavefronts that share rows, and leave the part --------------------------------
   const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
-  auto& lds = *(PartLds<NQ>*)pool;
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    l[x] = sum_over_kb(l[x]);
-    if (kb == 0) {
-      lds.m[wave][16 * x + n] = m[x];
-      lds.l[wave][16 * x + n] = l[x];
-    }
+  auto& lds = *(PartLds*)pool;
+  l = sum_over_kb(l);
+  if (kb == 0) {
+    lds.m[wave][n] = m;
+    lds.l[wave][n] = l;
   }
   __syncthreads();
-  float top[NQ], total[NQ];
+  float top = kPaNoMax, total = 0.0f;
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    top[x] = kPaNoMax;
+  for (int w = 0; w < kPaWaves; ++w) top = fmaxf(top, lds.m[w][n]);
 #pragma unroll
-    for (int w = 0; w < kPaWaves; ++w) top[x] = fmaxf(top[x], lds.m[w][16 * x + n]);
-    total[x] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kPaWaves; ++w)
-      total[x] += lds.l[w][16 * x + n] * __builtin_amdgcn_exp2f(lds.m[w][16 * x + n] - top[x]);
-    const float f = __builtin_amdgcn_exp2f(m[x] - top[x]) * vfac;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[x][j] *= f;
-  }
+  for (int w = 0; w < kPaWaves; ++w) total += lds.l[w][n] * __builtin_amdgcn_exp2f(lds.m[w][n] - top);
+  const float f = __builtin_amdgcn_exp2f(m - top) * vfac;
   // every wavefront leaves its rows; 32 threads add and write one
 #pragma unroll
-  for (int x = 0; x < NQ; ++x)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        *(f32x4*)&lds.o[wave][16 * x + n][32 * kb + 8 * i + j] =
-            f32x4{o[x][j][i], o[x][j + 1][i], o[x][j + 2][i], o[x][j + 3][i]};
+    for (int j = 0; j < 8; j += 4)
+      *(f32x4*)&lds.o[wave][n][32 * kb + 8 * i + j] = f32x4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]} * f;
   // the maxima and sums of the joined rows
   if (wave == 0 && kb == 0) {
-#pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      lds.top[16 * x + n] = top[x];
-      lds.total[16 * x + n] = total[x];
-    }
+    lds.top[n] = top;
+    lds.total[n] = total;
   }
   __syncthreads();
-  for (int r = threadIdx.x >> 5; r < ROWS; r += kPaThreads / 32) {
+  for (int r = threadIdx.x >> 5; r < 16; r += kPaThreads / 32) {
     const int row = row_of(r);
     if (row < 0) continue;
     const int c = 4 * (threadIdx.x & 31);
@@ -512,8 +474,8 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   }
 }
 
-// The same part for many rows: 128 rows per workgroup (32 per wavefront), whose wavefronts take every
-// tile of K and V from LDS. Streaming from L2 into every wavefront's registers would need
+// The same part for many rows: 64 or 128 per workgroup (NQ sets of 16 per wavefront), whose wavefronts take
+// every tile of K and V from LDS. Streaming from L2 into every wavefront's registers would need
 // 16 KB of L1 traffic per 32 tokens and 32 rows, twice what the products take.
 //
 // Products and softmax of a tile take 3 us beside 1 us of staging (a 32768-token prompt, 256 rows: 53 us).
@@ -528,7 +490,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 // product c takes channels 16 c .. 16 c + 15. A row of 256 bytes holds its 16 chunks of 16 bytes at place
 // c ^ f(row % 16), f(r) = 2 (r % 8) + r / 8: the K operand's loads (16 rows, one chunk) then touch every
 // bank once, and so do the transposing ones (four rows, two neighbouring chunks).
-constexpr int kStTile = 64, kStRows = 128;
+constexpr int kStTile = 64;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 __device__ __forceinline__ int swizzle(int row) { return (row & 7) * 2 + ((row >> 3) & 1); }
@@ -538,13 +500,12 @@ struct StagedLds {
   float ks[2][kStTile], vs[2][kStTile];
 };
 
-template <int QT, int KV, class RowOf>
+template <int QT, int KV, int NQ, class RowOf>
 __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int32_t* ids, int num_ids, int begin,
                                               int end, uint32_t kvh, int rows_here, RowOf row_of, uint32_t part,
                                               uint32_t parts, uint8_t* pool) {
   constexpr bool k8 = KV == TWL_I8 || KV == TWL_E4M3;
   constexpr int MT = k8 ? TWL_F16 : QT;
-  constexpr int NQ = 2;
   constexpr int NL = k8 ? 2 : 4;            // 16-byte loads of K (and of V) per thread and tile
   auto& lds = *(StagedLds*)pool;
   const int tx = threadIdx.x, lane = lane_id(), n = lane & 15, kb = lane >> 4, wave = tx / kWave;
@@ -737,16 +698,18 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
   }
 }
 
-// Ways to attend to a prefix part, by the rows of a kv head that share it: streaming into registers up to 32
-// rows, through LDS from there on (64 rows of a 32768-token bf16 prompt: 49 us streamed, 41 staged; 32 rows:
-// 42 and 41, of int8 35 and 38, where streaming saves the detour of the widened codes).
-enum PrefixMode { kStream16, kStream32, kStaged };
-template <int MODE>
-struct ModeLds { using type = PartLds<MODE == kStream16 ? 1 : 2>; };
-template <>
-struct ModeLds<kStaged> { using type = StagedLds; };
-constexpr size_t larger(size_t x, size_t y) { return x > y ? x : y; }
-constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStream32 ? 32 : kStRows; }
+// Ways to attend to a prefix part, by the rows of a kv head that share it (a 32768-token prompt, bf16 and int8):
+//   up to 16   streaming (16 rows: 36 and 27 us, through LDS 36 and 30)
+//   up to 64   through LDS, 16 rows a wavefront, so that none is without rows where half of 128 are (32 rows:
+//              38 and 34 us, streamed in two sets of 16 40 and 34; 48 rows: 40 and 35, with 32 rows a
+//              wavefront 42 and 42)
+//   above      through LDS, 32 rows a wavefront (96 rows: 47 and 44 us, in tiles of 64 46 and 52; 64 samples
+//              of four q heads with up to 600 tokens of their own: 84 us and 96)
+enum PrefixMode { kStream, kStaged64, kStaged128 };
+constexpr int mode_rows(int mode) { return mode == kStream ? 16 : mode == kStaged64 ? 64 : 128; }
+constexpr size_t mode_lds(int mode) {
+  return mode == kStream || sizeof(PartLds) > sizeof(StagedLds) ? sizeof(PartLds) : sizeof(StagedLds);
+}
 
 // Grid: the own parts (kv head, request, row tile, part: the parts that only long requests have come last),
 // then the prefix parts (eight of (kv head, part, group), row tile, the next eight, ...: the row tiles of a
@@ -756,7 +719,7 @@ constexpr int mode_rows(int mode) { return mode == kStream16 ? 16 : mode == kStr
 // of 16384, up to 1000: 40 and 35.5; 20 of 16384, up to 100: 32 and 30).
 template <int QT, int KV, int MODE>
 __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnArgs a) {
-  __shared__ __align__(16) uint8_t pool[larger(sizeof(typename ModeLds<MODE>::type), sizeof(PartLds<1>))];
+  __shared__ __align__(16) uint8_t pool[mode_lds(MODE)];
   const uint32_t parts = a.p_chunks + a.chunks;
   uint32_t id = blockIdx.x;
   if (id >= a.own_blocks) {
@@ -781,10 +744,11 @@ __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnAr
     };
     const int32_t* ids = a.p_ids + a.p_ptr[g];
     const int num_ids = a.p_ptr[g + 1] - a.p_ptr[g];
-    if constexpr (MODE == kStaged)
-      attend_staged<QT, KV>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts, pool);
+    if constexpr (MODE != kStream)
+      attend_staged<QT, KV, mode_rows(MODE) / 64>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts,
+                                                  pool);
     else
-      attend_part<QT, KV, MODE == kStream16 ? 1 : 2>(a, ids, num_ids, begin, end, kvh, row_of, c, parts, pool);
+      attend_part<QT, KV>(a, ids, num_ids, begin, end, kvh, row_of, c, parts, pool);
   } else {
     const uint32_t kvh = id % a.num_kv_heads;
     id /= a.num_kv_heads;
@@ -806,8 +770,8 @@ __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnAr
             put_row<QT>(a, row_of(r), 0, 1, 4 * (threadIdx.x & 31), f32x4{0, 0, 0, 0}, 0.0f, 0.0f);
       return;
     }
-    attend_part<QT, KV, 1>(a, a.ids + a.ptr[b], a.ptr[b + 1] - a.ptr[b], begin, end, kvh, row_of,
-                              a.p_chunks + c, parts, pool);
+    attend_part<QT, KV>(a, a.ids + a.ptr[b], a.ptr[b + 1] - a.ptr[b], begin, end, kvh, row_of,
+                        a.p_chunks + c, parts, pool);
   }
 }
 
@@ -891,7 +855,7 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
   PrefixPlan p{};
   const uint32_t G = num_q_heads / num_kv_heads;
   const uint64_t rows = (uint64_t)max_group * G;
-  p.mode = rows <= 16 ? kStream16 : rows <= 32 ? kStream32 : kStaged;
+  p.mode = rows <= 16 ? kStream : rows <= 64 ? kStaged64 : kStaged128;
   p.p_tiles = (uint32_t)((rows + mode_rows(p.mode) - 1) / mode_rows(p.mode));
   p.tiles = (G + 15) / 16;
   // Prefix tokens: two workgroups per compute unit, one full load of the chip
@@ -914,9 +878,9 @@ template <int QT, int KV>
 static void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& p, uint32_t blocks, hipStream_t st) {
 #define TWL_PA(MODE) \
   hipLaunchKernelGGL((prefix_attn_kernel<QT, KV, MODE>), dim3(blocks), dim3(kPaThreads), 0, st, a)
-  if (a.p_chunks == 0 || p.mode == kStream16) TWL_PA(kStream16);
-  else if (p.mode == kStream32) TWL_PA(kStream32);
-  else TWL_PA(kStaged);
+  if (a.p_chunks == 0 || p.mode == kStream) TWL_PA(kStream);
+  else if (p.mode == kStaged64) TWL_PA(kStaged64);
+  else TWL_PA(kStaged128);
 #undef TWL_PA
 }
 
