@@ -695,11 +695,11 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared& sh, uint64_t v, uin
 }
 
 // Among the entries of sh.list in [lo, hi] (no two alike), the one at which the running measure, from the
-// largest entry down, first reaches `target` (>= 1, <= the total). A digit at a time, of the bounds and
-// then of the range that is in use, until at most a wavefront's worth is left, which is ranked directly.
-// Expects and leaves the digits' sums, the members and their ranks cleared. Loops are not unrolled: a
-// workgroup goes through this code once, and fetching it is what takes the time (62 KB of code with the
-// entries in registers).
+// largest entry down, first reaches `target` (>= 1), or 0 where the total does not. A digit at a time, of
+// the bounds and then of the range that is in use, until at most a wavefront's worth is left, which is
+// ranked directly. Expects and leaves the digits' sums, the members and their ranks cleared. Loops are not
+// unrolled: a workgroup goes through this code once, and fetching it is what takes the time (with the
+// entries in registers it was 62 KB and 2 to 4 us slower).
 template <class F>
 __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, uint32_t entries, F meas, uint64_t target,
                                                    uint64_t lo, uint64_t hi) {
@@ -764,6 +764,7 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, uint32_t en
     c += (uint32_t)dpp<kDppXor2>(0, (int)c);
     const bool lead = threadIdx.x % 4 == 0;
     const uint64_t run = block_scan(sh, lead ? s : 0, total) + above;
+    if (digits == 0 && total < target) return 0;
     if (lead && run < target && run + s >= target) {
       sh.word[0] = threadIdx.x / 4;
       sh.word[1] = c;
@@ -871,13 +872,15 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
     uint64_t target = (uint64_t)f.k;
     if (by_mass) {
       if (!(f.p < 1.0) || n == 0) break;
-      uint64_t mine = 0, total;
+      double goal = c.goal - c.before;
+      if (f.by_rank) {
+        uint64_t mine = 0, total;
 #pragma unroll 1
-      for (uint32_t i = threadIdx.x; i < n; i += kSmpThreads) mine += sh.list[i] >= cut ? mass_of(sh.list[i]) : 0;
-      block_scan(sh, mine, total);
-      const double goal = f.by_rank ? f.p * (double)total : c.goal - c.before;
+        for (uint32_t i = threadIdx.x; i < n; i += kSmpThreads) mine += sh.list[i] >= cut ? mass_of(sh.list[i]) : 0;
+        block_scan(sh, mine, total);
+        goal = f.p * (double)total;
+      }
       target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
-      if (target > total) break;
     } else if (!f.by_rank || (uint32_t)f.k >= n) {
       continue;
     }
