@@ -858,7 +858,9 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
   p.mode = rows <= 16 ? kStream : rows <= 64 ? kStaged64 : kStaged128;
   p.p_tiles = (uint32_t)((rows + mode_rows(p.mode) - 1) / mode_rows(p.mode));
   p.tiles = (G + 15) / 16;
-  // Prefix tokens: two workgroups per compute unit, one full load of the chip
+  // Prefix tokens: two workgroups per compute unit, one full load of the chip (64 samples of a 32768-token bf16
+  // prompt: 256 of them 87 us, 512 73, 1024 84; 12 samples 36, 41 and 47, but 16 of int8 41 and 38, and 44
+  // int8 rows of three prompts 62, 45 and 41 where their lengths differ, 80, 54 and 59 where not)
   cut_tokens(groups ? max_prefix : 0, (uint64_t)num_kv_heads * groups * p.p_tiles, 512, 1u << 24, &p.p_chunk,
              &p.p_chunks);
   // Own tokens: about two workgroups per compute unit (at 32k tokens, 8 requests, 8 kv heads: 512 of them
