@@ -123,3 +123,45 @@ def test_shares_follow_the_weights(dev):
     at = torch.argsort(row, descending=True, stable=True)[:50]
     w[at] = torch.softmax(row[at].double(), 0)
     assert torch.all((torch.bincount(got, minlength=V).double() - n * w).abs() <= 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,V", [(520, 5003), (200, 20000), (130, 50001)])
+def test_batches_whose_slices_are_several_tiles(dev, dtype, B, V):
+    # enough rows for slices of two and four tiles of 4096 tokens, one or several slices a row; a few rows are
+    # drawn on the CPU too
+    x, u = _rows(B, V, dtype, B)
+    for t, k, p, m in ((0.8, 0, 0.9, 0.0), (1.0, 60, 0.95, 0.02), (1.5, 0, 1.0, 0.01), (0.0, 0, 1.0, 0.0)):
+        got = K.sample_tokens(x.to(dev), u.to(dev), temperature=t, top_k=k, top_p=p, min_p=m).cpu()
+        f32 = lambda v: float(torch.tensor(v))  # noqa: E731
+        for b in (0, 1, B // 2, B - 1):
+            want, margin = sample64(x[b], float(u[b]), f32(t), k, f32(p), f32(m))
+            assert margin > 1e-11, "a case too close to a border to be decided"
+            assert int(got[b]) == want
+        assert torch.equal(got, K.sample_tokens(x.to(dev), u.to(dev), temperature=t, top_k=k, top_p=p, min_p=m).cpu())
+
+
+def test_many_equal_candidates_at_the_cut(dev):
+    # bf16 rows whose cut falls among thousands of equal logits: the cut is found by index, and above 8192 of
+    # them over the whole row
+    for V, same in ((30000, 3000), (30000, 8000), (60000, 20000)):
+        g = torch.Generator().manual_seed(same)
+        x = torch.full((3, V), -30.0)
+        at = torch.randperm(V, generator=g)[:same].sort().values
+        x[:, at] = 1.0
+        x[:, at[5]] = 2.0
+        x = x.to(torch.bfloat16)
+        # top-k keeps the best one and the first k - 1 of the equal ones
+        k = same // 2
+        kept = at[:k]
+        u = torch.tensor([0.0, 0.4, 0.9999])
+        got = K.sample_tokens(x.to(dev), u.to(dev), top_k=k, temperature=1e30).tolist()
+        # equal weights: the running sum exceeds u k first after floor(u k) + 1 of them (the fp32 nearest to 0.9999
+        # is below it: 9998 of 10000)
+        assert got == [int(kept[int(float(v) * k)]) for v in u]
+        # top-p 0.25: the best one (e) and as many equal ones (1 each) as it takes to reach a quarter of the mass
+        p, total = 0.25, same - 1 + math.e
+        n = math.ceil(p * total - math.e)
+        ones = torch.cat([at[:5], at[6:]])[:n]
+        last = int(torch.cat([ones, at[5:6]]).max())
+        assert K.sample_tokens(x.to(dev), torch.full((3,), 1.0).to(dev), top_p=p).tolist() == [last] * 3
