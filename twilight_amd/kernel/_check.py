@@ -59,17 +59,17 @@ def stream_of(x: torch.Tensor) -> int:
     return torch.cuda.current_stream(x.device).cuda_stream
 
 
-def stream_and_switch(dev: torch.device):
-    """The raw handle of ``dev``'s current stream, and whether a launch needs the device switched first
+def stream_and_switch(index: int):
+    """The raw handle of the current stream of device ``index``, and whether a launch needs the device switched first
     (:func:`stream_of` and ``torch.cuda.device`` at a tenth of their cost: an op that is over in
     microseconds notices)."""
-    return torch._C._cuda_getCurrentRawStream(dev.index), torch.cuda.current_device() != dev.index
+    return torch._C._cuda_getCurrentRawStream(index), torch._C._cuda_getDevice() != index
 
 
-def fine_rows(dev: torch.device, dtype: torch.dtype, *tensors) -> bool:
-    """Whether every tensor is contiguous, of ``dtype`` and on ``dev``: the quick form of
+def fine_rows(index: int, dtype: torch.dtype, *tensors) -> bool:
+    """Whether every tensor is contiguous, of ``dtype`` and on device ``index``: the quick form of
     :func:`check_input`, :func:`check_dtype` and :func:`check_same_device`, which name what is wrong."""
     for t in tensors:
-        if t.dtype is not dtype or not t.is_contiguous() or t.device != dev:
+        if t.dtype is not dtype or not t.is_contiguous() or t.get_device() != index:
             return False
     return True

@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._check import (check_cuda, check_dim, check_dtype, check_input, check_same_device, fine_rows, ptr,
+from ._check import (check_dim, check_dtype, check_input, check_same_device, fine_rows, ptr,
                      stream_and_switch)
 from .attention import _cache_strides
 from .quant_cache import KV_FORMATS, check_page_table, check_quant_cache
@@ -34,10 +34,10 @@ def _bound(value, name: str, least: int) -> int:
 def _fine(q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len) -> bool:
     """Whether the operands are plainly right; if not, :func:`_check` finds out what is wrong."""
     try:
-        dev, cs = q.device, k_cache.stride()
-        if not (q.is_cuda and q.dim() == 3 and q.is_contiguous() and q.dtype in _QUERY_TYPES and len(cs) == 4
+        dev, cs = q.get_device(), k_cache.stride()
+        if not (dev >= 0 and q.dim() == 3 and q.is_contiguous() and q.dtype in _QUERY_TYPES and len(cs) == 4
                 and v_cache.stride() == cs and cs[3] == 1 and v_cache.shape == k_cache.shape
-                and v_cache.dtype is k_cache.dtype and k_cache.device == dev and v_cache.device == dev):
+                and v_cache.dtype is k_cache.dtype and k_cache.get_device() == dev and v_cache.get_device() == dev):
             return False
         B, H, D = q.shape
         pages, page, Hkv, Dk = k_cache.shape
@@ -50,7 +50,7 @@ def _fine(q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr
         return (v_scale is not None and k_cache.dtype in KV_FORMATS and k_scale.dtype is torch.float32
                 and v_scale.dtype is torch.float32 and k_scale.shape == k_cache.shape[:3]
                 and v_scale.shape == k_scale.shape and k_scale.stride() == v_scale.stride()
-                and k_scale.device == dev and v_scale.device == dev)
+                and k_scale.get_device() == dev and v_scale.get_device() == dev)
     except AttributeError:                    # no tensor
         return False
 
@@ -87,7 +87,7 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
             kv_last_page_len, max_tokens, sm_scale, return_lse, out, workspace, what):
     """The launch; the operands have been checked."""
     B, H, D = q.shape
-    Hkv, dev, dtype = k_cache.size(2), q.device, q.dtype
+    Hkv, dev, dtype = k_cache.size(2), q.get_device(), q.dtype
     cs = k_cache.stride()
     if k_scale is None:
         ss, fmt = (0, 0, 0), _QUERY_TYPES[dtype]
@@ -104,7 +104,7 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
         check_input(out, "out"); check_same_device(q, ("out", out))
         if out.shape != q.shape or out.dtype != dtype:
             raise RuntimeError("out must match q")
-    lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
+    lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     p_ids, p_ptr, p_last, g_ptr, groups, max_prefix, max_group = prefix
     L = _lib.lib()
@@ -113,8 +113,8 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
         workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     else:
         check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
-        if workspace.numel() < need or workspace.device != dev:
-            raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
+        if workspace.numel() < need or workspace.get_device() != dev:
+            raise RuntimeError(f"workspace must hold {need} bytes on {q.device}")
     rc = L.twl_prefix_attn(
         q.data_ptr(), out.data_ptr(), _QUERY_TYPES[dtype], k_cache.data_ptr(), v_cache.data_ptr(), fmt, cs[0], cs[1],
         cs[2], ptr(k_scale), ptr(v_scale), *ss, k_cache.size(0), ptr(p_ids), ptr(p_ptr), ptr(p_last), ptr(g_ptr),
@@ -179,16 +179,16 @@ def prefix_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     operands = (q, k_cache, v_cache, k_scale, v_scale, kv_page_indices, kv_page_indptr, kv_last_page_len)
     if not _fine(*operands):
         _check(*operands)
-    tables = (("group_indptr", group_indptr), ("prefix_page_indices", prefix_page_indices),
-              ("prefix_page_indptr", prefix_page_indptr), ("prefix_last_page_len", prefix_last_page_len))
-    for name, t in tables:
-        if not isinstance(t, torch.Tensor):
-            check_cuda(t, name)
-    groups, batch = group_indptr.numel() - 1, q.size(0)
-    if not (1 <= groups <= batch and prefix_page_indptr.numel() == groups + 1
-            and prefix_last_page_len.numel() == groups
-            and fine_rows(q.device, torch.int32, group_indptr, prefix_page_indices, prefix_page_indptr,
-                          prefix_last_page_len)):
+    batch = q.size(0)
+    try:
+        groups = group_indptr.numel() - 1
+        fine = (1 <= groups <= batch and prefix_page_indptr.numel() == groups + 1
+                and prefix_last_page_len.numel() == groups
+                and fine_rows(q.get_device(), torch.int32, group_indptr, prefix_page_indices, prefix_page_indptr,
+                              prefix_last_page_len))
+    except AttributeError:                    # no tensor
+        fine = False
+    if not fine:
         check_input(group_indptr, "group_indptr"); check_dtype(group_indptr, torch.int32, "group_indptr")
         if groups < 1 or groups > batch:
             raise RuntimeError("group_indptr must have groups + 1 elements, with 1 to batch groups")

@@ -62,13 +62,15 @@ def _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_las
 def _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len) -> bool:
     """Whether a cache and its tables are plainly right; if not, the checks above find out what is wrong."""
     try:
-        dev, cs, batch = k_cache.device, k_cache.stride(), token_indptr.numel() - 1
-        return (k_cache.is_cuda and len(cs) == 4 and cs[3] == 1 and k_cache.size(1) == _lib.PAGE
-                and k_cache.size(3) == _lib.HEAD_DIM and k_cache.dtype in KV_FORMATS and v_cache.dtype is k_cache.dtype
-                and v_cache.stride() == cs and v_cache.shape == k_cache.shape and v_cache.device == dev
+        dev, cs, batch = k_cache.get_device(), k_cache.stride(), token_indptr.numel() - 1
+        shape = k_cache.shape
+        return (dev >= 0 and len(cs) == 4 and cs[3] == 1 and shape[1] == _lib.PAGE and shape[3] == _lib.HEAD_DIM
+                and k_cache.dtype in KV_FORMATS and v_cache.dtype is k_cache.dtype
+                and v_cache.stride() == cs and v_cache.shape == shape and v_cache.get_device() == dev
                 and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
-                and k_scale.shape == k_cache.shape[:3] and v_scale.shape == k_scale.shape
-                and k_scale.stride() == v_scale.stride() and k_scale.device == dev and v_scale.device == dev
+                and k_scale.shape == shape[:3] and v_scale.shape == k_scale.shape
+                and k_scale.stride() == v_scale.stride() and k_scale.get_device() == dev
+                and v_scale.get_device() == dev
                 and batch >= 1 and kv_page_indptr.numel() == batch + 1 and kv_last_page_len.numel() == batch
                 and fine_rows(dev, torch.int32, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len))
     except AttributeError:                    # no tensor
@@ -92,13 +94,12 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
     if not _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len):
         check_quant_cache(k_cache, v_cache, k_scale, v_scale)
         _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
-    for name, t in (("k_new", k_new), ("v_new", v_new)):
-        if not isinstance(t, torch.Tensor):
-            check_cuda(t, name)
-    dev, Hkv, ns = k_cache.device, k_cache.size(2), k_new.stride()
+    if not (isinstance(k_new, torch.Tensor) and isinstance(v_new, torch.Tensor)):
+        check_cuda(k_new, "k_new"); check_cuda(v_new, "v_new")
+    dev, Hkv, ns = k_cache.get_device(), k_cache.size(2), k_new.stride()
     if not (k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and len(ns) == 3 and ns[2] == 1 and k_new.dtype in _ROW_TYPES
             and v_new.shape == k_new.shape and v_new.stride() == ns and v_new.dtype is k_new.dtype
-            and k_new.device == dev and v_new.device == dev):
+            and k_new.get_device() == dev and v_new.get_device() == dev):
         for name, t in (("k_new", k_new), ("v_new", v_new)):
             check_cuda(t, name); check_dim(3, t, name)
             if t.size(1) != Hkv or t.size(2) != _lib.HEAD_DIM or t.stride(2) != 1:
@@ -138,7 +139,7 @@ def kv_quant_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
     if not _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len):
         check_quant_cache(k_cache, v_cache, k_scale, v_scale)
         _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
-    dev, Hkv, tokens = k_cache.device, k_cache.size(2), int(tokens)
+    dev, Hkv, tokens = k_cache.get_device(), k_cache.size(2), int(tokens)
     if tokens < 0:
         raise RuntimeError("tokens must not be negative")
     code = dtype_code(dtype, "dtype")

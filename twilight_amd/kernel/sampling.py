@@ -194,7 +194,7 @@ def _row_filter(value, name: str, rows: int, ref: torch.Tensor, dtype: torch.dty
     """A filter of :func:`sample_tokens`: one number for every row, or a tensor with one per row.
     Returns its pointer (0: a number) and the number."""
     if isinstance(value, torch.Tensor):
-        if value.numel() != rows or not fine_rows(ref.device, dtype, value):
+        if value.numel() != rows or not fine_rows(ref.get_device(), dtype, value):
             check_input(value, name); check_dtype(value, dtype, name)
             check_same_device(ref, (name, value))
             raise RuntimeError(f"{name} tensor must have one element per row ({rows})")
@@ -236,7 +236,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
         raise RuntimeError("logits must have 1 to 65535 rows and 1 to 262144 columns")
     if vocab > 1 and logits.stride(1) != 1:
         raise RuntimeError("logits must be contiguous along the vocabulary")
-    code, dev = dtype_code(logits.dtype, "logits"), logits.device
+    code, dev = dtype_code(logits.dtype, "logits"), logits.get_device()
     if not isinstance(u, torch.Tensor) or u.numel() != rows or not fine_rows(dev, torch.float32, u):
         check_input(u, "u"); check_dtype(u, torch.float32, "u"); check_same_device(logits, ("u", u))
         raise RuntimeError(f"u must have one element per row ({rows})")
@@ -260,8 +260,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     else:
         check_input(workspace, "workspace"); check_dtype(workspace, torch.uint8, "workspace")
-        if workspace.numel() < need or workspace.device != dev:
-            raise RuntimeError(f"workspace must hold {need} bytes on {dev}")
+        if workspace.numel() < need or workspace.get_device() != dev:
+            raise RuntimeError(f"workspace must hold {need} bytes on {logits.device}")
     rc = _lib.lib().twl_sample_tokens(
         logits.data_ptr(), code, logits.stride(0), rows, vocab, u.data_ptr(), t_arr, t_val, k_arr, k_val, p_arr,
         p_val, m_arr, m_val, out.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
