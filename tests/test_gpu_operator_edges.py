@@ -16,7 +16,7 @@ F16, BF16 = torch.float16, torch.bfloat16
 
 @pytest.mark.parametrize("fmt,Hkv", [(I8, 6), (E4, 5)])
 def test_bulk_calls_with_heads_that_are_no_multiple_of_four(dev, fmt, Hkv):
-    # 33000 tokens of two sets of up to four heads: 66000 sets, over 4096 workgroups of 16
+    # 33000 tokens of two sets of up to four heads: 66000 sets, more than 1024 workgroups of 16
     g = torch.Generator().manual_seed(Hkv)
     lens = [20011, 0, 12989]
     T, pages = sum(lens), sum((n + 15) // 16 for n in lens) + 3

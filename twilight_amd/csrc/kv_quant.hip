@@ -262,12 +262,13 @@ int kv_quant_args(KvQuantArgs& a, uint8_t* k_cache, uint8_t* v_cache, int format
   return TWL_OK;
 }
 
-// Heads per row of 16 lanes, and the grid: four where that leaves two full loads of the chip (2 x 256
-// compute units x 8 workgroups of 16 rows). One head and four, to write and to read: 32768 tokens of 32 heads
-// 189 and 224 us, 166 and 176; 32768 of 8 heads 56 and 42, 51 and 36; 4096 of 8 heads 10.6 and 7.8, 10.8 and 7.5.
+// Heads per row of 16 lanes, and the grid: four where that leaves half a load of the chip (256 compute units x 4
+// workgroups of 16 rows). One head and four, to write and to read: 32768 tokens of 32 heads 189 and 224 us, 166
+// and 176; 16384 of 8 heads 31 and 19, 26 and 18; 8192 of 8 17 and 12, 16 and 10; 4096 of 8 10.6 and 7.8, 10.8
+// and 7.5.
 static bool quant_grid(const KvQuantArgs& a, dim3& grid) {
   const uint64_t four = ((uint64_t)a.tokens * ((a.num_kv_heads + 3) / 4) + 15) / 16;
-  const bool bulk = a.num_kv_heads >= 4 && four >= 4096;
+  const bool bulk = a.num_kv_heads >= 4 && four >= 1024;
   grid = dim3((uint32_t)(bulk ? four : ((uint64_t)a.tokens * a.num_kv_heads + 15) / 16));
   return bulk;
 }
