@@ -698,15 +698,16 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
   }
 }
 
-// Ways to attend to a prefix part, by the rows of a kv head that share it (a 32768-token prompt, bf16 and int8):
+// Kernels by the rows of a kv head that may share a prefix part: up to 16 rows are streamed, above that the
+// rows that a group really has decide (a 32768-token prompt, bf16 and int8):
 //   up to 16   streaming (16 rows: 36 and 27 us, through LDS 36 and 30)
 //   up to 64   through LDS, 16 rows a wavefront, so that none is without rows where half of 128 are (32 rows:
 //              38 and 34 us, streamed in two sets of 16 40 and 34; 48 rows: 40 and 35, with 32 rows a
 //              wavefront 42 and 42)
 //   above      through LDS, 32 rows a wavefront (96 rows: 47 and 44 us, in tiles of 64 46 and 52; 64 samples
 //              of four q heads with up to 600 tokens of their own: 84 us and 96)
-enum PrefixMode { kStream, kStaged64, kStaged128 };
-constexpr int mode_rows(int mode) { return mode == kStream ? 16 : mode == kStaged64 ? 64 : 128; }
+enum PrefixMode { kStream, kStaged };
+constexpr int mode_rows(int mode) { return mode == kStream ? 16 : 128; }
 constexpr size_t mode_lds(int mode) {
   return mode == kStream || sizeof(PartLds) > sizeof(StagedLds) ? sizeof(PartLds) : sizeof(StagedLds);
 }
@@ -744,11 +745,13 @@ __global__ __launch_bounds__(kPaThreads, 2) void prefix_attn_kernel(PrefixAttnAr
     };
     const int32_t* ids = a.p_ids + a.p_ptr[g];
     const int num_ids = a.p_ptr[g + 1] - a.p_ptr[g];
-    if constexpr (MODE != kStream)
-      attend_staged<QT, KV, mode_rows(MODE) / 64>(a, ids, num_ids, begin, end, kvh, rows - row0, row_of, c, parts,
-                                                  pool);
-    else
+    const int here = rows - row0;
+    if (MODE == kStream || here <= 16)
       attend_part<QT, KV>(a, ids, num_ids, begin, end, kvh, row_of, c, parts, pool);
+    else if (here <= 64)
+      attend_staged<QT, KV, 1>(a, ids, num_ids, begin, end, kvh, here, row_of, c, parts, pool);
+    else
+      attend_staged<QT, KV, 2>(a, ids, num_ids, begin, end, kvh, here, row_of, c, parts, pool);
   } else {
     const uint32_t kvh = id % a.num_kv_heads;
     id /= a.num_kv_heads;
@@ -855,7 +858,7 @@ static PrefixPlan prefix_plan(uint32_t batch, uint32_t num_q_heads, uint32_t num
   PrefixPlan p{};
   const uint32_t G = num_q_heads / num_kv_heads;
   const uint64_t rows = (uint64_t)max_group * G;
-  p.mode = rows <= 16 ? kStream : rows <= 64 ? kStaged64 : kStaged128;
+  p.mode = rows <= 16 ? kStream : kStaged;
   p.p_tiles = (uint32_t)((rows + mode_rows(p.mode) - 1) / mode_rows(p.mode));
   p.tiles = (G + 15) / 16;
   // Prefix tokens: two workgroups per compute unit, one full load of the chip (64 samples of a 32768-token bf16
@@ -881,8 +884,7 @@ static void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& p, uint32_t
 #define TWL_PA(MODE) \
   hipLaunchKernelGGL((prefix_attn_kernel<QT, KV, MODE>), dim3(blocks), dim3(kPaThreads), 0, st, a)
   if (a.p_chunks == 0 || p.mode == kStream) TWL_PA(kStream);
-  else if (p.mode == kStaged64) TWL_PA(kStaged64);
-  else TWL_PA(kStaged128);
+  else TWL_PA(kStaged);
 #undef TWL_PA
 }
 
