@@ -568,7 +568,7 @@ int twl_kv_quant_read(void* k_out, void* v_out, int dtype, const int32_t* token_
  * prefix_page_indptr / prefix_last_page_len, and then their own pages kv_page_*; a request outside
  * every group sees its own pages only. groups == 0: no prefix, the prefix arguments are ignored.
  *   out[b, h] = softmax(sm_scale * q[b, h] . K) V in dtype;  lse_out (nullable) float [batch, q heads]
- * A request that sees no token gives a zero row and lse -inf.
+ * A request that sees no token gives a zero row and lse -inf. sm_scale must be finite.
  * format: dtype itself for 16-bit pages, or TWL_I8 / TWL_E4M3 with k_scale / v_scale (see
  * twl_kv_quant_append). Any number of q heads per kv head. max_prefix_tokens, max_group_size and
  * max_tokens size the launch: prefix tokens beyond the first are not attended to, members of a group
@@ -577,9 +577,9 @@ int twl_kv_quant_read(void* k_out, void* v_out, int dtype, const int32_t* token_
  * that is not below num_pages is read as page num_pages - 1.
  * Strides in elements, multiples of 8 (16-bit pages) or 16 (8-bit); token stride <= 2^24.
  * The softmax weights are rounded to the 16-bit type of the V product (dtype, or fp16 over 8-bit
- * pages); their sum is not. workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means that the
- * call needs none), 16-byte aligned, no initial contents required;
- * calls that share it must not overlap in time.
+ * pages); their sum is not. workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means
+ * that the call needs none), 16-byte aligned, no initial contents required; calls that share it must
+ * not overlap in time.
  * ------------------------------------------------------------------------------------------- */
 uint64_t twl_prefix_attn_workspace_bytes(uint32_t batch, uint32_t num_q_heads,
                                          uint32_t num_kv_heads, uint32_t groups,
