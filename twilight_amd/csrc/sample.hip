@@ -29,8 +29,8 @@
 // pick alone, digit by digit over the whole row.
 //
 // Not bound by memory (64 bf16 rows of 128256: 16 MB, 3 us): hist and keep by the 64-bit weights of every token
-// (14 and 18 us there), pick by its chain of sums and by fetching code that is used once (15 us). One row of
-// 32000: 4, 7 and 8 us. Logits read a second time in a loop, instead of kept in registers through unrolled
+// (14 and 18 us there), pick by its chain of sums and by fetching code that is used once (14 us). One row of
+// 32000: 4, 7 and 6 us. Logits read a second time in a loop, instead of kept in registers through unrolled
 // code, cost hist and keep 1 and 2 us; copies of hist's bins against atomics on one address changed nothing.
 #include "twl_common.h"
 
@@ -736,48 +736,51 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, uint32_t en
         return hi;
       }
     }
-    const int shift = max(0, 64 - __builtin_clzll(hi - lo) - kSmpDigitBits);
+    uint32_t n = 0;
+    if (entries > kWave) {                  // few entries are ranked as they are (2 of them: pick 7.4 -> 6.4 us)
+      const int shift = max(0, 64 - __builtin_clzll(hi - lo) - kSmpDigitBits);
 #pragma unroll 1
-    for (uint32_t i = threadIdx.x; i < entries; i += kSmpThreads) {
-      const uint64_t e = sh.list[i];
-      if (e >= lo && e <= hi) {
-        const uint32_t at = (uint32_t)((hi - e) >> shift) * kSmpCopies + lane_id() % kSmpCopies;
-        atomicAdd((unsigned long long*)&sh.hist[at], (unsigned long long)meas(e));
-        atomicAdd(&sh.count[at], 1u);
+      for (uint32_t i = threadIdx.x; i < entries; i += kSmpThreads) {
+        const uint64_t e = sh.list[i];
+        if (e >= lo && e <= hi) {
+          const uint32_t at = (uint32_t)((hi - e) >> shift) * kSmpCopies + lane_id() % kSmpCopies;
+          atomicAdd((unsigned long long*)&sh.hist[at], (unsigned long long)meas(e));
+          atomicAdd(&sh.count[at], 1u);
+        }
       }
-    }
-    __syncthreads();
-    // a digit's copies are read by four neighbouring lanes
-    static_assert(kSmpSlots == 4 * kSmpThreads && kSmpCopies == 16, "four slots a thread, four threads a digit");
-    uint64_t s = 0, total;
-    uint32_t c = 0;
+      __syncthreads();
+      // a digit's copies are read by four neighbouring lanes
+      static_assert(kSmpSlots == 4 * kSmpThreads && kSmpCopies == 16, "four slots a thread, four threads a digit");
+      uint64_t s = 0, total;
+      uint32_t c = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s += sh.hist[4 * threadIdx.x + j];
-      c += sh.count[4 * threadIdx.x + j];
-      sh.hist[4 * threadIdx.x + j] = 0;
-      sh.count[4 * threadIdx.x + j] = 0;
+      for (int j = 0; j < 4; ++j) {
+        s += sh.hist[4 * threadIdx.x + j];
+        c += sh.count[4 * threadIdx.x + j];
+        sh.hist[4 * threadIdx.x + j] = 0;
+        sh.count[4 * threadIdx.x + j] = 0;
+      }
+      s += dpp64<kDppXor1, 0xF>(s);
+      s += dpp64<kDppXor2, 0xF>(s);
+      c += (uint32_t)dpp<kDppXor1>(0, (int)c);
+      c += (uint32_t)dpp<kDppXor2>(0, (int)c);
+      const bool lead = threadIdx.x % 4 == 0;
+      const uint64_t run = block_scan(sh, lead ? s : 0, total) + above;
+      if (digits == 0 && total < target) return 0;
+      if (lead && run < target && run + s >= target) {
+        sh.word[0] = threadIdx.x / 4;
+        sh.word[1] = c;
+        sh.wide[0] = run;
+      }
+      __syncthreads();
+      const uint64_t digit = sh.word[0];
+      n = sh.word[1];
+      above = sh.wide[0];
+      hi -= digit << shift;
+      const uint64_t width = (1ull << shift) - 1;
+      const uint64_t least = hi > width ? hi - width : 0;   // one type on both sides of max, or it is the double's
+      lo = max(lo, least);
     }
-    s += dpp64<kDppXor1, 0xF>(s);
-    s += dpp64<kDppXor2, 0xF>(s);
-    c += (uint32_t)dpp<kDppXor1>(0, (int)c);
-    c += (uint32_t)dpp<kDppXor2>(0, (int)c);
-    const bool lead = threadIdx.x % 4 == 0;
-    const uint64_t run = block_scan(sh, lead ? s : 0, total) + above;
-    if (digits == 0 && total < target) return 0;
-    if (lead && run < target && run + s >= target) {
-      sh.word[0] = threadIdx.x / 4;
-      sh.word[1] = c;
-      sh.wide[0] = run;
-    }
-    __syncthreads();
-    const uint64_t digit = sh.word[0];
-    const uint32_t n = sh.word[1];
-    above = sh.wide[0];
-    hi -= digit << shift;
-    const uint64_t width = (1ull << shift) - 1;
-    const uint64_t least = hi > width ? hi - width : 0;   // one type on both sides of max, or it is the double's
-    lo = max(lo, least);
     if (n <= kWave) {
 #pragma unroll 1
       for (uint32_t i = threadIdx.x; i < entries; i += kSmpThreads) {
@@ -788,7 +791,9 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, uint32_t en
           sh.left[at][1] = meas(e);
         }
       }
+      if (threadIdx.x == 0) sh.wide[1] = 0;
       __syncthreads();
+      n = sh.members;
       // the measure in front of every member, an eighth of the members per wavefront
       const uint32_t member = threadIdx.x % kWave, first = threadIdx.x / kWave * (kWave / kSmpWaves);
       if (member < n) {
@@ -807,8 +812,8 @@ __device__ __forceinline__ uint64_t entry_reaching(SampleShared& sh, uint32_t en
         sh.before[threadIdx.x] = 0;
         if (before < target && before + sh.left[threadIdx.x][1] >= target) sh.wide[1] = sh.left[threadIdx.x][0];
       }
-      if (threadIdx.x == 0) sh.members = 0;
       __syncthreads();
+      if (threadIdx.x == 0) sh.members = 0;
       const uint64_t got = sh.wide[1];
       __syncthreads();
       return got;
