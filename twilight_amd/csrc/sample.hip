@@ -548,7 +548,7 @@ template <class F>
 __device__ __forceinline__ uint32_t first_beyond(SampleShared& sh, uint32_t vocab, uint64_t target, F measure) {
   const uint32_t segs = (vocab + kWave - 1) / kWave;
   const int wave = threadIdx.x / kWave;
-  uint64_t before = 0;                  // measure of the segments in front of this round
+  uint64_t before = 0;                  // measure of the segments in front of these
   for (uint32_t s0 = 0; s0 < segs; s0 += kSmpThreads) {
     const uint32_t s = s0 + threadIdx.x;
     const uint64_t m = s < segs ? sh.seg[s] : 0ull;
