@@ -577,7 +577,9 @@ int twl_kv_quant_read(void* k_out, void* v_out, int dtype, const int32_t* token_
  * that is not below num_pages is read as page num_pages - 1.
  * Strides in elements, multiples of 8 (16-bit pages) or 16 (8-bit); token stride <= 2^24.
  * The softmax weights are rounded to the 16-bit type of the V product (dtype, or fp16 over 8-bit
- * pages); their sum is not. workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means
+ * pages); their sum is not. In fp16 a weight keeps its 11 bits down to 2^-26 of the row's largest one
+ * (over 8-bit pages: weight times V scale, down to 2^-25 of the largest weight times the largest V
+ * scale), and what lies below is off by up to 2^-37 (2^-36) of that. workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means
  * that the call needs none), 16-byte aligned, no initial contents required; calls that share it must
  * not overlap in time.
  * ------------------------------------------------------------------------------------------- */

@@ -1,0 +1,111 @@
+"""Decode attention where a few tokens take nearly all of the softmax and the answer comes from the others:
+dominant tokens whose V is zero or small, and V rows of very different size, attended to or not.
+
+Bounds. The rows are compared with attention in 64 bits on the values the pages hold, element by element and
+relative to the sum of p |v| that the element is made of. A weight that enters an fp16 product is off by half
+a step (2^-11 of it); below fp16's normal range by 2^-25 of the product's unit, but never by more than
+itself. The largest weight that a wavefront has seen is at least 2^12 units, so that 2^-25 is 2^-37 of it.
+Over 8-bit pages the weight is taken times its V scale relative to a power of two that is less than twice
+the largest V scale seen: 2^-36 of the largest weight times that scale. Logits are fp32 sums of 128 exact
+products (130 * 2^-24 of their summed magnitudes, in numerator and denominator), sums of n terms and exp2
+(n + 64) * 2^-24, the output's own rounding half a step."""
+import math
+
+import pytest
+import torch
+
+from _quant import HALF_STEP, decode, encode
+from test_gpu_prefix_attn import Case
+
+pytestmark = pytest.mark.gpu
+I8, E4 = torch.int8, torch.float8_e4m3fn
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+class Sink(Case):
+    """One kv head whose query reads channel 0 of K only: token ``at`` has a logit ``gap`` (nats) above all
+    others. ``vsize[t]`` is the size of token t's V. ``spare`` samples share the tokens as a prefix."""
+
+    def __init__(self, dev, dtype, fmt, H, n, gap, vsize, at=3, samples=1, seed=0):
+        prefix = dict(plens=[n], members=[samples], lens=[0] * samples) if fmt is None or samples > 1 else dict(lens=[n])
+        super().__init__(dev, dtype, fmt, H, 1, seed=seed, **prefix)
+        per = (self.pper if self.plens else self.per)[0]
+        g = torch.Generator().manual_seed(seed + 1)
+        k = torch.randn(n, 1, 128, generator=g)
+        k[:, :, 0] = 0.0
+        k[at, :, 0] = 4.0
+        v = (1 + torch.rand(n, 1, 128, generator=g)) * torch.as_tensor(vsize).float().reshape(-1, 1, 1)
+        self.q = torch.zeros(len(self.lens), H, 128)
+        self.q[:, :, 0] = gap * math.sqrt(128) / 4
+        self.q = self.q.to(dtype)
+        page, slot = per[torch.arange(n) // 16], torch.arange(n) % 16
+        self.n, self.vs = n, torch.ones(n, dtype=torch.float64)
+        for i, x in enumerate((k, v)):
+            if fmt is None:
+                self.pools[i][page, slot] = x.to(dtype).to(dev)
+                self.values[i][page, slot] = x.to(dtype).double()
+            else:
+                codes, scale = encode(x, fmt)
+                self.pools[i].view(torch.uint8)[page, slot] = codes.view(torch.uint8).to(dev)
+                self.scales[i][page, slot] = scale.to(dev)
+                self.values[i][page, slot] = decode(codes, scale).double()
+                if i:
+                    self.vs = scale[:, 0].double()
+
+    def check_small(self, got, scale=128 ** -0.5):
+        out = got[0].cpu().double()
+        for b in range(len(self.lens)):
+            k, v = (x[:, 0] for x in self.seen(b))                        # [n, 128]
+            q = self.q[b].double()
+            z = torch.matmul(q, k.T.contiguous()) * scale
+            p = torch.softmax(z, -1)                                      # [H, n]
+            ref, mag = torch.matmul(p, v), torch.matmul(p, v.abs())
+            dz = 130 * 2.0 ** -24 * (torch.matmul(q.abs(), k.abs().T.contiguous()) * scale).amax(-1, keepdim=True)
+            half, unit = (2.0 ** -11, 2.0 ** -36 if self.fmt is not None else 2.0 ** -37)
+            if self.fmt is None and self.dtype == BF16:
+                half, unit = 2.0 ** -8, 0.0
+            lost = unit * p.amax(-1, keepdim=True) * self.vs.max() / self.vs   # per weight, [H, n]
+            floor = torch.matmul(torch.minimum(p, lost), v.abs())
+            rel = half + 2 * dz + (self.n + 64) * 2.0 ** -24
+            bound = rel * mag + floor
+            bound = bound + HALF_STEP[self.dtype] * (ref.abs() + bound) + (2.0 ** -25 if self.dtype == F16 else 0.0)
+            err = (out[b] - ref).abs()
+            assert torch.all(err <= bound), f"off by {(err / bound).max():.2f} bounds, {(err / mag).max():.4f} of sum p|v|"
+
+
+@pytest.mark.parametrize("samples", [1, 5, 12])         # 4 rows are streamed; 20 and 48 go through LDS
+@pytest.mark.parametrize("fmt", [None, I8, E4])
+@pytest.mark.parametrize("gap", [12.0, 17.5, 18.5, 20.0])
+def test_dominant_token_without_a_value(dev, fmt, gap, samples):
+    # 17.5 nats are 2^-25.2, where weights relative to the largest one leave fp16. V of 2^20 keeps an fp16 answer
+    # in its normal range
+    n = 1500
+    v = torch.full((n,), 2.0 ** 10 if fmt is None else 2.0 ** 20)
+    v[3] = 0.0
+    c = Sink(dev, F16, fmt, 4, n, gap, v, samples=samples)
+    c.check_small(c.call())
+
+
+@pytest.mark.parametrize("samples", [1, 5])
+@pytest.mark.parametrize("fmt", [I8, E4])
+@pytest.mark.parametrize("gap,big", [(11.5, 8), (12.5, 8), (18.0, 0), (12.0, 20)])
+def test_values_of_very_different_size(dev, fmt, gap, big, samples):
+    # a dominant token with a small V, and one token of weight e^-gap like the rest whose V is 2^big times theirs, in
+    # the same tile
+    n = 1024
+    v = torch.full((n,), 1.0)
+    v[3], v[20] = 2.0 ** -18, 2.0 ** big
+    c = Sink(dev, BF16, fmt, 4, n, gap, v, samples=samples)
+    c.check_small(c.call())
+
+
+@pytest.mark.parametrize("samples", [1, 5])
+@pytest.mark.parametrize("fmt", [I8, E4])
+@pytest.mark.parametrize("big", [8, 16, 22])
+def test_answer_made_of_small_values_beside_a_large_one_nobody_attends_to(dev, fmt, big, samples):
+    # all tokens weigh the same but token 3 (e^-18) whose V is 2^big times the others'
+    n = 1024
+    v = torch.full((n,), 1.0)
+    v[3] = 2.0 ** big
+    c = Sink(dev, BF16, fmt, 4, n, -18.0, v, samples=samples)
+    c.check_small(c.call())

@@ -3,8 +3,8 @@
 // Request b of group g sees the tokens of the group's prefix pages and then its own:
 //     out[b, h] = softmax(sm_scale * q[b, h] . K) V        lse[b, h] = log sum exp(logit)
 // A softmax over a set of tokens is the merge of softmaxes over its parts: every part leaves
-// (m, l, acc) = (running maximum, sum of exp2(s - m), sum of exp2(s - m) V) of its tokens, and parts
-// are joined by rescaling to the common maximum. So the prefix is read once per group and kv head,
+// (m, l, acc) = (a reference, sum of exp2(s - m), sum of exp2(s - m) V) of its tokens, and parts
+// are joined by rescaling to the largest reference. So the prefix is read once per group and kv head,
 // with the queries of all its requests as the columns of one matrix product, and the requests' own
 // tokens are ordinary parts beside it.
 //
@@ -19,17 +19,24 @@
 //                 16 lanes covers a token's 128 channels) and transposes 8 x 8 in registers; product
 //                 j takes channel 8 n + j of every lane.
 // A lane of O^T then holds 32 consecutive channels of ONE query, so maxima, sums and rescaling are
-// per-lane scalars. The maximum is only raised (and the accumulators rescaled) when a logit exceeds
-// it by more than 8 in base 2: weights stay below 2^8, exact in what fp32 and the 16-bit operands
-// can hold, and most tiles need no reduction across lanes at all.
+// per-lane scalars. The reference m of a row's weights 2^(s - m) is only raised (and the accumulators rescaled)
+// when a logit leaves the room above it, so that most tiles need no reduction across lanes at all. l, the
+// accumulators and m belong together, wherever in that room the largest logit lies.
 //
 // 8-bit pages run on fp16 products (codes are exact in fp16). The scale of K multiplies the logit.
-// The scale of V joins the weight, relative to a running power of two that bounds the V scales seen
-// (weight * scale * 2^-e < 2^9 fits fp16 whatever the scales are); a bf16 query is first brought
-// into fp16's range by a power of two of its own.
+// The scale of V joins the weight, relative to a running power of two that bounds the V scales seen; a bf16
+// query is first brought into fp16's range by a power of two of its own.
 //
-// The weights are rounded to the product's 16-bit type (half a step, relative to each weight); the
-// sum l takes them before that rounding, in fp32.
+// The weights are rounded to the product's 16-bit type; the sum l takes them before that rounding, in fp32. In
+// bf16 that is half a step (2^-8) of each weight. So it is in fp16 (2^-11) down to fp16's normal range, below
+// which a weight is off by up to 2^-25 of the product's unit. A token that takes nearly all of the weight and
+// has a small V leaves the answer to weights like that, so fp16 products use the range above 1: a row's
+// reference is put 12 below its largest logit in base 2 and a logit may exceed it by 14 before it is raised.
+// Weights are then below 2^14, also times a V scale (taken below 1), the largest one seen at least 2^12, and what
+// is lost below the normal range is 2^-37 of that one (over 8-bit pages 2^-36 of it times the largest V scale
+// seen). The smaller room raises references more often: 33 samples over int8 in three groups 39.3 -> 40.4 us, 8
+// requests of 32768 int8 tokens 98 before and after.
+// bf16 has fp32's range: the reference is the maximum and the room 8.
 //
 // What bounds it: one read of K and V where few rows share it (8 requests of 32768 int8 tokens, 8 kv heads:
 // 554 MB in 93 us, 5.9 TB/s), products and exponentials where many do (256 samples of a 32768-token bf16
@@ -47,8 +54,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int kPaThreads = 256;
 constexpr int kPaWaves = kPaThreads / kWave;
 constexpr int kPaTile = 32;                 // tokens of one step of a wavefront
-constexpr float kPaNoMax = -3.0e38f;        // running maximum before the first token
-constexpr float kPaSlack = 8.0f;            // how far a logit may exceed it, in base 2
+constexpr float kPaNoMax = -3.0e38f;        // reference before the first token
 constexpr uint32_t kPaMaxParts = 256;       // of one kind, per row
 constexpr float kPaLeastScale = 1.17549435e-38f;   // 2^-126: -inf times it is -inf
 constexpr float kLn2 = 0.693147180559945309f;
@@ -104,6 +110,19 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
                                                   __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                  __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// How far a row's reference lies below its largest logit when it is set, and how far above it a logit may
+// come, in base 2 (MT: type of the second product's operands).
+template <int MT> constexpr float kPaBelow = MT == TWL_F16 ? 12.0f : 0.0f;
+template <int MT> constexpr float kPaRoom = MT == TWL_F16 ? 14.0f : 8.0f;
+
+// The reference m raised for a largest logit of `top`. Where the difference is lost in fp32's steps (logits
+// beyond 2^26) it is the logit itself.
+template <int MT>
+__device__ __forceinline__ float raised(float m, float top) {
+  const float up = fmaxf(m, top - kPaBelow<MT>);
+  return top - up > kPaRoom<MT> ? top : up;
 }
 
 template <int MT>
@@ -349,7 +368,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
         rise = e1 - vexp;
         vexp = e1;
       }
-      const float down = as_f32((127 - vexp) << 23);
+      const float down = 0.5f * as_f32((127 - vexp) << 23);
 #pragma unroll
       for (int i = 0; i < 8; ++i) vs[i >> 2][i & 3] *= down;
     }
@@ -363,8 +382,8 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
       top = fmaxf(top, z);
     }
     top *= row_scale;
-    if (__any(top > m + kPaSlack)) {
-      const float up = fmaxf(m, max_over_kb(top));
+    if (__any(top - m > kPaRoom<MT>)) {
+      const float up = raised<MT>(m, max_over_kb(top));
       const float alpha = __builtin_amdgcn_exp2f(m - up);
       m = up;
       l *= alpha;
@@ -437,7 +456,7 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   }
 
   // ---- join the wavefronts that share rows, and leave the part --------------------------------
-  const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
+  const float vfac = k8 ? 2.0f * as_f32((127 + vexp) << 23) : 1.0f;
   auto& lds = *(PartLds*)pool;
   l = sum_over_kb(l);
   if (kb == 0) {
@@ -611,7 +630,7 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
       const int e = max(min((as_i32(top) >> 23) - 127, 126), vexp);
       rise = e - vexp;
       vexp = e;
-      const float down = as_f32((127 - vexp) << 23);
+      const float down = 0.5f * as_f32((127 - vexp) << 23);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         ks[p] = *(const f32x4*)&lds.ks[buf][32 * h + 16 * p + 4 * kb];
@@ -630,8 +649,8 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
         top = fmaxf(top, z);
       }
       top *= row_scale[x];
-      if (__any(top > m[x] + kPaSlack)) {
-        const float up = fmaxf(m[x], max_over_kb(top));
+      if (__any(top - m[x] > kPaRoom<MT>)) {
+        const float up = raised<MT>(m[x], max_over_kb(top));
         const float alpha = __builtin_amdgcn_exp2f(m[x] - up);
         m[x] = up;
         l[x] *= alpha;
@@ -687,7 +706,7 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
     products(tiles - 1, 1, Always{});
   }
 
-  const float vfac = k8 ? as_f32((127 + vexp) << 23) : 1.0f;
+  const float vfac = k8 ? 2.0f * as_f32((127 + vexp) << 23) : 1.0f;
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
     const float total = sum_over_kb(l[x]);
