@@ -109,3 +109,31 @@ def test_answer_made_of_small_values_beside_a_large_one_nobody_attends_to(dev, f
     v[3] = 2.0 ** big
     c = Sink(dev, BF16, fmt, 4, n, -18.0, v, samples=samples)
     c.check_small(c.call())
+
+
+@pytest.mark.parametrize("samples", [1, 5, 12])
+@pytest.mark.parametrize("fmt", [I8, E4])
+@pytest.mark.parametrize("down", [12, 20, 24])
+def test_query_channels_of_very_different_size(dev, fmt, down, samples):
+    # a bf16 query whose largest channel meets zeros in K, so that the logits come from channels 2^down smaller:
+    # each of them keeps its 8 bits, so that the bounds are those of any other query
+    prefix = dict(plens=[300], members=[samples], lens=[7] * samples) if samples > 1 else dict(lens=[300])
+    c = Case(dev, BF16, fmt, 8, 2, seed=down, **prefix)
+    c.pools[0].view(torch.uint8)[..., 0] = 0
+    c.values[0][..., 0] = 0.0
+    q = c.q.float() * 2.0 ** -down
+    q[:, :, 0] = 1.5
+    c.q = q.to(BF16)
+    c.check(c.call(sm_scale=2.0 ** down * 128 ** -0.5), scale=2.0 ** down * 128 ** -0.5)
+
+
+@pytest.mark.parametrize("samples", [1, 5])
+@pytest.mark.parametrize("fmt", [I8, E4])
+def test_tiny_queries_over_huge_keys(dev, fmt, samples):
+    # K scales of 2^103 and a query that makes up for them: products stay below fp32's largest number
+    prefix = dict(plens=[200], members=[samples], lens=[7] * samples) if samples > 1 else dict(lens=[200])
+    c = Case(dev, BF16, fmt, 8, 2, gain=2.0 ** 108, seed=1, **prefix)
+    c.q = (c.q.float() * 2.0 ** -108).to(BF16)
+    got = c.call()
+    assert torch.isfinite(got[0]).all()
+    c.check(got)

@@ -201,7 +201,11 @@ __device__ __forceinline__ void load_query(const PrefixAttnArgs& a, int row, int
       for (int i = 0; i < 8; ++i) top = max(top, as_i32(f[j][i]) & 0x7FFFFFFF);
     }
     top = as_i32(max_over_kb(as_f32(top)));
-    const int e = min(max((top >> 23) - 127, -126), 126);   // |q| < 2^(e + 1); NaN stays NaN
+    // |q| < 2^(e + 15), below fp16's 2^16, so that a channel keeps its 8 bits down to 2^-31 of the largest one
+    // (relative to 1 it was 2^-16, and logits can come from channels smaller than that). A query below 2^-60 meets
+    // K scales whose products with that would overflow: it comes down to 1. NaN stays NaN
+    const int size = (top >> 23) - 127;
+    const int e = min(max(size - min(max(size + 74, 0), 14), -126), 126);
     const float down = as_f32((127 - e) << 23);
     scale *= as_f32((127 + e) << 23);
 #pragma unroll
