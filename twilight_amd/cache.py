@@ -38,13 +38,14 @@ class _PageTable:
         ip = kv_page_indptr.cpu().long()
         npg = ip[1:] - ip[:-1]
         self.max_pages_per_req = int(npg.max().item())
-        self._seq_lens = ((npg - 1) * PAGE + kv_last_page_len.cpu().long()).tolist()
+        lens = (npg - 1) * PAGE + kv_last_page_len.cpu().long()
+        self._seq_lens = torch.where(npg > 0, lens, 0).tolist()   # a request without pages holds nothing
         # host mirrors of the table: append() never reads the device copies back
         ids = kv_page_indices.cpu().tolist()
         ipl = ip.tolist()
         self._per_req = [ids[ipl[b]:ipl[b + 1]] for b in range(len(ipl) - 1)]
         self._last = kv_last_page_len.cpu().tolist()
-        self._room = PAGE - max(self._last) if self._last else 0
+        self._room = PAGE - max(self._last) if self._last and all(self._per_req) else 0
         self._append_key = None
         self._table_cap = 0
 
@@ -78,7 +79,7 @@ class _PageTable:
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, free_pages: Optional[list] = None) -> None:
         """Decode append of one token per request: ``k_new`` / ``v_new`` [B, Hkv, 128]. Extends the
-        page table when a request's last page is full (taking ids from ``free_pages``; host-side
+        page table when a request's last page is full or it has none (taking ids from ``free_pages``; host-side
         bookkeeping only, nothing is read back from the device), then one kernel writes the token
         and updates the lengths (and, beside 16-bit pages, the shadow records). The two halves are also callable on their
         own: :meth:`advance_host` every step before a recorded step is replayed,
@@ -88,13 +89,13 @@ class _PageTable:
 
     def advance_host(self, free_pages: Optional[list] = None) -> None:
         """Host half of :meth:`append`: make room for one more token per request (a new page from
-        ``free_pages`` where the last one is full) and count the token."""
+        ``free_pages`` where the last one is full or there is none) and count the token."""
         B = self.batch
         per_req, last = self._per_req, self._last
         grew = False
-        if self._room <= 0:  # some request may have filled its last page
+        if self._room <= 0:  # some request may have filled its last page, or has none yet
             for b in range(B):
-                if last[b] == PAGE:
+                if last[b] == PAGE or not per_req[b]:
                     if not free_pages:
                         raise RuntimeError("PagedKVCache.append: no free page left")
                     per_req[b].append(int(free_pages.pop(0)))
