@@ -92,39 +92,43 @@ class _PageTable:
         ``free_pages`` where the last one is full or there is none) and count the token."""
         B = self.batch
         per_req, last = self._per_req, self._last
-        grew = False
         if self._room <= 0:  # some request may have filled its last page, or has none yet
-            for b in range(B):
-                if last[b] == PAGE or not per_req[b]:
-                    if not free_pages:
-                        raise RuntimeError("PagedKVCache.append: no free page left")
-                    per_req[b].append(int(free_pages.pop(0)))
-                    last[b] = 0
-                    grew = True
+            new = [b for b in range(B) if last[b] == PAGE or not per_req[b]]
+            if new:
+                self._take_pages(new, free_pages)
             self._room = PAGE - max(last)
-        if grew:  # a request took a new page: the CSR arrays change shape, lengths are re-sent
-            flat = [p for r in per_req for p in r]
-            ptr = [0]
-            for r in per_req:
-                ptr.append(ptr[-1] + len(r))
-            if self._table_cap:
-                if max(len(r) for r in per_req) > self._table_cap:
-                    raise RuntimeError("PagedKVCache.append: request outgrew reserve_page_table")
-                self.kv_page_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
-                self.kv_page_indptr.copy_(torch.tensor(ptr, dtype=torch.int32))
-            else:
-                self.kv_page_indices = torch.tensor(flat, dtype=torch.int32, device=self.device)
-                self.kv_page_indptr = torch.tensor(ptr, dtype=torch.int32, device=self.device)
-                self.max_pages_per_req = max(len(r) for r in per_req)
-            if self.meta_planes is not None and self.max_pages_per_req > self.meta_planes.size(4):
-                raise RuntimeError("PagedKVCache.append: request outgrew the plane buffer "
-                                   "(enable_planes with a larger cap_pages)")
-            # same tensor object every step, so cached argument blocks of the layer stay valid
-            self.kv_last_page_len.copy_(torch.tensor(last, dtype=torch.int32))
         self._room -= 1
         for b in range(B):
             last[b] += 1
             self._seq_lens[b] += 1
+
+    def _take_pages(self, requests: list, free_pages: Optional[list]) -> None:
+        """A new page from ``free_pages`` for each of ``requests``: the CSR arrays change shape, lengths are re-sent.
+        What is refused is refused before anything changes."""
+        per_req, last, what = self._per_req, self._last, f"{type(self).__name__}.append"
+        if len(free_pages or ()) < len(requests):
+            raise RuntimeError(f"{what}: no free page left")
+        longest = max(max(len(r) for r in per_req), max(len(per_req[b]) + 1 for b in requests))
+        if self._table_cap and longest > self._table_cap:
+            raise RuntimeError(f"{what}: request outgrew reserve_page_table")
+        if self.meta_planes is not None and longest > self.meta_planes.size(4):
+            raise RuntimeError(f"{what}: request outgrew the plane buffer (enable_planes with a larger cap_pages)")
+        for b in requests:
+            per_req[b].append(int(free_pages.pop(0)))
+            last[b] = 0
+        flat = [p for r in per_req for p in r]
+        ptr = [0]
+        for r in per_req:
+            ptr.append(ptr[-1] + len(r))
+        if self._table_cap:
+            self.kv_page_indices[:len(flat)].copy_(torch.tensor(flat, dtype=torch.int32))
+            self.kv_page_indptr.copy_(torch.tensor(ptr, dtype=torch.int32))
+        else:
+            self.kv_page_indices = torch.tensor(flat, dtype=torch.int32, device=self.device)
+            self.kv_page_indptr = torch.tensor(ptr, dtype=torch.int32, device=self.device)
+            self.max_pages_per_req = longest
+        # same tensor object every step, so cached argument blocks of the layer stay valid
+        self.kv_last_page_len.copy_(torch.tensor(last, dtype=torch.int32))
 
 
 class PagedKVCache(_PageTable):
