@@ -8,6 +8,7 @@ import torch
 
 from . import _lib
 from .kernel import kv_append, kv_quant_append, kv_quant_read, kv_shadow_build, meta_planes_build
+from .kernel._check import check_cuda, check_same_device
 
 PAGE = _lib.PAGE
 HEAD_DIM = _lib.HEAD_DIM
@@ -18,6 +19,7 @@ class _PageTable:
     the layout benchmark/efficiency/bench_gemv.py:425-431 builds) with its host mirror."""
 
     device: torch.device
+    num_kv_heads: int
     meta_planes: Optional[torch.Tensor] = None
 
     def _no_table(self) -> None:
@@ -79,13 +81,21 @@ class _PageTable:
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, free_pages: Optional[list] = None) -> None:
         """Decode append of one token per request: ``k_new`` / ``v_new`` [B, Hkv, 128]. Extends the
-        page table when a request's last page is full or it has none (taking ids from ``free_pages``; host-side
-        bookkeeping only, nothing is read back from the device), then one kernel writes the token
-        and updates the lengths (and, beside 16-bit pages, the shadow records). The two halves are also callable on their
-        own: :meth:`advance_host` every step before a recorded step is replayed,
-        :meth:`append_device` inside the recorded step."""
+        page table when a request's last page is full or it has none (taking ids from ``free_pages``;
+        host-side bookkeeping only, nothing is read back from the device), then writes the token and
+        updates the lengths on the device (and, beside 16-bit pages, the shadow records). Rows that do not
+        fit are refused before anything is counted. The two halves are also callable on their own:
+        :meth:`advance_host` every step before a recorded step is replayed, :meth:`append_device` inside
+        the recorded step."""
+        self._check_rows(k_new, v_new)
         self.advance_host(free_pages)
         self.append_device(k_new, v_new)
+
+    def _check_rows(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+        shape = (self.batch, self.num_kv_heads, HEAD_DIM)
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            if not isinstance(t, torch.Tensor) or t.shape != shape:
+                raise RuntimeError(f"{type(self).__name__}.append: {name} must be {list(shape)}")
 
     def advance_host(self, free_pages: Optional[list] = None) -> None:
         """Host half of :meth:`append`: make room for one more token per request (a new page from
@@ -346,12 +356,23 @@ class QuantPagedKVCache(_PageTable):
         return c
 
     def append_device(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
-        """Device half of :meth:`append`: count one token per request and write it, ``k_new`` / ``v_new``
-        [B, Hkv, 128] (fp16 / bf16). :meth:`advance_host` must have made room for it."""
+        """Device half of :meth:`append`: count one token per request, then write it (two launches), ``k_new`` /
+        ``v_new`` [B, Hkv, 128] (fp16 / bf16). :meth:`advance_host` must have made room for it."""
+        self._check_rows(k_new, v_new)
+        ks = k_new.stride()
+        if v_new.stride() != ks or ks[2] != 1 or (ks[0] | ks[1]) & 7 or (k_new.data_ptr() | v_new.data_ptr()) & 15:
+            # not as the kernel's 16-byte loads take them
+            k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
         self.kv_last_page_len.add_(1)
-        if k_new.stride() != v_new.stride() or k_new.stride(-1) != 1:
-            k_new, v_new = k_new.contiguous(), v_new.contiguous()
         kv_quant_append(k_new, v_new, self._one_each, *self.pools, *self.table)
+
+    def _check_rows(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+        super()._check_rows(k_new, v_new)
+        if k_new.dtype not in (torch.float16, torch.bfloat16) or v_new.dtype != k_new.dtype:
+            raise RuntimeError("QuantPagedKVCache.append: k_new and v_new must be float16 or bfloat16, both the same")
+        for name, t in (("k_new", k_new), ("v_new", v_new)):
+            check_cuda(t, name)
+        check_same_device(self.k_cache, ("k_new", k_new), ("v_new", v_new))
 
     def read(self, dtype: torch.dtype = torch.bfloat16):
         """The values of every request's tokens, ``(k, v)`` [sum of lengths, Hkv, 128] in order."""
