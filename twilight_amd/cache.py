@@ -9,6 +9,7 @@ import torch
 from . import _lib
 from .kernel import kv_append, kv_quant_append, kv_quant_read, kv_shadow_build, meta_planes_build
 from .kernel._check import check_cuda, check_same_device
+from .kernel.quant_cache import row_strides
 
 PAGE = _lib.PAGE
 HEAD_DIM = _lib.HEAD_DIM
@@ -359,8 +360,9 @@ class QuantPagedKVCache(_PageTable):
         """Device half of :meth:`append`: count one token per request, then write it (two launches), ``k_new`` /
         ``v_new`` [B, Hkv, 128] (fp16 / bf16). :meth:`advance_host` must have made room for it."""
         self._check_rows(k_new, v_new)
-        ks = k_new.stride()
-        if v_new.stride() != ks or ks[2] != 1 or (ks[0] | ks[1]) & 7 or (k_new.data_ptr() | v_new.data_ptr()) & 15:
+        t, h = row_strides(k_new)
+        if row_strides(v_new) != (t, h) or k_new.stride(2) != 1 or v_new.stride(2) != 1 or (t | h) & 7 \
+                or (k_new.data_ptr() | v_new.data_ptr()) & 15:
             # not as the kernel's 16-byte loads take them
             k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
         self.kv_last_page_len.add_(1)

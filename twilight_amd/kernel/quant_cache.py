@@ -77,15 +77,24 @@ def _fine(k_cache, v_cache, k_scale, v_scale, token_indptr, kv_page_indices, kv_
         return False
 
 
+def row_strides(rows: torch.Tensor) -> Tuple[int, int]:
+    """Token and head stride of [T,Hkv,128] rows, 0 where there is one token or head and the tensor's own stride
+    means nothing."""
+    T, Hkv, _ = rows.shape
+    t, h, _ = rows.stride()
+    return t if T > 1 else 0, h if Hkv > 1 else 0
+
+
 def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torch.Tensor,
                     k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, kv_page_indices: torch.Tensor,
                     kv_page_indptr: torch.Tensor, kv_last_page_len: torch.Tensor) -> None:
-    """Quantise the rows of ``k_new`` / ``v_new`` [T,Hkv,128] (fp16 / bf16, head_dim contiguous) into
-    8-bit pages in one launch.
+    """Quantise the rows of ``k_new`` / ``v_new`` [T,Hkv,128] (fp16 / bf16, head_dim contiguous, the other
+    strides the same for both and multiples of 8, 16-byte aligned) into 8-bit pages in one launch.
 
-    ``k_cache`` / ``v_cache`` [pages,16,Hkv,128] int8 or float8_e4m3fn (any page / token / head
-    strides), ``k_scale`` / ``v_scale`` fp32 [pages,16,Hkv]. Every (token, kv head) row is scaled by its
+    ``k_cache`` / ``v_cache`` [pages,16,Hkv,128] int8 or float8_e4m3fn (page / token / head strides
+    that are multiples of 8; attention over them takes multiples of 16), ``k_scale`` / ``v_scale`` fp32
+    [pages,16,Hkv] of any strides. Every (token, kv head) row is scaled by its
     own largest magnitude: ``scale = max(max|x| / T, 2**-126)`` with T = 127 or 448, code = x / scale
     rounded to nearest even. Rows ``token_indptr[b]`` to ``token_indptr[b + 1]`` (int32 [B+1]) are the
     last tokens of request b: the page table counts them already. Rows from ``token_indptr[B]`` on are
@@ -96,9 +105,10 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
         _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
     if not (isinstance(k_new, torch.Tensor) and isinstance(v_new, torch.Tensor)):
         check_cuda(k_new, "k_new"); check_cuda(v_new, "v_new")
-    dev, Hkv, ns = k_cache.get_device(), k_cache.size(2), k_new.stride()
-    if not (k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and len(ns) == 3 and ns[2] == 1 and k_new.dtype in _ROW_TYPES
-            and v_new.shape == k_new.shape and v_new.stride() == ns and v_new.dtype is k_new.dtype
+    dev, Hkv = k_cache.get_device(), k_cache.size(2)
+    if not (k_new.dim() == 3 and k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and k_new.dtype in _ROW_TYPES
+            and v_new.shape == k_new.shape and k_new.stride(2) == v_new.stride(2) == 1
+            and row_strides(v_new) == row_strides(k_new) and v_new.dtype is k_new.dtype
             and k_new.get_device() == dev and v_new.get_device() == dev):
         for name, t in (("k_new", k_new), ("v_new", v_new)):
             check_cuda(t, name); check_dim(3, t, name)
@@ -106,7 +116,7 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
                 raise RuntimeError(f"{name} must be [T, {Hkv}, {_lib.HEAD_DIM}] with contiguous head_dim")
             if t.dtype not in _ROW_TYPES:
                 raise RuntimeError(f"{name} must be float16 or bfloat16")
-        if v_new.shape != k_new.shape or v_new.stride() != k_new.stride() or v_new.dtype != k_new.dtype:
+        if v_new.shape != k_new.shape or row_strides(v_new) != row_strides(k_new) or v_new.dtype != k_new.dtype:
             raise RuntimeError("k_new and v_new must share shape, dtype and strides")
         check_same_device(k_cache, ("k_new", k_new), ("v_new", v_new))
     if k_new.size(0) == 0:
@@ -116,7 +126,7 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
         with torch.cuda.device(dev):
             return kv_quant_append(k_new, v_new, token_indptr, k_cache, v_cache, k_scale, v_scale, kv_page_indices,
                                    kv_page_indptr, kv_last_page_len)
-    cs, ss = k_cache.stride(), k_scale.stride()
+    ns, cs, ss = row_strides(k_new), k_cache.stride(), k_scale.stride()
     rc = _lib.lib().twl_kv_quant_append(
         k_new.data_ptr(), v_new.data_ptr(), _ROW_TYPES[k_new.dtype], ns[0], ns[1], token_indptr.data_ptr(),
         k_new.size(0), k_cache.data_ptr(), v_cache.data_ptr(), KV_FORMATS[k_cache.dtype], cs[0], cs[1], cs[2],
