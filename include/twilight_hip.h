@@ -574,7 +574,8 @@ int twl_kv_quant_read(void* k_out, void* v_out, int dtype, const int32_t* token_
  * max_tokens size the launch: prefix tokens beyond the first are not attended to, members of a group
  * beyond the second do not see the prefix, own tokens beyond the third are not attended to
  * (each <= 2^24, groups <= batch, max_group_size <= batch, batch * q heads <= 65535). A page id
- * that is not below num_pages is read as page num_pages - 1.
+ * that is not below num_pages is read as page num_pages - 1. kv_page_indices may be NULL where max_tokens
+ * is 0, prefix_page_indices where max_prefix_tokens is 0.
  * Strides in elements, multiples of 8 (16-bit pages) or 16 (8-bit); token stride <= 2^24.
  * The softmax weights are rounded to the 16-bit type of the V product (dtype, or fp16 over 8-bit
  * pages); their sum is not. In fp16 a weight keeps its 11 bits down to 2^-26 of the row's largest one

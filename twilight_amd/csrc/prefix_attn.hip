@@ -937,9 +937,10 @@ extern "C" int twl_prefix_attn(
     uint32_t num_kv_heads, float sm_scale, float* lse_out, void* workspace,
     uint64_t workspace_bytes, void* stream) {
   const bool k8 = format == TWL_I8 || format == TWL_E4M3;
-  if (!q || !out || !k_cache || !v_cache || !kv_page_indices || !kv_page_indptr || !kv_last_page_len)
+  if (!q || !out || !k_cache || !v_cache || (max_tokens && !kv_page_indices) || !kv_page_indptr || !kv_last_page_len)
     return TWL_ENULL;
-  if (groups && (!prefix_page_indices || !prefix_page_indptr || !prefix_last_page_len || !group_indptr))
+  if (groups && ((max_prefix_tokens && !prefix_page_indices) || !prefix_page_indptr || !prefix_last_page_len ||
+                 !group_indptr))
     return TWL_ENULL;
   if (k8 && (!k_scale || !v_scale)) return TWL_ENULL;
   if (dtype != TWL_F16 && dtype != TWL_BF16) return TWL_EDTYPE;

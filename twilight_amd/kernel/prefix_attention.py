@@ -107,6 +107,10 @@ def _attend(q, k_cache, v_cache, k_scale, v_scale, prefix, kv_page_indices, kv_p
     lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     p_ids, p_ptr, p_last, g_ptr, groups, max_prefix, max_group = prefix
+    if kv_page_indices.numel() == 0:          # no list holds a page, and the tensor has no address
+        max_tokens = 0
+    if groups and p_ids.numel() == 0:
+        max_prefix = 0
     L = _lib.lib()
     need = L.twl_prefix_attn_workspace_bytes(B, H, Hkv, groups, max_prefix, max_group, max_tokens)
     if workspace is None:

@@ -119,8 +119,8 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
         if v_new.shape != k_new.shape or row_strides(v_new) != row_strides(k_new) or v_new.dtype != k_new.dtype:
             raise RuntimeError("k_new and v_new must share shape, dtype and strides")
         check_same_device(k_cache, ("k_new", k_new), ("v_new", v_new))
-    if k_new.size(0) == 0:
-        return
+    if k_new.size(0) == 0 or kv_page_indices.numel() == 0:
+        return                                # no row, or none that has a place
     stream, switch = stream_and_switch(dev)
     if switch:
         with torch.cuda.device(dev):
@@ -170,6 +170,8 @@ def kv_quant_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.T
         v_out = torch.empty(shape, dtype=dtype, device=dev)
     if tokens == 0:
         return k_out, v_out
+    if kv_page_indices.numel() == 0:          # no list holds a page, and the tensor has no address
+        kv_page_indices, kv_page_indptr = kv_page_indptr, torch.zeros_like(kv_page_indptr)
     cs, ss = k_cache.stride(), k_scale.stride()
     rc = _lib.lib().twl_kv_quant_read(
         k_out.data_ptr(), v_out.data_ptr(), code, token_indptr.data_ptr(), tokens, k_cache.data_ptr(),
