@@ -613,8 +613,8 @@ int twl_prefix_attn(const void* q, void* out, int dtype, const void* k_cache, co
  *   The best rank always stays. tokens[r] int64 = the first token in vocabulary order whose running sum of
  *   kept w exceeds u times the sum of all kept w.
  * temperature <= 0 (or NaN in an array): the best token. -inf and NaN logits are never drawn; a row
- * with nothing else gives -1. w is computed in 64 bits and held as a multiple of 2^-45 in integers;
- * equal inputs give equal tokens. workspace: at least twl_sample_tokens_workspace_bytes(rows, vocab)
+ * with nothing else gives -1. w is computed in 64 bits and held as a multiple of 2^-45 in integers,
+ * whose sums are exact: a row's token does not depend on the other rows or on their number. workspace: at least twl_sample_tokens_workspace_bytes(rows, vocab)
  * bytes, 8-byte aligned, no initial contents required; calls that share it must not overlap in
  * time. rows <= 65535.
  * ------------------------------------------------------------------------------------------- */

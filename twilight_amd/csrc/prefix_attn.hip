@@ -85,9 +85,6 @@ struct PrefixAttnArgs {
   f32x2* ml;                                // [rows, parts]
 };
 
-struct Always { static constexpr bool value = true; };
-struct Never { static constexpr bool value = false; };
-
 __device__ __forceinline__ float max_over_kb(float x) {
   const uint32_t u = as_u32(x);
   const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);

@@ -16,22 +16,27 @@
 // No row is sorted. Three launches, the first two with several workgroups (slices) per row so that a
 // small batch fills the chip (w costs about twenty 64-bit operations per token, which a single
 // compute unit would be at for most of the time):
-//   hist  Every slice finds its largest logit and, relative to that, adds up w (top-p) or counts tokens
-//         (top-k) in 512 bins of width T / 16. A bin is floor(16 x / T), so bins of different slices
-//         are the same intervals and the slices' sums join after one rescaling each.
-//   keep  Every slice joins its row's bins and finds the one that holds the cut. With top-p, tokens
-//         above it are kept: their w goes into sums over 512 consecutive tokens, and the tokens of the
-//         cut bin become candidates. With top-k, all tokens down to the cut bin are candidates.
+//   hist  Every slice finds its largest logit and, relative to that, adds up w (top-p, in 32 bits) or
+//         counts tokens (top-k) in 512 bins of width T / 16. A bin is floor(16 x / T), so bins of
+//         different slices are the same intervals and the slices' sums join after one rescaling each.
+//   keep  Every slice joins its row's bins and finds the one that holds the cut. With top-p these are
+//         approximate sums: where a bin ends within their error of the cut, the next one may hold it too.
+//         Tokens above are kept: their w goes into sums over 512 consecutive tokens, and the tokens of
+//         the cut's bin or bins become candidates. On the way every w, relative to the row's best token, is
+//         added up exactly: what top-p reaches for. With top-k, all tokens down to the cut bin are
+//         candidates.
 //   pick  One workgroup per row finds the exact cut among the candidates, digit by digit of the logit's
 //         ordered bit pattern (then of the index, where equal logits are cut), adds the kept ones to
 //         the sums and draws.
 // A row whose candidates do not fit (more than kSmpMaxCand tokens within T / 16 of the cut) is done by
 // pick alone, digit by digit over the whole row.
 //
-// Not bound by memory (64 bf16 rows of 128256: 16 MB, 3 us): hist and keep by the 64-bit weights of every token
-// (14 and 18 us there), pick by its chain of sums and by fetching code that is used once (14 us). One row of
-// 32000: 4, 7 and 6 us. Logits read a second time in a loop, instead of kept in registers through unrolled
-// code, cost hist and keep 1 and 2 us; copies of hist's bins against atomics on one address changed nothing.
+// Not bound by memory (64 bf16 rows of 128256: 16 MB, 3 us): hist by the atomics and the weights of every token (11
+// us there), keep by their 64-bit weights (26; 18 when it weighed kept tokens only and took the mass to reach
+// from the bins, so that the cut could depend on how a batch is sliced), pick by its chain of sums and by
+// fetching code that is used once (15 us). One row of 32000: 4, 7 and 7 us. Weights in 64 bits cost hist 4 us.
+// Logits read a second time in a loop, instead of kept in registers through unrolled code, cost hist and keep 1
+// and 2 us; copies of hist's bins against atomics on one address changed nothing.
 #include "twl_common.h"
 
 namespace twl {
@@ -44,6 +49,7 @@ constexpr int kSmpBins = 512;
 constexpr int kSmpSeg = 512;                   // tokens of one running sum: a wavefront, 8 a lane
 constexpr int kSmpStep = kSmpThreads * 8;      // tokens of one pass of a workgroup
 constexpr uint32_t kSmpMaxCand = 8192;
+constexpr double kSmpHistError = 1.0 / (1 << 18);   // of a row's mass, what the bins' sums may be off by
 
 struct SampleArgs {
   const void* logits;
@@ -66,12 +72,12 @@ struct SampleArgs {
   uint32_t cand_stride;       // min(kSmpMaxCand, vocab)
   struct SampleCut* cut;      // [rows]
   uint32_t* cand_count;       // [rows]
+  uint64_t* mass;             // [rows, slices, 2]  summed w of all tokens, and of those above the cut's bin
 };
 
 // What keep leaves for pick. Tokens from `keep` up are kept, those from `cand` up to there are
-// candidates (a NaN: there are none); for top-p, the mass above the cut's bin and the mass to reach.
+// candidates (a NaN: there are none).
 struct SampleCut {
-  double before, goal;
   float keep, cand;
 };
 
@@ -335,7 +341,8 @@ __global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) 
   const Weigher wt(table, top, f.T);
   const Binner bn = binner(f);
   const int top_bin = bn.bin(top);
-  if (f.by_rank || wt.endless) {
+  // temperatures whose reciprocal 32 bits do not hold, or no longer times a masked logit, are for 64
+  if (f.by_rank || wt.endless || !(f.T > 1e-18 && f.T < 1e18)) {
 #pragma unroll
     for (int t = 0; t < ITERS; ++t)
 #pragma unroll
@@ -345,12 +352,17 @@ __global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) 
           atomicAdd((unsigned long long*)&hist[rel], f.by_rank ? 1ull : (unsigned long long)wt.mass(x[t][j]));
       }
   } else {
+    // w in 32 bits, as a multiple of 2^-45. Off by 1.5 |z| 2^-23 ln 2 + 2^-22 of itself, z = log2 w: the roundings of
+    // the difference, the factor and the product, and the exponential's. |z| averages at most log2 of the
+    // tokens over the mass of a row, 18, so that sums are off by 21 * 2^-23 of the row's mass (kSmpHistError)
+    const float per = (float)(1.44269504088896341 / f.T);
 #pragma unroll
     for (int t = 0; t < ITERS; ++t)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t rel = bn.below(top_bin, x[t][j]);
-        const uint64_t v = Weigher::fixed(wt.scaled(x[t][j]));
+        const float w = __builtin_amdgcn_exp2f((x[t][j] - top) * per) * (float)kSmpOne;
+        const uint64_t v = Weigher::fixed((double)w);
         if (rel < kSmpBins) atomicAdd((unsigned long long*)&hist[rel], (unsigned long long)v);
       }
   }
@@ -372,8 +384,8 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
   __shared__ double wsum[kSmpWaves], table[64];
   __shared__ int slice_shift[64];
   __shared__ double slice_weight[64];
-  __shared__ double cut_before;
-  __shared__ int cut_bin;
+  __shared__ uint64_t wmass[kSmpWaves][2];
+  __shared__ int cut_bin, sure_bin;         // the last bin that the cut may be in, and the first
   __shared__ float cut_keep, cut_cand;
   __shared__ uint32_t list_n, list_at;
   const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
@@ -391,14 +403,12 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
   const int top_bin = bn.bin(top);
   if (threadIdx.x == 0) {
     list_n = 0;
-    cut_bin = f.by_rank ? kSmpBins - 1 : kSmpBins;
-    cut_before = 0.0;
+    cut_bin = sure_bin = kSmpBins - 1;
     cut_keep = -__FLT_MAX__;              // without a cut: everything but -inf, and no candidates
     cut_cand = __builtin_nanf("");
   }
   __syncthreads();
   const Weigher wt(table, top, f.T);
-  double goal = (double)f.k;
   if (f.by_rank || f.by_mass) {
     // this thread's bin of the row, from the slices in order: their shifts and weights first, by one
     // thread each, so that the loads of the bins do not wait for one another
@@ -437,23 +447,24 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
       if (w < wave) off += wsum[w];
       total += wsum[w];
     }
-    if (f.by_mass) goal = f.p * total;
-    const double after = off + incl, before = after - v;
-    // the first bin whose running sum reaches the goal. before may be off by a rounding from the
-    // previous bin's after, so the choice is made once, by the lowest bin that reaches it
-    const uint64_t hit = __ballot(after >= goal && v > 0.0);
+    // the first bin whose running sum reaches the goal. Counts are exact; with masses, the first that may and the
+    // first that surely does. Two units per token are the roundings of its w here and in the exact sums
+    const double goal = f.by_mass ? f.p * total : (double)f.k, after = off + incl;
+    const double off_by = f.by_mass ? total * kSmpHistError + 2.0 * (double)a.vocab : 0.0;
+    const uint64_t sure = __ballot(after >= goal - off_by && v > 0.0);
+    const uint64_t hit = __ballot(after >= goal + off_by && v > 0.0);
+    if (sure && lane_id() == __builtin_ctzll(sure)) atomicMin(&sure_bin, (int)threadIdx.x);
     if (hit && lane_id() == __builtin_ctzll(hit)) atomicMin(&cut_bin, (int)threadIdx.x);
     __syncthreads();
-    if ((int)threadIdx.x == cut_bin) cut_before = before;
-    if (threadIdx.x < 2 && cut_bin < kSmpBins) {
-      const float e = bn.edge((int64_t)top_bin - cut_bin + threadIdx.x);
+    if (threadIdx.x < 2) {
+      const float e = bn.edge((int64_t)top_bin - (threadIdx.x == 0 ? cut_bin : sure_bin - 1));
       if (threadIdx.x == 0) cut_cand = e;
       else cut_keep = f.by_rank ? __builtin_nanf("") : e;
     }
     __syncthreads();
   }
   const float keep = cut_keep, cand = cut_cand;
-  if (slice == 0 && threadIdx.x == 0) a.cut[row] = SampleCut{cut_before, goal, keep, cand};
+  if (slice == 0 && threadIdx.x == 0) a.cut[row] = SampleCut{keep, cand};
   // candidates first: their place in the row's list is a round trip that the weights can hide
   uint32_t hits[ITERS];                   // bit j: token j of the eight is a candidate
 #pragma unroll
@@ -484,7 +495,10 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
   if (!f.by_rank) {
     const double min_w = f.min_p > 0.0 ? f.min_p * kSmpOne : -1.0;
     const uint32_t segs = (a.vocab + kSmpSeg - 1) / kSmpSeg;
-    auto sums = [&](auto weigh) {
+    // FILTERED: min-p is in use, and the mass above the cut's bin is not that of the kept tokens
+    auto sums = [&](auto weigh, auto filtered) {
+      constexpr bool FILTERED = decltype(filtered)::value;
+      uint64_t all = 0, above = 0;
 #pragma unroll
       for (int t = 0; t < ITERS; ++t) {
         uint64_t mine = 0;
@@ -492,20 +506,35 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
         for (int j = 0; j < 8; ++j) {
           const float y = x[t][j];
           const double w = weigh(y);
-          const bool in = y >= keep && (w >= min_w || y == top);
-          mine += in ? Weigher::fixed(w) : 0;
+          const uint64_t v = Weigher::fixed(w);
+          all += v;
+          if (FILTERED) above += y >= keep ? v : 0;
+          mine += y >= keep && (!FILTERED || w >= min_w || y == top) ? v : 0;
         }
         const uint64_t s = wave_sum(mine);
         const uint32_t g = (first + t * kSmpStep) / kSmpSeg;
         if (lane_id() == 0 && g < segs) a.seg[(size_t)row * segs + g] = s;
+        if (!FILTERED) above += s;
+      }
+      all = wave_sum(all);
+      if (FILTERED) above = wave_sum(above);
+      if (lane_id() == 0) {
+        wmass[threadIdx.x / kWave][0] = all;
+        wmass[threadIdx.x / kWave][1] = above;
       }
     };
-    if (wt.endless) sums([&](float y) { return wt.weight(y); });
-    else sums([&](float y) { return wt.scaled(y); });
+    if (wt.endless) sums([&](float y) { return wt.weight(y); }, Always{});
+    else if (f.min_p > 0.0) sums([&](float y) { return wt.scaled(y); }, Always{});
+    else sums([&](float y) { return wt.scaled(y); }, Never{});
   }
-  if (n == 0) return;
   if (threadIdx.x == 0) list_at = row_at;
   __syncthreads();
+  if (f.by_mass && threadIdx.x < 2) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSmpWaves; ++w) sum += wmass[w][threadIdx.x];
+    a.mass[((size_t)row * a.slices + slice) * 2 + threadIdx.x] = sum;
+  }
   for (uint32_t i = threadIdx.x; i < min(n, kSmpMaxCand); i += kSmpThreads)
     if (list_at + i < a.cand_stride) a.cand[(size_t)row * a.cand_stride + list_at + i] = list[i];
 }
@@ -831,6 +860,12 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
   uint64_t best = slice_best(a, row);
   const uint32_t n = a.cand_count[row];
   const SampleCut c = a.cut[row];
+  uint64_t mass[2] = {0, 0};
+  if (lane_id() < a.slices) {
+    const uint64_t* const m = a.mass + ((size_t)row * a.slices + lane_id()) * 2;
+    mass[0] = m[0];
+    mass[1] = m[1];
+  }
   uint64_t seg = threadIdx.x < segs ? a.seg[(size_t)row * segs + threadIdx.x] : 0;
   const uint64_t* const cand = a.cand + (size_t)row * a.cand_stride;
   const uint64_t first = threadIdx.x < a.cand_stride ? cand[threadIdx.x] : 0;
@@ -877,15 +912,19 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
     uint64_t target = (uint64_t)f.k;
     if (by_mass) {
       if (!(f.p < 1.0) || n == 0) break;
-      double goal = c.goal - c.before;
+      uint64_t total, above = 0;
       if (f.by_rank) {
-        uint64_t mine = 0, total;
+        uint64_t mine = 0;
 #pragma unroll 1
         for (uint32_t i = threadIdx.x; i < n; i += kSmpThreads) mine += sh.list[i] >= cut ? mass_of(sh.list[i]) : 0;
         block_scan(sh, mine, total);
-        goal = f.p * (double)total;
+      } else {
+        total = wave_sum(mass[0]);
+        above = wave_sum(mass[1]);
       }
+      const double goal = f.p * (double)total;
       target = goal > 1.0 ? (uint64_t)ceil(goal) : 1ull;
+      target = target > above ? target - above : 1ull;
     } else if (!f.by_rank || (uint32_t)f.k >= n) {
       continue;
     }
@@ -941,7 +980,7 @@ __global__ __launch_bounds__(kSmpThreads) void sample_pick_kernel(SampleArgs a) 
 
 struct SamplePlan {
   uint32_t slices, iters;
-  uint64_t best, hist, seg, cand, cut, count, bytes;   // offsets into the workspace
+  uint64_t best, hist, seg, cand, mass, cut, count, bytes;   // offsets into the workspace
 };
 // Slices of 4096, 8192 or 16384 tokens: as large as leaves a workgroup per compute unit, or two where a row
 // has few slices. Every slice reads the bins of all the row's slices, which is what many of them cost (63
@@ -959,7 +998,8 @@ static SamplePlan sample_plan(uint32_t rows, uint32_t vocab) {
   p.hist = p.best + r * p.slices * 8;
   p.seg = p.hist + r * p.slices * kSmpBins * 8;
   p.cand = p.seg + r * segs * 8;
-  p.cut = p.cand + r * (vocab < kSmpMaxCand ? vocab : kSmpMaxCand) * 8;
+  p.mass = p.cand + r * (vocab < kSmpMaxCand ? vocab : kSmpMaxCand) * 8;
+  p.cut = p.mass + r * p.slices * 16;
   p.count = p.cut + r * sizeof(SampleCut);
   p.bytes = p.count + r * 4;
   return p;
@@ -1012,7 +1052,7 @@ extern "C" int twl_sample_tokens(const void* logits, int dtype, uint64_t row_str
   uint8_t* const ws = (uint8_t*)workspace;
   a.slices = p.slices; a.iters = p.iters; a.best = (uint64_t*)(ws + p.best); a.hist = (uint64_t*)(ws + p.hist);
   a.seg = (uint64_t*)(ws + p.seg); a.cand = (uint64_t*)(ws + p.cand); a.cut = (twl::SampleCut*)(ws + p.cut);
-  a.cand_count = (uint32_t*)(ws + p.count);
+  a.cand_count = (uint32_t*)(ws + p.count); a.mass = (uint64_t*)(ws + p.mass);
   a.cand_stride = vocab < twl::kSmpMaxCand ? vocab : twl::kSmpMaxCand;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == TWL_F16) twl::launch_sample<TWL_F16>(a, st);

@@ -9,6 +9,10 @@
 
 namespace twl {
 
+// truth values as types, for generic lambdas
+struct Always { static constexpr bool value = true; };
+struct Never { static constexpr bool value = false; };
+
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
