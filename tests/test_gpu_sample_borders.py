@@ -117,3 +117,23 @@ def test_temperatures_of_all_sizes(dev, T, rows):
         got = K.sample_tokens(x.to(dev).expand(rows, -1).contiguous(), torch.full((rows,), LAST, device=dev), temperature=t,
                               top_p=p)
         assert got.tolist() == [want] * rows, (p, flat)
+
+
+@pytest.mark.parametrize("below", [14, 18, 20, 24])
+@pytest.mark.parametrize("V", [9001, 50001])
+def test_a_nucleus_of_nearly_everything(dev, below, V):
+    # p = 1 - 2^-below: the cut lies among tokens of next to no weight, found with the same sums
+    g = torch.Generator().manual_seed(300 + below)
+    x = torch.randn(3, V, generator=g) * 3
+    x[:, -1] = x.min() - 0.5                             # the worst token, last in the vocabulary
+    p = 1.0 - 2.0 ** -below
+    want = []
+    for row in x.double():
+        w, order = torch.sort(torch.exp(row - row.max()), descending=True, stable=True)
+        before = torch.cumsum(w, 0) - w
+        gap = (before - p * w.sum()).abs().min() / w.sum()
+        assert gap > 1e-11, "a case too close to a border to be decided"
+        want.append(int(order[before < p * w.sum()].max()))
+    u = torch.full((3,), 1.0, device=dev)                # the last kept token
+    assert K.sample_tokens(x.to(dev), u, top_p=p).tolist() == want
+    assert K.sample_tokens(x.to(dev).repeat(200, 1), u.repeat(200), top_p=p).tolist() == want * 200

@@ -49,7 +49,8 @@ constexpr int kSmpBins = 512;
 constexpr int kSmpSeg = 512;                   // tokens of one running sum: a wavefront, 8 a lane
 constexpr int kSmpStep = kSmpThreads * 8;      // tokens of one pass of a workgroup
 constexpr uint32_t kSmpMaxCand = 8192;
-constexpr double kSmpHistError = 1.0 / (1 << 18);   // of a row's mass, what the bins' sums may be off by
+constexpr double kSmpHistError = 1.0 / (1 << 18);   // of a row's mass, what the bins' sums may be off by,
+constexpr double kSmpSumError = 1.0 / (1ull << 45); // and in 64 bits: some 80 roundings of 2^-53
 
 struct SampleArgs {
   const void* logits;
@@ -172,6 +173,7 @@ struct RowFilter {
   double T, p, min_p;
   int32_t k;
   bool greedy, by_rank, by_mass;   // the best token only; top-k cuts; top-p cuts (and no top-k)
+  bool fine;                       // bins are summed in 64 bits
 };
 __device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, uint32_t row) {
   RowFilter f;
@@ -183,6 +185,9 @@ __device__ __forceinline__ RowFilter row_filter(const SampleArgs& a, uint32_t ro
   f.greedy = !(T > 0.0f) || f.k == 1;
   f.by_rank = f.k > 0 && (uint32_t)f.k < a.vocab;
   f.by_mass = !f.by_rank && f.p < 1.0;
+  // temperatures whose reciprocal 32 bits do not hold, or no longer times a masked logit, and cuts so near the end
+  // that the bins' error in 32 bits would make candidates of the whole tail
+  f.fine = !(f.T > 1e-18 && f.T < 1e18) || f.p > 0.9999;
   return f;
 }
 
@@ -341,8 +346,7 @@ __global__ __launch_bounds__(kSmpThreads) void sample_hist_kernel(SampleArgs a) 
   const Weigher wt(table, top, f.T);
   const Binner bn = binner(f);
   const int top_bin = bn.bin(top);
-  // temperatures whose reciprocal 32 bits do not hold, or no longer times a masked logit, are for 64
-  if (f.by_rank || wt.endless || !(f.T > 1e-18 && f.T < 1e18)) {
+  if (f.by_rank || wt.endless || f.fine) {
 #pragma unroll
     for (int t = 0; t < ITERS; ++t)
 #pragma unroll
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
     // the first bin whose running sum reaches the goal. Counts are exact; with masses, the first that may and the
     // first that surely does. Two units per token are the roundings of its w here and in the exact sums
     const double goal = f.by_mass ? f.p * total : (double)f.k, after = off + incl;
-    const double off_by = f.by_mass ? total * kSmpHistError + 2.0 * (double)a.vocab : 0.0;
+    const double off_by = !f.by_mass ? 0.0 : total * (f.fine ? kSmpSumError : kSmpHistError) + 2.0 * (double)a.vocab;
     const uint64_t sure = __ballot(after >= goal - off_by && v > 0.0);
     const uint64_t hit = __ballot(after >= goal + off_by && v > 0.0);
     if (sure && lane_id() == __builtin_ctzll(sure)) atomicMin(&sure_bin, (int)threadIdx.x);

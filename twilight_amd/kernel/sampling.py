@@ -221,8 +221,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     larger first and equal ones by index: ``top_k`` > 0 keeps the ranks below it; ``top_p`` < 1 keeps, of
     those, the ranks before which less than ``top_p`` of their mass lies; ``min_p`` keeps w >= ``min_p``;
     the best token is always kept. The answer is the first token, in vocabulary order, whose running
-    sum of kept w exceeds ``u`` times the sum of all kept w: w is held as a multiple of 2**-45
-    and sums of it are exact, so that equal rows give equal tokens, in any batch. ``temperature`` 0 takes the best token. Logits of -inf or NaN are never
+    sum of kept w exceeds ``u`` times the sum of all kept w: w is held as a multiple of 2**-45 and sums
+    of it are exact, so that equal rows give equal tokens, in any batch. ``temperature`` 0 takes the best
+    token. Logits of -inf or NaN are never
     drawn; a row that has nothing else gives -1. In tensors, ``temperature`` <= 0 or NaN takes the best
     token; ``top_k`` <= 0, ``top_p`` >= 1 or NaN and ``min_p`` <= 0 or NaN are off; ``top_p`` <= 0 keeps the
     best token only and ``min_p`` >= 1 those whose logit equals the best. ``workspace``: a uint8 tensor of
