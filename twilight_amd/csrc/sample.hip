@@ -32,11 +32,11 @@
 // pick alone, digit by digit over the whole row.
 //
 // Not bound by memory (64 bf16 rows of 128256: 16 MB, 3 us): hist by the atomics and the weights of every token (11
-// us there), keep by their 64-bit weights (26; 18 when it weighed kept tokens only and took the mass to reach
-// from the bins, so that the cut could depend on how a batch is sliced), pick by its chain of sums and by
-// fetching code that is used once (15 us). One row of 32000: 4, 7 and 7 us. Weights in 64 bits cost hist 4 us.
-// Logits read a second time in a loop, instead of kept in registers through unrolled code, cost hist and keep 1
-// and 2 us; copies of hist's bins against atomics on one address changed nothing.
+// us there, 14 with weights in 64 bits), keep by their 64-bit weights (19.5; 18 when it weighed kept tokens only
+// and took the mass to reach from the bins, so that the cut could depend on how a batch is sliced), pick by
+// its chain of sums and by fetching code that is used once (14 us). One row of 32000: 4, 7 and 7 us. Logits
+// read a second time in a loop, instead of kept in registers through unrolled code, cost hist and keep 1 and 2
+// us; copies of hist's bins against atomics on one address changed nothing.
 #include "twl_common.h"
 
 namespace twl {
@@ -381,8 +381,9 @@ __device__ __forceinline__ uint64_t slice_best(const SampleArgs& a, uint32_t row
 }
 
 // ---- second launch -----------------------------------------------------------------------------
+// 128 registers at most, or a compute unit holds one workgroup instead of two (64 rows of 128256: 26 us so, 19.5)
 template <int DT, int ITERS>
-__global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kSmpThreads, 4) void sample_keep_kernel(SampleArgs a) {
   static_assert(kSmpBins == kSmpThreads, "one bin per thread");
   __shared__ uint64_t list[kSmpMaxCand];
   __shared__ double wsum[kSmpWaves], table[64];
@@ -508,7 +509,8 @@ __global__ __launch_bounds__(kSmpThreads) void sample_keep_kernel(SampleArgs a) 
         uint64_t mine = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = x[t][j];
+          float y = x[t][j];
+          asm("" : "+v"(y));                // or what the three uses share is computed before them and fills registers
           const double w = weigh(y);
           const uint64_t v = Weigher::fixed(w);
           all += v;
