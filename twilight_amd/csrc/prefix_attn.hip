@@ -37,6 +37,9 @@
 // seen). The smaller room raises references more often: 33 samples over int8 in three groups 39.3 -> 40.4 us, 8
 // requests of 32768 int8 tokens 98 before and after.
 // bf16 has fp32's range: the reference is the maximum and the room 8.
+// What the rounding costs (64 samples of a 32768-token bf16 prompt): out is off by 0.0023 (root mean square) of its
+// size, 0.0017 of which is its own rounding to bf16. A second product with what the weights lose leaves that
+// 0.0017 and takes 89 us instead of 81. fp16: 0.0003, of which 0.0002.
 //
 // What bounds it: one read of K and V where few rows share it (8 requests of 32768 int8 tokens, 8 kv heads:
 // 554 MB in 93 us, 5.9 TB/s), products and exponentials where many do (256 samples of a 32768-token bf16
@@ -508,8 +511,10 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
 // on that way, once per workgroup. The V operand comes out of LDS transposed (ds_read_b64_tr_b16: of the
 // 4 x 16 elements that 16 lanes name, four consecutive ones each, a lane gets one column), so that
 // product c takes channels 16 c .. 16 c + 15. A row of 256 bytes holds its 16 chunks of 16 bytes at place
-// c ^ f(row % 16), f(r) = 2 (r % 8) + r / 8: the K operand's loads (16 rows, one chunk) then touch every
-// bank once, and so do the transposing ones (four rows, two neighbouring chunks).
+// c ^ f(row % 16), f(r) = 2 (r % 8) + r / 8: 16 rows of one chunk, which the K operand's loads take, and eight
+// rows of two neighbouring chunks, which the transposing ones take, then name every bank once. The
+// counter does not go to zero for that: 2.1 M conflict cycles beside 3.2 M of LDS instructions at work (64
+// samples of a 32768-token prompt), two per transposing load, whose lanes the hardware groups its own way.
 constexpr int kStTile = 64;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;

@@ -105,10 +105,9 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
         _check_tokens(k_cache, token_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
     if not (isinstance(k_new, torch.Tensor) and isinstance(v_new, torch.Tensor)):
         check_cuda(k_new, "k_new"); check_cuda(v_new, "v_new")
-    dev, Hkv = k_cache.get_device(), k_cache.size(2)
-    if not (k_new.dim() == 3 and k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and k_new.dtype in _ROW_TYPES
-            and v_new.shape == k_new.shape and k_new.stride(2) == v_new.stride(2) == 1
-            and row_strides(v_new) == row_strides(k_new) and v_new.dtype is k_new.dtype
+    dev, Hkv, ns = k_cache.get_device(), k_cache.size(2), k_new.stride()
+    if not (k_new.shape[1:] == (Hkv, _lib.HEAD_DIM) and len(ns) == 3 and ns[2] == 1 and k_new.dtype in _ROW_TYPES
+            and v_new.shape == k_new.shape and v_new.stride() == ns and v_new.dtype is k_new.dtype
             and k_new.get_device() == dev and v_new.get_device() == dev):
         for name, t in (("k_new", k_new), ("v_new", v_new)):
             check_cuda(t, name); check_dim(3, t, name)
@@ -119,17 +118,20 @@ def kv_quant_append(k_new: torch.Tensor, v_new: torch.Tensor, token_indptr: torc
         if v_new.shape != k_new.shape or row_strides(v_new) != row_strides(k_new) or v_new.dtype != k_new.dtype:
             raise RuntimeError("k_new and v_new must share shape, dtype and strides")
         check_same_device(k_cache, ("k_new", k_new), ("v_new", v_new))
-    if k_new.size(0) == 0 or kv_page_indices.numel() == 0:
+    T = k_new.size(0)
+    if T == 0 or kv_page_indices.numel() == 0:
         return                                # no row, or none that has a place
     stream, switch = stream_and_switch(dev)
     if switch:
         with torch.cuda.device(dev):
             return kv_quant_append(k_new, v_new, token_indptr, k_cache, v_cache, k_scale, v_scale, kv_page_indices,
                                    kv_page_indptr, kv_last_page_len)
-    ns, cs, ss = row_strides(k_new), k_cache.stride(), k_scale.stride()
+    if T == 1 or Hkv == 1:
+        ns = row_strides(k_new)
+    cs, ss = k_cache.stride(), k_scale.stride()
     rc = _lib.lib().twl_kv_quant_append(
         k_new.data_ptr(), v_new.data_ptr(), _ROW_TYPES[k_new.dtype], ns[0], ns[1], token_indptr.data_ptr(),
-        k_new.size(0), k_cache.data_ptr(), v_cache.data_ptr(), KV_FORMATS[k_cache.dtype], cs[0], cs[1], cs[2],
+        T, k_cache.data_ptr(), v_cache.data_ptr(), KV_FORMATS[k_cache.dtype], cs[0], cs[1], cs[2],
         k_scale.data_ptr(), v_scale.data_ptr(), *ss, k_cache.size(0), kv_page_indices.data_ptr(),
         kv_page_indptr.data_ptr(), kv_last_page_len.data_ptr(), token_indptr.numel() - 1, Hkv, stream)
     if rc:
