@@ -165,3 +165,15 @@ def test_random_rows_whose_values_differ_by_powers_of_two(dev, fmt, prefix, gain
     c = Case(dev, BF16, fmt, 8, 2, [400, 90, 1, 33, 0, 170, 16], seed=9, vgain=12, **more)
     c.q = (c.q.float() * gain).to(BF16)
     check_small(c, c.call())
+
+
+@pytest.mark.parametrize("samples", [1, 5, 12])
+@pytest.mark.parametrize("fmt", [I8, E4])
+def test_large_values_of_one_sign(dev, fmt, samples):
+    # V around 2^112 over 3000 tokens of equal weight: sums of weights times V stay below fp32's largest number
+    n = 3000
+    c = Sink(dev, BF16, fmt, 4, n, 0.0, torch.full((n,), 2.0 ** 112), samples=samples)
+    got = c.call()
+    assert torch.isfinite(got[0]).all()
+    check_small(c, got)
+    assert torch.allclose(got[1].cpu(), torch.full((len(c.lens), 4), math.log(n)))

@@ -83,7 +83,7 @@ struct PrefixAttnArgs {
   uint32_t p_chunk, p_chunks, p_tiles;      // prefix: tokens per part, parts, row tiles per group
   uint32_t chunk, chunks, tiles;            // own tokens: the same
   uint32_t own_blocks;                      // workgroups of the own parts, first in the grid
-  float scale_log2;
+  float scale_log2, lse_below;
   float* acc;                               // [rows, parts, 128]
   f32x2* ml;                                // [rows, parts]
 };
@@ -116,6 +116,9 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 // come, in base 2 (MT: type of the second product's operands).
 template <int MT> constexpr float kPaBelow = MT == TWL_F16 ? 12.0f : 0.0f;
 template <int MT> constexpr float kPaRoom = MT == TWL_F16 ? 14.0f : 8.0f;
+// What sums leave a part with, so that they are as large as if the reference were the largest logit (2^-below): V
+// up to fp32's largest number over the tokens stays finite. lse adds `lse_below` for it.
+template <int MT> constexpr float kPaUnit = MT == TWL_F16 ? 1.0f / 4096.0f : 1.0f;
 
 // The reference m raised for a largest logit of `top`. Where the difference is lost in fp32's steps (logits
 // beyond 2^26) it is the logit itself.
@@ -229,7 +232,7 @@ __device__ __forceinline__ void put_row(const PrefixAttnArgs& a, int row, uint32
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *(u32x2*)((uint16_t*)a.out + (size_t)row * TWL_HEAD_DIM + c) =
       u32x2{pack2<QT>(x[0] * inv, x[1] * inv), pack2<QT>(x[2] * inv, x[3] * inv)};
-  if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : m * kLn2 + logf(l);
+  if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : m * kLn2 + (logf(l) + a.lse_below);
 }
 
 // What the wavefronts of a workgroup exchange at the end of a part.
@@ -460,9 +463,9 @@ __device__ __forceinline__ void attend_part(const PrefixAttnArgs& a, const int32
   }
 
   // ---- join the wavefronts that share rows, and leave the part --------------------------------
-  const float vfac = k8 ? 2.0f * as_f32((127 + vexp) << 23) : 1.0f;
+  const float vfac = kPaUnit<MT> * (k8 ? 2.0f * as_f32((127 + vexp) << 23) : 1.0f);
   auto& lds = *(PartLds*)pool;
-  l = sum_over_kb(l);
+  l = sum_over_kb(l) * kPaUnit<MT>;
   if (kb == 0) {
     lds.m[wave][n] = m;
     lds.l[wave][n] = l;
@@ -712,10 +715,10 @@ __device__ __forceinline__ void attend_staged(const PrefixAttnArgs& a, const int
     products(tiles - 1, 1, Always{});
   }
 
-  const float vfac = k8 ? 2.0f * as_f32((127 + vexp) << 23) : 1.0f;
+  const float vfac = kPaUnit<MT> * (k8 ? 2.0f * as_f32((127 + vexp) << 23) : 1.0f);
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
-    const float total = sum_over_kb(l[x]);
+    const float total = sum_over_kb(l[x]) * kPaUnit<MT>;
     const int row = row_of((wave * NQ + x) * 16 + n);
     if (row < 0) continue;
 #pragma unroll
@@ -852,7 +855,7 @@ __global__ __launch_bounds__(kPaThreads) void prefix_attn_merge_kernel(PrefixAtt
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *(u32x2*)((uint16_t*)a.out + (size_t)row * TWL_HEAD_DIM + 4 * c) =
       u32x2{pack2<QT>(acc[0] * inv, acc[1] * inv), pack2<QT>(acc[2] * inv, acc[3] * inv)};
-  if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : top * kLn2 + logf(l);
+  if (a.lse && c == 0) a.lse[row] = l == 0.0f ? -__builtin_inff() : top * kLn2 + (logf(l) + a.lse_below);
 }
 
 // How a call is cut into workgroups: from the sizes alone, the same for the workspace and the launch.
@@ -991,6 +994,7 @@ extern "C" int twl_prefix_attn(
   a.p_chunks = p.p_chunks; a.p_tiles = p.p_tiles; a.chunk = p.chunk; a.chunks = p.chunks;
   a.tiles = p.tiles; a.own_blocks = (uint32_t)own_blocks;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.lse_below = (k8 || dtype == TWL_F16 ? twl::kPaBelow<TWL_F16> : twl::kPaBelow<TWL_BF16>) * twl::kLn2;
   a.acc = (float*)workspace;
   a.ml = (twl::f32x2*)((float*)workspace + rows * parts * TWL_HEAD_DIM);
   hipStream_t st = (hipStream_t)stream;
