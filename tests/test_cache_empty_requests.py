@@ -83,3 +83,14 @@ def test_16_bit_pages_too(dev):
     c.append(new.to(dev), -new.to(dev), [3])
     assert torch.equal(c.k_cache[3, 0].cpu(), new[0]) and torch.equal(c.v_cache[1, 2].cpu(), -new[1])
     assert c.kv_last_page_len.tolist() == [1, 3] and torch.count_nonzero(c.k_cache).item() == torch.count_nonzero(new).item()
+
+
+@pytest.mark.gpu
+def test_a_cache_from_no_tokens(dev):
+    none = torch.zeros(2, 3, 0, 128, dtype=torch.float16)
+    c = QuantPagedKVCache.from_dense(none, none, torch.int8, dev, spare_pages=4)
+    assert c._seq_lens == [0, 0] and [t.shape[0] for t in c.read()] == [0, 0]
+    new, free = torch.randn(2, 3, 128).half(), [3, 0, 1]
+    c.append(new.to(dev), -new.to(dev), free)
+    k, v = c.read(torch.float32)
+    assert free == [1] and torch.equal(k.cpu(), decode(*encode(new, torch.int8))) and torch.equal(v, -k)

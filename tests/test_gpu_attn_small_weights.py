@@ -177,3 +177,35 @@ def test_large_values_of_one_sign(dev, fmt, samples):
     assert torch.isfinite(got[0]).all()
     check_small(c, got)
     assert torch.allclose(got[1].cpu(), torch.full((len(c.lens), 4), math.log(n)))
+
+
+@pytest.mark.parametrize("samples", [1, 5])
+@pytest.mark.parametrize("fmt", [None, I8])
+@pytest.mark.parametrize("e", [4, 10, 15, 20, 23, 24, 25, 26, 27])
+def test_logits_of_all_sizes(dev, fmt, e, samples):
+    # logits around 2^e in base 2, where fp32's steps grow to 16: every third token has the largest one, the others lie
+    # 2^-9 of it below, which from e = 15 on leaves them nothing
+    n = 500
+    c = Sink(dev, F16, fmt, 4, n, 1.0, torch.ones(n), samples=samples)
+    per = (c.pper if c.plens else c.per)[0]
+    page, slot = per[torch.arange(n) // 16], torch.arange(n) % 16
+    k = torch.zeros(n, 1, 128)
+    k[:, 0, 0] = torch.where(torch.arange(n) % 3 == 0, 1.0, 1.0 - 2.0 ** -9)
+    if fmt is None:
+        c.pools[0][page, slot] = k.half().to(dev)
+        c.values[0][page, slot] = k.double()
+    else:
+        codes, scale = encode(k, fmt)
+        c.pools[0][page, slot], c.scales[0][page, slot] = codes.to(dev), scale.to(dev)
+        c.values[0][page, slot] = decode(codes, scale).double()
+    c.q[:] = 0
+    c.q[:, :, 0] = 1.0
+    out, lse = c.call(sm_scale=2.0 ** e * math.log(2))
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    if e >= 15:
+        for b in range(len(c.lens)):
+            v = c.seen(b)[1][::3, 0]                    # [n / 3, 128], equal weights
+            err = (out[b].cpu().double() - v.mean(0)).abs()
+            assert torch.all(err <= 2.0 ** -10 * v.abs().mean(0))
+    else:
+        check_small(c, (out, lse), scale=2.0 ** e * math.log(2))

@@ -137,3 +137,41 @@ def test_a_nucleus_of_nearly_everything(dev, below, V):
     u = torch.full((3,), 1.0, device=dev)                # the last kept token
     assert K.sample_tokens(x.to(dev), u, top_p=p).tolist() == want
     assert K.sample_tokens(x.to(dev).repeat(200, 1), u.repeat(200), top_p=p).tolist() == want * 200
+
+
+def test_what_a_workspace_holds_does_not_matter(dev):
+    # all bits set (NaN, counts of -1), and what a call of other sizes left
+    x = (torch.randn(5, 40000, generator=torch.Generator().manual_seed(1)) * 3).to(dev)
+    u = torch.rand(5, generator=torch.Generator().manual_seed(2)).to(dev)
+    need = K.sample_tokens_workspace_bytes(5, 40000)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=30), dict(top_k=3000, top_p=0.5, min_p=0.01), dict(temperature=0.0),
+               dict(top_k=20000), dict(top_p=0.99999)):
+        ws = torch.full((need,), 0xFF, dtype=torch.uint8, device=dev)
+        want = K.sample_tokens(x, u, workspace=ws, **kw)
+        assert torch.equal(want, K.sample_tokens(x, u, workspace=ws, **kw))
+        K.sample_tokens(x[:2, :777], u[:2], workspace=ws, top_p=0.3)
+        assert torch.equal(want, K.sample_tokens(x, u, workspace=ws, **kw)) and torch.equal(want, K.sample_tokens(x, u, **kw))
+
+
+def test_a_recorded_draw(dev):
+    # replayed with other logits, filters and numbers in the same tensors, and eager work in between
+    g = torch.Generator().manual_seed(3)
+    B, V = 7, 50001
+    x, u, p = torch.zeros(B, V, device=dev), torch.zeros(B, device=dev), torch.ones(B, device=dev)
+    k = torch.zeros(B, dtype=torch.int32, device=dev)
+    ws = torch.empty(K.sample_tokens_workspace_bytes(B, V), dtype=torch.uint8, device=dev)
+    out = torch.zeros(B, dtype=torch.int64, device=dev)
+    call = lambda o, w: K.sample_tokens(x, u, top_p=p, top_k=k, out=o, workspace=w)  # noqa: E731
+    call(out, ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, ws)
+    for step in range(6):
+        x.copy_(torch.randn(B, V, generator=g) * (1 + step))
+        u.copy_(torch.rand(B, generator=g))
+        p.copy_(torch.rand(B, generator=g))
+        k.copy_(torch.randint(-50, 50, (B,), generator=g).to(torch.int32))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, call(torch.zeros_like(out), None))
+        torch.cuda.synchronize()
