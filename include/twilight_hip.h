@@ -574,15 +574,15 @@ int twl_kv_quant_read(void* k_out, void* v_out, int dtype, const int32_t* token_
  * max_tokens size the launch: prefix tokens beyond the first are not attended to, members of a group
  * beyond the second do not see the prefix, own tokens beyond the third are not attended to
  * (each <= 2^24, groups <= batch, max_group_size <= batch, batch * q heads <= 65535). A page id
- * that is not below num_pages is read as page num_pages - 1. kv_page_indices may be NULL where max_tokens
- * is 0, prefix_page_indices where max_prefix_tokens is 0.
+ * that is not below num_pages is read as page num_pages - 1. kv_page_indices may be NULL where
+ * max_tokens is 0, prefix_page_indices where max_prefix_tokens is 0.
  * Strides in elements, multiples of 8 (16-bit pages) or 16 (8-bit); token stride <= 2^24.
  * The softmax weights are rounded to the 16-bit type of the V product (dtype, or fp16 over 8-bit
  * pages); their sum is not. In fp16 a weight keeps its 11 bits down to 2^-26 of the row's largest one
  * (over 8-bit pages: weight times V scale, down to 2^-25 of the largest weight times the largest V
- * scale), and what lies below is off by up to 2^-37 (2^-36) of that. workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means
- * that the call needs none), 16-byte aligned, no initial contents required; calls that share it must
- * not overlap in time.
+ * scale), and what lies below is off by up to 2^-37 (2^-36) of that.
+ * workspace: at least twl_prefix_attn_workspace_bytes(...) bytes (0 means that the call needs none),
+ * 16-byte aligned, no initial contents required; calls that share it must not overlap in time.
  * ------------------------------------------------------------------------------------------- */
 uint64_t twl_prefix_attn_workspace_bytes(uint32_t batch, uint32_t num_q_heads,
                                          uint32_t num_kv_heads, uint32_t groups,
@@ -614,9 +614,9 @@ int twl_prefix_attn(const void* q, void* out, int dtype, const void* k_cache, co
  *   kept w exceeds u times the sum of all kept w.
  * temperature <= 0 (or NaN in an array): the best token. -inf and NaN logits are never drawn; a row
  * with nothing else gives -1. w is computed in 64 bits and held as a multiple of 2^-45 in integers,
- * whose sums are exact: a row's token does not depend on the other rows or on their number. workspace: at least twl_sample_tokens_workspace_bytes(rows, vocab)
- * bytes, 8-byte aligned, no initial contents required; calls that share it must not overlap in
- * time. rows <= 65535.
+ * whose sums are exact: a row's token does not depend on the other rows or on their number.
+ * workspace: at least twl_sample_tokens_workspace_bytes(rows, vocab) bytes, 8-byte aligned, no initial
+ * contents required; calls that share it must not overlap in time. rows <= 65535.
  * ------------------------------------------------------------------------------------------- */
 uint64_t twl_sample_tokens_workspace_bytes(uint32_t rows, uint32_t vocab);
 int twl_sample_tokens(const void* logits, int dtype, uint64_t row_stride, uint32_t rows,

@@ -141,7 +141,8 @@ def quant_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache
     :func:`group_paged_decode_attention`.
 
     ``q`` [B,H,128] fp16 / bf16; ``k_cache`` / ``v_cache`` [pages,16,Hkv,128] int8 or float8_e4m3fn with
-    ``k_scale`` / ``v_scale`` fp32 [pages,16,Hkv]; any H that is a multiple of Hkv. ``max_tokens`` bounds
+    ``k_scale`` / ``v_scale`` fp32 [pages,16,Hkv]; any H that is a multiple of Hkv,
+    up to 65535 rows B * H. ``max_tokens`` bounds
     the requests' lengths (tokens beyond it are not attended to). Returns ``out`` [B,H,128] in q's
     dtype (and ``lse`` fp32 [B,H]); a request without tokens gives zeros and -inf. ``workspace``: a
     uint8 tensor of :func:`prefix_attention_workspace_bytes` (..., 0, 0, 0, max_tokens) bytes that
